@@ -406,6 +406,53 @@ int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void*
 int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64_t H, int dtype,
                        awq_stream_t stream);
 
+/* ---- low-rank adapters beside a projection -----------------------------------
+ * Adapters of many requests on one projection's output, in one call for the
+ * whole batch.  Row m names adapter e(m); with the adapter's rank r <= max_rank
+ * and the projection's `parts` column parts (q, k, v of a fused qkv; gate, up),
+ *   v[p, j]  = sum_k x[m, k] * a[e][p * max_rank + j, k]
+ *   y'[m, n] = y[m, n] + scaling[e] * sum_{j < r} v[part of n, j] * b[e][n, j]
+ * in fp32 and rounded once; rows that name none keep y.  No counterpart in the
+ * reference.
+ *
+ * awq_lora_route sorts the rows by adapter (stable) into 16-row blocks; one
+ * call serves every projection of the step.  Ids outside [0, num_adapters)
+ * name no adapter.
+ *   adapter_ids [M]
+ *   sorted_ids[awq_moe_sorted_capacity(M, num_adapters + 1, 16)]  rows, M in padding
+ *   block_adapters[awq_moe_block_capacity(M, num_adapters + 1, 16)]
+ *       adapter of each block, num_adapters: none, -1 past the last block
+ *   num_rows_post_pad[1], adapter_offsets[num_adapters + 2] (padded bucket starts)
+ *
+ * awq_lora_add
+ *   y      [M, N], x [M, K] (the projection's output and input)
+ *   a      [num_adapters, parts * max_rank, K], b [num_adapters, N, max_rank]:
+ *          finite; the rows of a and columns of b at and past an adapter's rank
+ *          are not read as values
+ *   scaling, ranks [num_adapters] (a rank above max_rank counts as max_rank,
+ *          one of 0 or less adds nothing)
+ *   part_cols [parts], on the host: columns of each part, in order
+ *   activation 0: out [M, N], which may be y itself (rows without an adapter are
+ *          then not touched); AWQ_ACT_SILU / AWQ_ACT_GELU: parts are gate and up
+ *          of equal width and out [M, N / 2] = act(y'_gate) * y'_up for every row
+ *   N, K, max_rank and every part multiples of 8; y, x, a, b, out 16-byte aligned
+ *   ws     awq_lora_workspace_bytes bytes, 16-byte aligned, any content
+ * Limits: num_adapters <= AWQ_LORA_MAX_ADAPTERS, max_rank <= AWQ_LORA_MAX_RANK,
+ * parts <= AWQ_LORA_MAX_PARTS, M < 2^24; x, one adapter's a and one adapter's b
+ * below 2 GiB each. */
+#define AWQ_LORA_MAX_ADAPTERS 511
+#define AWQ_LORA_MAX_RANK 256
+#define AWQ_LORA_MAX_PARTS 4
+int awq_lora_route(const int32_t* adapter_ids, int64_t M, int64_t num_adapters, int32_t* sorted_ids,
+                   int32_t* block_adapters, int32_t* num_rows_post_pad, int32_t* adapter_offsets,
+                   awq_stream_t stream);
+int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts);
+int awq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling,
+                 const int32_t* ranks, void* out, int64_t M, int64_t N, int64_t K, int64_t num_adapters,
+                 int64_t max_rank, int parts, const int64_t* part_cols, int dtype, int activation,
+                 const int32_t* sorted_ids, const int32_t* block_adapters, void* ws, int64_t ws_bytes,
+                 awq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

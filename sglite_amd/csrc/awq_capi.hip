@@ -80,6 +80,7 @@ int check_shape(int64_t K, int64_t N, int64_t G, int dtype, int64_t* G_out) {
 // given (else a second kernel sums the k-slices); the others need them.
 constexpr int64_t counter_bytes_for(int64_t N) { return kFixupBytes + ((N + 15) / 16) * 4; }
 static_assert(AWQ_COUNTER_TILE_BYTES == kFixupBytes, "header and kernels agree on the tile counters");
+static_assert(AWQ_LORA_MAX_PARTS == kLoraParts, "header and kernels agree on the parts of a projection");
 static_assert(AWQ_MLP_COUNTER_BYTES == kMlpCounterBytes && AWQ_MLP_DEFAULT_POLLS == kMlpDefaultPolls,
               "header and kernel agree on the gated MLP counters");
 
@@ -786,6 +787,119 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
   if (!aligned(in, 16) || !aligned(out, 16))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_sum_reduce: in and out must be 16-byte aligned");
   return hip_status(launch_moe_sum(in, out, T, topk, H, dtype, (hipStream_t)stream), "awq_moe_sum_reduce launch");
+}
+
+int awq_lora_route(const int32_t* adapter_ids, int64_t M, int64_t num_adapters, int32_t* sorted_ids,
+                   int32_t* block_adapters, int32_t* num_rows_post_pad, int32_t* adapter_offsets,
+                   awq_stream_t stream) {
+  const TraceRange range("awq_lora_route");
+  if (num_adapters < 1 || num_adapters > AWQ_LORA_MAX_ADAPTERS)
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_route: num_adapters must be in [1, %d], got %lld",
+                AWQ_LORA_MAX_ADAPTERS, (long long)num_adapters);
+  if (M < 0 || M >= (int64_t(1) << 24))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_route: M must be in [0, 2^24), got %lld", (long long)M);
+  if ((M > 0 && !adapter_ids) || !sorted_ids || !block_adapters || !num_rows_post_pad || !adapter_offsets)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_route: null pointer argument");
+  return hip_status(launch_lora_route(adapter_ids, M, num_adapters, sorted_ids, block_adapters, num_rows_post_pad,
+                                      adapter_offsets, (hipStream_t)stream),
+                    "awq_lora_route launch");
+}
+
+namespace {
+
+int check_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int parts, const char* who) {
+  if (M < 0 || N <= 0 || K <= 0 || R <= 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: M >= 0 and positive N, K, max_rank required", who);
+  if (N % 8 != 0 || K % 8 != 0 || R % 8 != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT,
+                "%s: N, K and max_rank must be multiples of 8 (N=%lld, K=%lld, max_rank=%lld)", who, (long long)N,
+                (long long)K, (long long)R);
+  if (parts < 1 || parts > AWQ_LORA_MAX_PARTS)
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: the projection must have 1 to %d parts, got %d", who, AWQ_LORA_MAX_PARTS,
+                parts);
+  if (R > AWQ_LORA_MAX_RANK)
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: max_rank must be at most %d, got %lld", who, AWQ_LORA_MAX_RANK,
+                (long long)R);
+  if (L < 1 || L > AWQ_LORA_MAX_ADAPTERS)
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: num_adapters must be in [1, %d], got %lld", who, AWQ_LORA_MAX_ADAPTERS,
+                (long long)L);
+  // Row and weight offsets inside one buffer range are 32-bit, past-the-end ones bit 31.
+  const int64_t lim = int64_t(1) << 31;
+  if (M >= (int64_t(1) << 24) || K >= (int64_t(1) << 24) || N >= (int64_t(1) << 30) || M * K * 2 >= lim ||
+      parts * R * K * 2 >= lim || N * R * 2 >= lim)
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: x, one adapter's A and one adapter's B must each span below 2 GiB", who);
+  // Workgroups of the expand: 256 columns (128 gated) by 16 rows, a launch dimension below 2^24 of them.
+  if ((N / 128 + parts) * (M / 16 + L + 1) >= (int64_t(1) << 24))
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: M * N must be below 2^35", who);
+  return AWQ_STATUS_OK;
+}
+
+}  // namespace
+
+int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts) {
+  const int st = check_lora(M, N, K, num_adapters, max_rank, parts, "awq_lora_workspace_bytes");
+  if (st != 0) return st;
+  ok();
+  return M == 0 ? 0 : plan_lora(M, K, num_adapters, max_rank, parts).ws_bytes;
+}
+
+int awq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling,
+                 const int32_t* ranks, void* out, int64_t M, int64_t N, int64_t K, int64_t num_adapters,
+                 int64_t max_rank, int parts, const int64_t* part_cols, int dtype, int activation,
+                 const int32_t* sorted_ids, const int32_t* block_adapters, void* ws, int64_t ws_bytes,
+                 awq_stream_t stream) {
+  const TraceRange range("awq_lora_add");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: dtype must be 0 or 1, got %d", dtype);
+  const int st = check_lora(M, N, K, num_adapters, max_rank, parts, "awq_lora_add");
+  if (st != 0) return st;
+  if (activation != 0 && activation != AWQ_ACT_SILU && activation != AWQ_ACT_GELU)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: unknown activation %d", activation);
+  if (!part_cols) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: null pointer argument");
+  int64_t cols = 0;
+  for (int i = 0; i < parts; ++i) {
+    if (part_cols[i] <= 0 || part_cols[i] % 8 != 0 || part_cols[i] > N)
+      return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: part %d has %lld columns: a positive multiple of 8 needed",
+                  i, (long long)part_cols[i]);
+    cols += part_cols[i];
+  }
+  if (cols != N)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: the parts' columns sum to %lld, not N=%lld",
+                (long long)cols, (long long)N);
+  if (activation != 0 && (parts != 2 || part_cols[0] != part_cols[1]))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: an activation needs two equal parts, gate and up");
+  if (M == 0) return ok();
+  if (!y || !x || !a || !b || !scaling || !ranks || !out || !sorted_ids || !block_adapters)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: null pointer argument");
+  if (!aligned(y, 16) || !aligned(x, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(out, 16))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: y, x, a, b and out must be 16-byte aligned");
+  if (activation != 0 && out == y)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: with an activation out must not be y");
+  const int64_t need = plan_lora(M, K, num_adapters, max_rank, parts).ws_bytes;
+  if (!ws || ws_bytes < need || !aligned(ws, 16))
+    return fail(AWQ_STATUS_WORKSPACE, "awq_lora_add: a 16-byte aligned workspace of %lld bytes needed, %lld given",
+                (long long)need, (long long)ws_bytes);
+  LoraParams p{};
+  p.y = y;
+  p.x = x;
+  p.a = a;
+  p.b = b;
+  p.scaling = scaling;
+  p.ranks = ranks;
+  p.out = out;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.L = num_adapters;
+  p.R = max_rank;
+  p.parts = parts;
+  p.part_cols = part_cols;
+  p.act = activation;
+  p.dtype = dtype;
+  p.sorted = sorted_ids;
+  p.bucket = block_adapters;
+  p.ws = (float*)ws;
+  return hip_status(launch_lora(p, (hipStream_t)stream), "awq_lora_add launch");
 }
 
 }  // extern "C"

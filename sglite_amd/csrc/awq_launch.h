@@ -155,6 +155,39 @@ int plan_threads(const GemmPlan& p);
 
 hipError_t launch_moe_sum(const void* in, void* out, int64_t T, int64_t k, int64_t H, int dtype, hipStream_t s);
 
+// Low-rank adapters beside a projection (awq_lora.hip).
+constexpr int kLoraBlock = 16;    // rows of a block of the sorted table
+constexpr int kLoraParts = 4;     // column parts of a projection, at most
+constexpr int kLoraColTiles = 4;  // 16-column tiles of a wave of the expand
+struct LoraPlan {
+  int64_t blocks;  // 16-row blocks the grids cover
+  int row_tiles;   // of a workgroup of the shrink
+  int rank_tiles;  // ... and its 16-rank tiles
+  int slices;      // k-slices of the shrink, summed by the expand
+  int per;         // row blocks that a workgroup of the expand takes in turn
+  int64_t ws_bytes;
+};
+LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts);
+hipError_t launch_lora_route(const int32_t* ids, int64_t n, int64_t L, int32_t* sorted, int32_t* bucket,
+                             int32_t* num_post_pad, int32_t* offsets, hipStream_t s);
+struct LoraParams {
+  const void* y;
+  const void* x;
+  const void* a;
+  const void* b;
+  const float* scaling;
+  const int32_t* ranks;
+  void* out;
+  int64_t M, N, K, L, R;
+  int parts;
+  const int64_t* part_cols;
+  int act, dtype;
+  const int32_t* sorted;  // from launch_lora_route
+  const int32_t* bucket;
+  float* ws;
+};
+hipError_t launch_lora(const LoraParams& p, hipStream_t s);
+
 // Gated MLP block in one launch (awq_mlp.hip).  Counters: 128-byte slots of
 // 32 words; word 2 of slot 0 counts workgroups that gave up waiting, slot
 // 1 + s is k-slice s's barrier, slot 1 + S + g column group g's.

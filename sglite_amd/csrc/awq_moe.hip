@@ -179,6 +179,8 @@ struct AlignLds {
   int wtot[kAlignWaves];
 };
 
+// STRAYS: ids outside [0, E - 1) count as expert E - 1 instead of being dropped.
+template <bool STRAYS = false>
 __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restrict__ ids, int n, int E, int bs,
                                            int32_t* __restrict__ sorted, int32_t* __restrict__ expert_ids,
                                            int blocks_cap, int32_t* __restrict__ num_post_pad,
@@ -203,6 +205,7 @@ __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restr
     for (int r = 0; r < kAlignBatch; ++r) {
       const int i = b0 + r * 64 + lane;
       er[r] = i < r1 ? ids[i] : -1;
+      if (STRAYS && i < r1 && (uint32_t)er[r] >= (uint32_t)E) er[r] = E - 1;
     }
   };
   const bool one_batch = chunk <= 64 * kAlignBatch;  // the ids stay in registers between the passes
@@ -295,6 +298,16 @@ __global__ __launch_bounds__(kAlignThreads) void align_kernel(const int32_t* __r
                                                               int32_t* __restrict__ offsets) {
   __shared__ AlignLds lds;
   align_rows(lds, ids, n, E, bs, sorted, expert_ids, blocks_cap, num_post_pad, offsets);
+}
+
+// The rows of a batch by their adapters: expert E - 1 takes those that name none.
+__global__ __launch_bounds__(kAlignThreads) void lora_route_kernel(const int32_t* __restrict__ ids, int n, int E,
+                                                                   int bs, int32_t* __restrict__ sorted,
+                                                                   int32_t* __restrict__ expert_ids, int blocks_cap,
+                                                                   int32_t* __restrict__ num_post_pad,
+                                                                   int32_t* __restrict__ offsets) {
+  __shared__ AlignLds lds;
+  align_rows<true>(lds, ids, n, E, bs, sorted, expert_ids, blocks_cap, num_post_pad, offsets);
 }
 
 // Routing and alignment of a decode batch in one launch: each wave of one
@@ -892,6 +905,13 @@ hipError_t launch_moe_align(const int32_t* ids, int64_t n, int64_t E, int64_t bs
                             int32_t* num_post_pad, int32_t* offsets, hipStream_t s) {
   hipLaunchKernelGGL(align_kernel, dim3(1), dim3(kAlignThreads), 0, s, ids, (int)n, (int)E, (int)bs, sorted, expert_ids,
                      (int)moe_block_capacity(n, E, bs), num_post_pad, offsets);
+  return hipGetLastError();
+}
+
+hipError_t launch_lora_route(const int32_t* ids, int64_t n, int64_t L, int32_t* sorted, int32_t* bucket,
+                             int32_t* num_post_pad, int32_t* offsets, hipStream_t s) {
+  hipLaunchKernelGGL(lora_route_kernel, dim3(1), dim3(kAlignThreads), 0, s, ids, (int)n, (int)(L + 1), kLoraBlock,
+                     sorted, bucket, (int)moe_block_capacity(n, L + 1, kLoraBlock), num_post_pad, offsets);
   return hipGetLastError();
 }
 

@@ -80,8 +80,11 @@ class GatedMLP:
         if self._mlp_counters is not None:
             ops.mlp_check(self._mlp_counters)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        one = self._one_launch_weights(x)
+    def forward(self, x: torch.Tensor, adapters: Optional[ops.LoraBatch] = None) -> torch.Tensor:
+        """``adapters``: a step's ``ops.lora_route``, for projections that hold adapter slots."""
+        if self.gate_up_proj._lora is None and self.down_proj._lora is None:
+            adapters = None
+        one = self._one_launch_weights(x) if adapters is None else None
         if one is not None:
             gu, dn, H, I, G = one
             if self._mlp_counters is None or self._mlp_counters.device != x.device:
@@ -91,6 +94,6 @@ class GatedMLP:
             if self.down_proj._tp_size > 1:
                 torch.distributed.all_reduce(y, group=self.down_proj._group)
             return y
-        return self.down_proj.forward(self.gate_up_proj.forward_act(x, self.hidden_act))
+        return self.down_proj.forward(self.gate_up_proj.forward_act(x, self.hidden_act, adapters), adapters)
 
     __call__ = forward

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from typing import Dict, Iterator, List, NamedTuple, Optional, Tuple
+from typing import Dict, Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -1013,8 +1013,236 @@ def moe_sum_reduce(inp: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     return out
 
 
+# ---------------------------------------------------------------------------
+# Low-rank adapters of many requests beside a projection (awq_lora_add).
+# ---------------------------------------------------------------------------
+
+LORA_MAX_ADAPTERS = _lib.AWQ_LORA_MAX_ADAPTERS
+LORA_MAX_RANK = _lib.AWQ_LORA_MAX_RANK
+
+
+class LoraStack(NamedTuple):
+    """The adapters of one projection, stacked over ``num_adapters`` slots.
+
+    ``a[e, p * max_rank + j]`` is row j of adapter e's A for column part p and ``b[e, n]`` row n of its B, so
+    a slot's values at and past its rank do not count.  Both must be finite."""
+    a: torch.Tensor        # [num_adapters, parts * max_rank, K]
+    b: torch.Tensor        # [num_adapters, N, max_rank]
+    scaling: torch.Tensor  # float32 [num_adapters]
+    ranks: torch.Tensor    # int32 [num_adapters]
+    parts: Tuple[int, ...]  # columns of each part, summing to N
+
+
+class LoraBatch(NamedTuple):
+    """A step's rows in the order of their adapters (``lora_route``)."""
+    sorted_ids: torch.Tensor      # int32, rows; the row count in padding
+    block_adapters: torch.Tensor  # int32, adapter of each 16-row block (num_adapters: none, -1: past the last)
+    offsets: torch.Tensor         # int32 [num_adapters + 2], padded bucket starts
+    rows: int
+    num_adapters: int
+
+
+def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[int], dtype: torch.dtype,
+                    device: torch.device) -> LoraStack:
+    """An empty stack (every slot of rank 0, which adds nothing)."""
+    dtype_code(dtype)
+    N = sum(parts)
+    return LoraStack(torch.zeros((num_adapters, len(parts) * max_rank, K), dtype=dtype, device=device),
+                     torch.zeros((num_adapters, N, max_rank), dtype=dtype, device=device),
+                     torch.zeros(num_adapters, dtype=torch.float32, device=device),
+                     torch.zeros(num_adapters, dtype=torch.int32, device=device), tuple(int(n) for n in parts))
+
+
+def _lora_route_launch(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    dev = adapter_ids.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _lora_route_launch(adapter_ids, num_adapters)
+    M = adapter_ids.numel()
+    cap = M + (num_adapters + 1) * 15  # awq_moe_sorted_capacity(M, num_adapters + 1, 16)
+    bcap = (cap + 15) // 16
+    # One allocation: sorted ids, block adapters, offsets, the padded row count.
+    n0, n1 = (cap + 3) // 4 * 4, (bcap + 3) // 4 * 4
+    buf = torch.empty(n0 + n1 + num_adapters + 3, dtype=torch.int32, device=dev)
+    sorted_ids, blocks = buf[:cap], buf[n0:n0 + bcap]
+    offsets = buf[n0 + n1:n0 + n1 + num_adapters + 2]
+    p = buf.data_ptr()
+    _lib.check(_lib.load().awq_lora_route(adapter_ids.data_ptr() if M else None, M, num_adapters, p, p + 4 * n0,
+                                          p + 4 * (n0 + n1 + num_adapters + 2), p + 4 * (n0 + n1), _stream(dev)),
+               "awq_lora_route")
+    return sorted_ids, blocks, offsets
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_lora_route", mutates_args=(), device_types="cuda")
+def _lora_route_op(adapter_ids: torch.Tensor,
+                   num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    # Outputs of a registered op are tensors of their own.
+    return tuple(t.clone() for t in _lora_route_launch(adapter_ids, num_adapters))
+
+
+@_lora_route_op.register_fake
+def _(adapter_ids, num_adapters):
+    cap = adapter_ids.numel() + (num_adapters + 1) * 15
+    return (adapter_ids.new_empty(cap), adapter_ids.new_empty((cap + 15) // 16),
+            adapter_ids.new_empty(num_adapters + 2))
+
+
+def lora_route(adapter_ids: torch.Tensor, num_adapters: int) -> LoraBatch:
+    """Sort a step's rows by adapter; one call serves every projection of the step.
+
+    ``adapter_ids`` [M] int32 names each row's slot; an id outside ``[0, num_adapters)``, as -1, names none."""
+    if adapter_ids.dim() != 1 or adapter_ids.dtype != torch.int32:
+        raise ValueError(f"adapter_ids must be int32 [M], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
+    if not 1 <= num_adapters <= _lib.AWQ_LORA_MAX_ADAPTERS:
+        raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
+    _require_cuda(adapter_ids)
+    ids = _aligned(adapter_ids, 4)
+    if _undispatched(ids):
+        t = _lora_route_launch(ids, num_adapters)
+    else:
+        t = torch.ops.sglite_awq.awq_lora_route(ids, num_adapters)
+    return LoraBatch(*t, ids.numel(), num_adapters)
+
+
+def _lora_launch(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                 ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor, out: torch.Tensor,
+                 parts: Sequence[int], act: int) -> None:
+    M, K = x.shape
+    if M == 0:
+        return
+    dev = x.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):  # the C ABI's planning fills the current device's CUs
+            return _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, out, parts, act)
+    L, N, R = b.shape
+    lib = _lib.load()
+    wsb = _lib.check(lib.awq_lora_workspace_bytes(M, N, K, L, R, len(parts)), "awq_lora_workspace_bytes")
+    ws = _workspace(wsb, dev)
+    cols = (ctypes.c_int64 * len(parts))(*parts)
+    _lib.check(lib.awq_lora_add(y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(),
+                                ranks.data_ptr(), out.data_ptr(), M, N, K, L, R, len(parts), cols,
+                                dtype_code(x.dtype), act, sorted_ids.data_ptr(), block_adapters.data_ptr(),
+                                ws.data_ptr(), wsb, _stream(dev)), "awq_lora_add")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_lora_add", mutates_args=(), device_types="cuda")
+def _lora_add_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                 ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor, parts: List[int],
+                 activation: str) -> torch.Tensor:
+    act = _ACT_CODE[_ACT_NAME[activation]]
+    out = torch.empty((y.shape[0], y.shape[1] // 2 if act else y.shape[1]), dtype=y.dtype, device=y.device)
+    _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, out, parts, act)
+    return out
+
+
+@_lora_add_op.register_fake
+def _(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, parts, activation):
+    return y.new_empty((y.shape[0], y.shape[1] if activation == "none" else y.shape[1] // 2))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_lora_add_", mutates_args=("y",), device_types="cuda")
+def _lora_add_inplace_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                         ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor,
+                         parts: List[int]) -> None:
+    _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, y, parts, 0)
+
+
+@_lora_add_inplace_op.register_fake
+def _(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, parts):
+    return None
+
+
+def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch,
+                activation: Optional[str]) -> None:
+    a, b = stack.a, stack.b
+    if a.dim() != 3 or b.dim() != 3:
+        raise ValueError("a must be [adapters, parts * max_rank, K] and b [adapters, N, max_rank]")
+    L, N, R = b.shape
+    P, K = len(stack.parts), a.shape[2]
+    if tuple(a.shape) != (L, P * R, K):
+        raise ValueError(f"a must be {(L, P * R, K)} beside b {tuple(b.shape)} with {P} parts, got {tuple(a.shape)}")
+    if sum(stack.parts) != N:
+        raise ValueError(f"the parts {stack.parts} do not sum to the {N} columns of b")
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be [M, {K}], got {tuple(x.shape)}")
+    M = x.shape[0]
+    if tuple(y.shape) != (M, N):
+        raise ValueError(f"y must be {(M, N)}, got {tuple(y.shape)}")
+    dtype_code(x.dtype)
+    if not (x.dtype == y.dtype == a.dtype == b.dtype):
+        raise ValueError(f"y, x, a and b must share a dtype, got {y.dtype}, {x.dtype}, {a.dtype}, {b.dtype}")
+    if stack.scaling.dtype != torch.float32 or tuple(stack.scaling.shape) != (L,):
+        raise ValueError(f"scaling must be float32 [{L}]")
+    if stack.ranks.dtype != torch.int32 or tuple(stack.ranks.shape) != (L,):
+        raise ValueError(f"ranks must be int32 [{L}]")
+    for t in (a, b, stack.scaling, stack.ranks):
+        if not t.is_contiguous() or t.data_ptr() % (16 if t.dtype == x.dtype else 4):
+            raise ValueError("the stack's tensors must be contiguous (a and b 16-byte aligned)")
+    dev = x.device
+    for t in (y, a, b, stack.scaling, stack.ranks, batch.sorted_ids, batch.block_adapters):
+        if t.device != dev:
+            raise ValueError("y, x, the stack and the batch must be on one device")
+    if batch.rows != M or batch.num_adapters != L:
+        raise ValueError(f"the batch was routed for {batch.rows} rows and {batch.num_adapters} adapters, "
+                         f"not {M} and {L}")
+    if activation is not None:
+        if activation not in _GATED_ACT:
+            raise ValueError(f"unsupported activation {activation!r}")
+        if P != 2 or stack.parts[0] != stack.parts[1]:
+            raise ValueError(f"an activation needs two equal parts, gate and up, got {stack.parts}")
+    _require_cuda(y, x, a, b, stack.scaling, stack.ranks, batch.sorted_ids, batch.block_adapters)
+
+
+def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the address ranges that two tensors' elements span meet."""
+    if s.numel() == 0 or t.numel() == 0:
+        return False
+
+    def end(v: torch.Tensor) -> int:
+        return v.data_ptr() + (sum((n - 1) * st for n, st in zip(v.shape, v.stride())) + 1) * v.element_size()
+    return s.data_ptr() < end(t) and t.data_ptr() < end(s)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch, activation: Optional[str] = None,
+             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y + scaling * B (A x)`` of every row's adapter, summed in fp32 and rounded once, on x's current stream.
+
+    ``y`` [M, N] is the projection's output for ``x`` [M, K]; rows that name no adapter keep it.  ``out`` may be
+    ``y`` itself: then only rows with an adapter are written.  With ``activation`` ("silu" or "gelu") the two
+    parts are gate and up and the result is ``act(gate) * up``, [M, N / 2], for every row (``out`` is not taken)."""
+    _check_lora(y, x, stack, batch, activation)
+    if out is not None:
+        if activation is not None:
+            raise ValueError("out is not taken with an activation")
+        _check_out(out, tuple(y.shape), y.dtype, y.device)
+        if out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        if _overlap(out, x) or (_overlap(out, y) and (out.data_ptr() != y.data_ptr() or not y.is_contiguous())):
+            raise ValueError("out must not share memory with x, nor with y unless it is y")
+    x = _aligned(x)
+    a, b, scaling, ranks = stack.a, stack.b, stack.scaling, stack.ranks
+    tables = (batch.sorted_ids, batch.block_adapters)
+    if out is not None:
+        if out.data_ptr() != y.data_ptr():
+            out.copy_(y)
+        if _undispatched(out, x, a, b, scaling, ranks, *tables):
+            _lora_launch(out, x, a, b, scaling, ranks, *tables, out, stack.parts, 0)
+        else:
+            torch.ops.sglite_awq.awq_lora_add_(out, x, a, b, scaling, ranks, *tables, list(stack.parts))
+        return out
+    y = _aligned(y)
+    if _undispatched(y, x, a, b, scaling, ranks, *tables):
+        act = _ACT_CODE[activation]
+        out = torch.empty((y.shape[0], y.shape[1] // 2 if act else y.shape[1]), dtype=y.dtype, device=y.device)
+        _lora_launch(y, x, a, b, scaling, ranks, *tables, out, stack.parts, act)
+        return out
+    return torch.ops.sglite_awq.awq_lora_add(y, x, a, b, scaling, ranks, *tables, list(stack.parts),
+                                             "none" if activation is None else activation)
+
+
 REGISTERED_OPS: List[str] = [
     "awq_repack_cdna4", "awq_unrepack_cdna4", "awq_dequant", "awq_dequant_repacked", "awq_w4a16_gemm",
     "awq_w4a16_gemm_out", "awq_w4a16_gemm_act", "awq_w4a16_gemm_act_out", "awq_repack_experts",
     "awq_moe_topk_softmax", "awq_moe_align_block_size", "awq_moe_route", "awq_moe_w4a16_gemm", "awq_moe_sum_reduce",
+    "awq_lora_route", "awq_lora_add", "awq_lora_add_",
 ]
