@@ -400,6 +400,24 @@ int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void*
                        const int32_t* expert_offsets, const float* topk_weights, int64_t num_routed, int64_t top_k,
                        int activation, int mul_routed_weight, void* out, awq_stream_t stream);
 
+/* The same product for dense (fp16 or bf16) experts; replaces fused_moe_kernel
+ * (python/sglite/kernels/triton/fused_moe.py:54-183) for the weights that the
+ * reference's backend holds.
+ *   a        [a_rows, K]; routed row r reads activation row r / top_k
+ *   w        [E, N, K], each expert's rows contiguous
+ *   out      activation == AWQ_MOE_ACT_NONE: [num_routed, N]
+ *            activation != NONE: N = 2I (gate rows first, then up) ->
+ *            act(gate) * up, [num_routed, I], I % 8 == 0
+ *   mul_routed_weight: multiply each sum by topk_weights[r] first
+ * All in fp32, rounded once (gate and up are not rounded before the
+ * activation).  Rows that the sorted table does not hold are not written.
+ * N % 8 == 0, K % 8 == 0; a, w, out 16-byte aligned; E <= 512; the routed
+ * activation rows and one expert's weights below 2 GiB each. */
+int awq_moe_dense_gemm(const void* a, int64_t a_rows, const void* w, int64_t E, int64_t N, int64_t K, int dtype,
+                       const int32_t* sorted_ids, int64_t sorted_cap, const int32_t* expert_offsets,
+                       const float* topk_weights, int64_t num_routed, int64_t top_k, int activation,
+                       int mul_routed_weight, void* out, awq_stream_t stream);
+
 /* out[t, :] = rnd(sum_j in[t, j, :]) with an fp32 sum; replaces
  * moe_sum_reduce_triton (python/sglite/kernels/moe_triton.py:68-102).
  * H % 8 == 0; in and out 16-byte aligned. */

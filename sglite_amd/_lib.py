@@ -74,6 +74,8 @@ SIGNATURES = {
     "awq_moe_route": (_int, [_vp, _int, _i64, _i64, _i64, _int, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "awq_moe_w4a16_gemm": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64,
                                   _i64, _int, _int, _vp, _vp]),
+    "awq_moe_dense_gemm": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64, _int, _int,
+                                  _vp, _vp]),
     "awq_moe_sum_reduce": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "awq_lora_route": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "awq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),

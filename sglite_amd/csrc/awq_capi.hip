@@ -773,6 +773,59 @@ int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void*
   return hip_status(launch_moe_gemm(p, (hipStream_t)stream), "awq_moe_w4a16_gemm launch");
 }
 
+int awq_moe_dense_gemm(const void* a, int64_t a_rows, const void* w, int64_t E, int64_t N, int64_t K, int dtype,
+                       const int32_t* sorted_ids, int64_t sorted_cap, const int32_t* expert_offsets,
+                       const float* topk_weights, int64_t num_routed, int64_t top_k, int activation,
+                       int mul_routed_weight, void* out, awq_stream_t stream) {
+  const TraceRange range("awq_moe_dense_gemm");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: dtype must be 0 or 1, got %d", dtype);
+  if (N <= 0 || K <= 0 || N % 8 != 0 || K % 8 != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: N and K must be positive multiples of 8 (N=%lld, K=%lld)",
+                (long long)N, (long long)K);
+  if (E <= 0 || E > 512)
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_moe_dense_gemm: E must be in [1, 512], got %lld", (long long)E);
+  if (activation != AWQ_MOE_ACT_NONE && activation != AWQ_MOE_ACT_SILU && activation != AWQ_MOE_ACT_GELU)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: unknown activation %d", activation);
+  if (activation != AWQ_MOE_ACT_NONE && N % 16 != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT,
+                "awq_moe_dense_gemm: gate/up pairing needs N = 2I with I %% 8 == 0, got N=%lld", (long long)N);
+  if (top_k <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: top_k must be positive");
+  if (num_routed < 0 || num_routed >= (int64_t(1) << 24) || sorted_cap < 0 || sorted_cap >= (int64_t(1) << 30))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_moe_dense_gemm: num_routed must be below 2^24 and sorted_cap below 2^30");
+  const int64_t rows = (num_routed + top_k - 1) / top_k, lim = int64_t(1) << 31;
+  if (rows > a_rows)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT,
+                "awq_moe_dense_gemm: %lld routed rows with top_k %lld need %lld activation rows, a has %lld",
+                (long long)num_routed, (long long)top_k, (long long)rows, (long long)a_rows);
+  // Offsets inside one buffer range are 32-bit, past-the-end ones bit 31.
+  if (K >= lim / 2 || rows * K * 2 >= lim || N >= lim / 2 || N * K * 2 >= lim)
+    return fail(AWQ_STATUS_UNSUPPORTED,
+                "awq_moe_dense_gemm: the routed activation rows and one expert's weights must each span below 2 GiB");
+  if (num_routed == 0 || sorted_cap == 0) return ok();
+  if (!a || !w || !sorted_ids || !expert_offsets || !out || (mul_routed_weight && !topk_weights))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: null pointer argument");
+  if (!aligned(a, 16) || !aligned(w, 16) || !aligned(out, 16))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: a, w and out must be 16-byte aligned");
+  MoeDenseParams p{};
+  p.x = a;
+  p.w = w;
+  p.sorted = sorted_ids;
+  p.offsets = expert_offsets;
+  p.topk_w = topk_weights;
+  p.out = out;
+  p.E = E;
+  p.N = N;
+  p.K = K;
+  p.a_div = top_k;
+  p.num_routed = num_routed;
+  p.sorted_cap = sorted_cap;
+  p.act = activation;
+  p.mul_rw = mul_routed_weight ? 1 : 0;
+  p.dtype = dtype;
+  return hip_status(launch_moe_dense(p, (hipStream_t)stream), "awq_moe_dense_gemm launch");
+}
+
 int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64_t H, int dtype,
                        awq_stream_t stream) {
   const TraceRange range("awq_moe_sum_reduce");

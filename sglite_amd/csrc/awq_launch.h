@@ -155,6 +155,21 @@ int plan_threads(const GemmPlan& p);
 
 hipError_t launch_moe_sum(const void* in, void* out, int64_t T, int64_t k, int64_t H, int dtype, hipStream_t s);
 
+// Grouped products of dense experts (awq_moe_dense.hip).
+struct MoeDenseParams {
+  const void* x;           // activation rows
+  const void* w;           // [E, N, K]
+  const int32_t* sorted;   // from launch_moe_align
+  const int32_t* offsets;  // padded bucket offsets [E + 1]
+  const float* topk_w;     // routed weights [num_routed]
+  void* out;
+  int64_t E, N, K, a_div, num_routed, sorted_cap;
+  int act;     // 0 plain, 1 silu, 2 gelu (gate and up halves of N)
+  int mul_rw;  // multiply the sums by the routed weight
+  int dtype;
+};
+hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s);
+
 // Low-rank adapters beside a projection (awq_lora.hip).
 constexpr int kLoraBlock = 16;    // rows of a block of the sorted table
 constexpr int kLoraParts = 4;     // column parts of a projection, at most

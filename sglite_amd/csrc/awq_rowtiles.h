@@ -1,0 +1,64 @@
+// Tiles of consecutive sorted rows of one expert, counted over the experts'
+// buckets in order.
+#pragma once
+
+#include "awq_device.h"
+
+namespace sgl_awq {
+
+// One lane per EPL (2 or 8) experts; every wave of a workgroup finds its tiles
+// by itself.  Offsets are clamped to the sorted table, whatever they hold.
+template <int EPL>
+struct RowTiles {
+  int r0[EPL], nr[EPL];  // first sorted row and rows of the lane's experts
+  int excl, incl;        // tiles before the lane's first expert and past its last one
+
+  __device__ __forceinline__ void scan(const int32_t* offsets, int E, int sorted_cap, int tile_rows, int lane) {
+    int o[EPL + 1];
+#pragma unroll
+    for (int i = 0; i <= EPL; ++i) o[i] = offsets[min(lane * EPL + i, E)];
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      r0[i] = min(max(o[i], 0), sorted_cap);
+      const int r1 = min(max(o[i + 1], r0[i]), sorted_cap);
+      nr[i] = lane * EPL + i < E ? r1 - r0[i] : 0;
+      sum += (nr[i] + tile_rows - 1) / tile_rows;
+    }
+    incl = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int u = __shfl_up(incl, d);
+      if (lane >= d) incl += u;
+    }
+    excl = incl - sum;
+  }
+
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, 63); }
+
+  // Tile t's expert, first sorted row and rows (at most tile_rows); e = -1 past the last tile.
+  __device__ __forceinline__ void find(int t, int tile_rows, int lane, int& e, int& rb, int& rows) const {
+    const uint64_t hit = __ballot(t >= excl && t < incl);
+    if (hit == 0) {
+      e = -1;
+      return;
+    }
+    int fe = 0, fb = 0, fn = 0, pos = excl;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int n = (nr[i] + tile_rows - 1) / tile_rows;
+      if (t >= pos && t < pos + n) {
+        fe = lane * EPL + i;
+        fb = r0[i] + (t - pos) * tile_rows;
+        fn = min(tile_rows, r0[i] + nr[i] - fb);
+      }
+      pos += n;
+    }
+    const int src = __builtin_ctzll(hit);
+    e = __builtin_amdgcn_readlane(fe, src);
+    rb = __builtin_amdgcn_readlane(fb, src);
+    rows = __builtin_amdgcn_readlane(fn, src);
+  }
+};
+
+}  // namespace sgl_awq

@@ -1,19 +1,19 @@
-"""Grouped W4A16 MoE backend (AWQ experts on the gfx950 engine).
+"""Grouped MoE backends (AWQ W4A16 and dense experts on the gfx950 engine).
 
 Mirrors the fused MoE backend interface of
 python/sglite/srt/model_executor/layers/fused_moe/ (registry __init__.py:22-35,
-BaseMoeBackend base.py:8-26, FusedMoe fused.py:205-233) with AWQ expert stacks
-in place of the dense ``[E, 2I, H]`` / ``[E, H, I]`` weights.
+BaseMoeBackend base.py:8-26, FusedMoe fused.py:205-233): ``fused`` over dense
+``[E, 2I, H]`` / ``[E, H, I]`` weights, ``awq_fused`` over AWQ expert stacks.
 """
 
 from __future__ import annotations
 
 from typing import Callable, Dict
 
-from .fused import (AWQFusedMoe, AWQMoeWeights, BaseMoeBackend, fused_experts_impl, fused_topk, get_default_config,
-                    moe_align_block_size, process_awq_moe_weights)
+from .fused import (AWQFusedMoe, AWQMoeWeights, BaseMoeBackend, FusedMoe, fused_experts_impl, fused_topk,
+                    get_default_config, moe_align_block_size, process_awq_moe_weights)
 
-SUPPORTED_MOE_BACKENDS: Dict[str, Callable[[], BaseMoeBackend]] = {"awq_fused": AWQFusedMoe}
+SUPPORTED_MOE_BACKENDS: Dict[str, Callable[[], BaseMoeBackend]] = {"awq_fused": AWQFusedMoe, "fused": FusedMoe}
 
 
 def create_moe_backend(backend: str) -> BaseMoeBackend:
@@ -24,7 +24,7 @@ def create_moe_backend(backend: str) -> BaseMoeBackend:
         raise ValueError(f"unknown MoE backend {backend!r}; registered: {sorted(SUPPORTED_MOE_BACKENDS)}") from None
 
 
-from .layer import AWQExpertStack, AWQMoELayer  # noqa: E402  (the layer resolves backends by name)
+from .layer import AWQExpertStack, AWQMoELayer, MoELayer  # noqa: E402  (the layer resolves backends by name)
 
 __all__ = [
     "AWQExpertStack",
@@ -32,6 +32,8 @@ __all__ = [
     "AWQMoELayer",
     "AWQMoeWeights",
     "BaseMoeBackend",
+    "FusedMoe",
+    "MoELayer",
     "SUPPORTED_MOE_BACKENDS",
     "create_moe_backend",
     "fused_experts_impl",

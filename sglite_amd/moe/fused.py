@@ -1,4 +1,4 @@
-"""Fused MoE forward with AWQ W4A16 experts.
+"""Fused MoE forward with AWQ W4A16 or dense (fp16 / bf16) experts.
 
 Follows python/sglite/srt/model_executor/layers/fused_moe/fused.py:
   fused_topk            fused.py:11-31   (topk_softmax + renormalise)
@@ -15,7 +15,7 @@ weight into the second's.
 from __future__ import annotations
 
 from abc import ABC, abstractmethod
-from typing import Dict, NamedTuple, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -35,6 +35,18 @@ class AWQMoeWeights(NamedTuple):
     @property
     def num_experts(self) -> int:
         return self.experts.w.shape[0]
+
+
+# An expert stack: repacked AWQ, or dense [E, N, K] as a checkpoint holds it.
+MoeWeights = Union[AWQMoeWeights, torch.Tensor]
+
+
+def _expert_dims(w: MoeWeights) -> Tuple[int, int, int]:
+    """(experts, input size, output size) of a stack."""
+    if isinstance(w, torch.Tensor):
+        assert w.dim() == 3, "dense expert weights must be [E, N, K]"
+        return w.shape[0], w.shape[2], w.shape[1]
+    return w.num_experts, w.input_size, w.output_size
 
 
 def process_awq_moe_weights(qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Tensor) -> AWQMoeWeights:
@@ -72,7 +84,7 @@ def get_default_config(M: int, E: int, N: int, K: int, topk: int) -> Dict[str, i
     return {"BLOCK_SIZE_M": BLOCK_SIZE_M}
 
 
-def fused_experts_impl(hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, topk_weights: torch.Tensor,
+def fused_experts_impl(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, topk_weights: torch.Tensor,
                        topk_ids: torch.Tensor, activation: str = "silu",
                        apply_router_weight_on_input: bool = False) -> torch.Tensor:
     """Run alignment, both grouped GEMMs and the top-k sum; writes into ``hidden_states``
@@ -82,23 +94,34 @@ def fused_experts_impl(hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMo
     T, top_k = hidden_states.shape[0], topk_ids.shape[1]
     if T * top_k == 0:
         return hidden_states
-    config = get_default_config(T, w1.num_experts, w1.output_size, w1.input_size, top_k)
-    align = ops.moe_align_block_size(topk_ids.to(torch.int32), config["BLOCK_SIZE_M"], w1.num_experts)
+    E, K, N = _expert_dims(w1)
+    config = get_default_config(T, E, N, K, top_k)
+    align = ops.moe_align_block_size(topk_ids.to(torch.int32), config["BLOCK_SIZE_M"], E)
     return _run_experts(hidden_states, w1, w2, topk_weights, top_k, align, activation, apply_router_weight_on_input)
 
 
-def _check_experts(hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, activation: str) -> None:
+def _check_experts(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, activation: str) -> None:
     if activation not in ("silu", "gelu"):
         raise ValueError(f"unsupported activation {activation!r}")
-    assert hidden_states.shape[1] == w1.input_size, "Hidden size mismatch"
+    (E1, K1, N1), (E2, K2, N2) = _expert_dims(w1), _expert_dims(w2)
+    assert hidden_states.shape[1] == K1, "Hidden size mismatch"
     assert hidden_states.is_contiguous(), "Hidden_states must be contiguous"
     assert hidden_states.dtype in (torch.float16, torch.bfloat16)
-    assert w1.num_experts == w2.num_experts, "expert counts differ"
-    assert w2.input_size == w1.output_size // 2, "w2's input size must be half of w1's output size"
-    assert w2.output_size == hidden_states.shape[1], "w2's output size must equal the hidden size"
+    assert E1 == E2, "expert counts differ"
+    assert K2 == N1 // 2, "w2's input size must be half of w1's output size"
+    assert N2 == hidden_states.shape[1], "w2's output size must equal the hidden size"
 
 
-def _run_experts(hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, topk_weights: torch.Tensor,
+def _expert_gemm(a: torch.Tensor, w: MoeWeights, align: ops.MoeAlignment, topk_weights: torch.Tensor, num_routed: int,
+                 top_k: int, activation: Optional[str], mul_routed_weight: bool) -> torch.Tensor:
+    if isinstance(w, torch.Tensor):
+        return ops.moe_dense_gemm(a, w, align, topk_weights, num_routed, top_k, activation=activation,
+                                  mul_routed_weight=mul_routed_weight)
+    return ops.moe_gemm(a, w.experts, w.input_size, w.output_size, w.group_size, align, topk_weights, num_routed,
+                        top_k, activation=activation, mul_routed_weight=mul_routed_weight)
+
+
+def _run_experts(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, topk_weights: torch.Tensor,
                  top_k: int, align: ops.MoeAlignment, activation: str,
                  apply_router_weight_on_input: bool) -> torch.Tensor:
     """Both grouped GEMMs over aligned rows and the top-k sum, into ``hidden_states``."""
@@ -106,12 +129,11 @@ def _run_experts(hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeigh
     num_routed = T * top_k
     # First GEMM: gate/up, routed row r reads token r // top_k; act(gate) * up
     # fused into the epilogue (intermediate_cache1 -> intermediate_cache2).
-    cache2 = ops.moe_gemm(hidden_states, w1.experts, w1.input_size, w1.output_size, w1.group_size, align, topk_weights,
-                          num_routed, top_k, activation=activation, mul_routed_weight=apply_router_weight_on_input)
+    cache2 = _expert_gemm(hidden_states, w1, align, topk_weights, num_routed, top_k, activation,
+                          apply_router_weight_on_input)
     # Second GEMM: down, routed row r reads cache2[r]; the routed weight is
     # applied in fp32 before the cast (MUL_ROUTED_WEIGHT = not on input).
-    cache3 = ops.moe_gemm(cache2, w2.experts, w2.input_size, w2.output_size, w2.group_size, align, topk_weights,
-                          num_routed, 1, activation=None, mul_routed_weight=not apply_router_weight_on_input)
+    cache3 = _expert_gemm(cache2, w2, align, topk_weights, num_routed, 1, None, not apply_router_weight_on_input)
     ops.moe_sum_reduce(cache3.view(T, top_k, H), hidden_states)
     return hidden_states
 
@@ -128,13 +150,14 @@ class BaseMoeBackend(ABC):
 class AWQFusedMoe(BaseMoeBackend):
     """Fused MoE backend over AWQ expert stacks (FusedMoe, fused.py:205-233)."""
 
-    def forward(self, hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, gating_output: torch.Tensor,
+    def forward(self, hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, gating_output: torch.Tensor,
                 topk: int, renormalize: bool, activation: str = "silu",
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
         T, E = gating_output.shape
-        if T > 0 and hidden_states.shape[0] == T and E == w1.num_experts:
+        E1, K1, N1 = _expert_dims(w1)
+        if T > 0 and hidden_states.shape[0] == T and E == E1:
             _check_experts(hidden_states, w1, w2, activation)
-            config = get_default_config(T, E, w1.output_size, w1.input_size, topk)
+            config = get_default_config(T, E, N1, K1, topk)
             topk_weights, _, align = ops.moe_route(gating_output, topk, renormalize, config["BLOCK_SIZE_M"])
             return _run_experts(hidden_states, w1, w2, topk_weights, topk, align, activation,
                                 apply_router_weight_on_input)
@@ -142,3 +165,15 @@ class AWQFusedMoe(BaseMoeBackend):
                                             renormalize=renormalize)
         return fused_experts_impl(hidden_states, w1, w2, topk_weights, topk_ids, activation,
                                   apply_router_weight_on_input=apply_router_weight_on_input)
+
+
+class FusedMoe(AWQFusedMoe):
+    """The same backend over dense experts, w1 [E, 2I, H] and w2 [E, H, I] (FusedMoe, fused.py:205-233)."""
+
+    def forward(self, hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, gating_output: torch.Tensor,
+                topk: int, renormalize: bool, activation: str = "silu",
+                apply_router_weight_on_input: bool = False) -> torch.Tensor:
+        if not (isinstance(w1, torch.Tensor) and isinstance(w2, torch.Tensor)):
+            raise ValueError("the fused backend takes dense expert weights; repacked AWQ ones go to awq_fused")
+        return super().forward(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
+                               apply_router_weight_on_input)

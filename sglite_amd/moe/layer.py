@@ -1,6 +1,6 @@
-"""Mixture-of-experts layer over AWQ expert stacks.
+"""Mixture-of-experts layers over AWQ expert stacks and over dense experts.
 
-Mirror of ``MoELayer`` (python/sglite/srt/model_executor/layers/moe_layer.py:11-64)
+``AWQMoELayer`` is a mirror of ``MoELayer`` (python/sglite/srt/model_executor/layers/moe_layer.py:11-64)
 for AWQ checkpoints:
 
 * the constructor takes the same arguments (num_experts, top_k, hidden_size,
@@ -24,16 +24,20 @@ for AWQ checkpoints:
 * ``forward(hidden_states, router_logits)`` runs the MoE backend (routing,
   grouped GEMMs, top-k sum) and all-reduces the output when tp_size > 1
   (moe_layer.py:48-64).
+
+``MoELayer`` is the same block for experts that a checkpoint leaves unquantised:
+its state dict holds gate_up_proj [E, 2I, H] and down_proj [E, H, I], which the
+products read as they are.
 """
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
 from ..linear import div_even
-from .fused import AWQMoeWeights, process_awq_moe_weights
+from .fused import AWQMoeWeights, MoeWeights, process_awq_moe_weights
 
 _AWQ_NAMES = ("qweight", "qzeros", "scales")
 
@@ -93,13 +97,14 @@ class AWQExpertStack:
         self._weights = process_awq_moe_weights(items["qweight"], items["qzeros"], items["scales"])
 
 
-class AWQMoELayer:
-    """Experts of one MoE block with AWQ W4A16 weights (MoELayer, moe_layer.py:11-64)."""
+class _MoEBlock:
+    """Routing parameters and the forward of one MoE block (MoELayer, moe_layer.py:11-64)."""
 
-    def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
-                 renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,
-                 group_size: int = 128, params_dtype: torch.dtype = torch.float16, tp_size: int = 1,
-                 process_group=None, backend: str = "awq_fused"):
+    # Columns of the gate (and up) projection come in multiples of this.
+    _COLUMNS = 16
+
+    def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int, renormalize: bool,
+                 activation: str, apply_router_weight_on_input: bool, tp_size: int, process_group, backend: str):
         if activation not in ("silu", "gelu"):
             raise ValueError(f"unsupported activation {activation!r}")
         if not 1 <= top_k <= num_experts:
@@ -114,15 +119,45 @@ class AWQMoELayer:
         self.tp_size = tp_size
         self._group = process_group
         local = div_even(intermediate_size, tp_size)
-        if local % 16:
-            raise ValueError(f"the per-rank intermediate size {local} must be a multiple of 16 "
-                             "(gate/up pairs are combined in 16-column tiles)")
+        if local % self._COLUMNS:
+            raise ValueError(f"the per-rank intermediate size {local} must be a multiple of {self._COLUMNS} "
+                             f"(gate/up pairs are combined in {self._COLUMNS}-column tiles)")
         self.intermediate_size_per_partition = local
-        self.gate_up_proj = AWQExpertStack(num_experts, hidden_size, 2 * local, group_size, params_dtype)
-        self.down_proj = AWQExpertStack(num_experts, local, hidden_size, group_size, params_dtype)
         from . import create_moe_backend
 
         self._backend = create_moe_backend(backend)
+
+    def _expert_weights(self) -> Tuple[MoeWeights, MoeWeights]:
+        raise NotImplementedError
+
+    def forward(self, hidden_states: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
+        """Route ``hidden_states [T, H]`` by ``router_logits [T, E]`` through the experts."""
+        w1, w2 = self._expert_weights()
+        out = self._backend.forward(hidden_states=hidden_states, w1=w1, w2=w2, gating_output=router_logits,
+                                    topk=self.top_k, renormalize=self.renormalize, activation=self.activation,
+                                    apply_router_weight_on_input=self.apply_router_weight_on_input)
+        if self.tp_size > 1:
+            torch.distributed.all_reduce(out, group=self._group)
+        return out
+
+    __call__ = forward
+
+
+class AWQMoELayer(_MoEBlock):
+    """Experts of one MoE block with AWQ W4A16 weights (MoELayer, moe_layer.py:11-64)."""
+
+    def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
+                 renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,
+                 group_size: int = 128, params_dtype: torch.dtype = torch.float16, tp_size: int = 1,
+                 process_group=None, backend: str = "awq_fused"):
+        super().__init__(num_experts, top_k, hidden_size, intermediate_size, renormalize, activation,
+                         apply_router_weight_on_input, tp_size, process_group, backend)
+        local = self.intermediate_size_per_partition
+        self.gate_up_proj = AWQExpertStack(num_experts, hidden_size, 2 * local, group_size, params_dtype)
+        self.down_proj = AWQExpertStack(num_experts, local, hidden_size, group_size, params_dtype)
+
+    def _expert_weights(self) -> Tuple[MoeWeights, MoeWeights]:
+        return self.gate_up_proj.weights, self.down_proj.weights
 
     def state_dict(self, *, prefix: str = "", result: Optional[Dict[str, torch.Tensor]] = None):
         result = result if result is not None else {}
@@ -146,14 +181,55 @@ class AWQMoELayer:
         if not _internal and state_dict:
             raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
 
-    def forward(self, hidden_states: torch.Tensor, router_logits: torch.Tensor) -> torch.Tensor:
-        """Route ``hidden_states [T, H]`` by ``router_logits [T, E]`` through the experts."""
-        out = self._backend.forward(hidden_states=hidden_states, w1=self.gate_up_proj.weights,
-                                    w2=self.down_proj.weights, gating_output=router_logits, topk=self.top_k,
-                                    renormalize=self.renormalize, activation=self.activation,
-                                    apply_router_weight_on_input=self.apply_router_weight_on_input)
-        if self.tp_size > 1:
-            torch.distributed.all_reduce(out, group=self._group)
-        return out
 
-    __call__ = forward
+_DENSE_NAMES = ("gate_up_proj", "down_proj")
+
+
+class MoELayer(_MoEBlock):
+    """Experts of one MoE block with dense weights (MoELayer, moe_layer.py:11-64)."""
+
+    _COLUMNS = 8  # rows of the weights are whole 16-byte vectors
+
+    def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
+                 renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,
+                 params_dtype: torch.dtype = torch.float16, tp_size: int = 1, process_group=None,
+                 backend: str = "fused"):
+        super().__init__(num_experts, top_k, hidden_size, intermediate_size, renormalize, activation,
+                         apply_router_weight_on_input, tp_size, process_group, backend)
+        if params_dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dense experts are float16 or bfloat16, got {params_dtype}")
+        if hidden_size % 8:
+            raise ValueError(f"the hidden size {hidden_size} must be a multiple of 8")
+        local = self.intermediate_size_per_partition
+        # What the state dict must hold, until it is loaded.
+        self.gate_up_proj = torch.empty((num_experts, 2 * local, hidden_size), dtype=params_dtype, device="meta")
+        self.down_proj = torch.empty((num_experts, hidden_size, local), dtype=params_dtype, device="meta")
+
+    def state_dict(self, *, prefix: str = "", result: Optional[Dict[str, torch.Tensor]] = None):
+        result = result if result is not None else {}
+        for name in _DENSE_NAMES:
+            result[_concat_prefix(prefix, name)] = getattr(self, name)
+        return result
+
+    def state_dict_keys(self, prefix: str = "") -> List[str]:
+        return list(self.state_dict(prefix=prefix).keys())
+
+    def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
+                        _internal: bool = False) -> None:
+        keys = {name: _concat_prefix(prefix, name) for name in _DENSE_NAMES}
+        for name, key in keys.items():  # check everything before any change
+            if key not in state_dict:
+                raise KeyError(key)
+            param, item = getattr(self, name), state_dict[key]
+            assert isinstance(item, torch.Tensor)
+            assert param.shape == item.shape and param.dtype == item.dtype, (
+                f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
+        for name, key in keys.items():
+            setattr(self, name, state_dict.pop(key).contiguous())
+        if not _internal and state_dict:
+            raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
+
+    def _expert_weights(self) -> Tuple[MoeWeights, MoeWeights]:
+        if self.gate_up_proj.is_meta:
+            raise RuntimeError("expert weights are not loaded (call load_state_dict first)")
+        return self.gate_up_proj, self.down_proj

@@ -481,6 +481,16 @@ def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, de
         raise ValueError(f"{what} must be contiguous and 8-byte aligned")
 
 
+def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether the address ranges that two tensors' elements span meet."""
+    if s.numel() == 0 or t.numel() == 0:
+        return False
+
+    def end(v: torch.Tensor) -> int:
+        return v.data_ptr() + (sum((n - 1) * st for n, st in zip(v.shape, v.stride())) + 1) * v.element_size()
+    return s.data_ptr() < end(t) and t.data_ptr() < end(s)
+
+
 def _check_counters(counters: torch.Tensor, N: int, device: torch.device) -> None:
     if counters.dtype != torch.int32:
         raise ValueError(f"counters must be int32, got {counters.dtype}")
@@ -987,6 +997,91 @@ def moe_gemm(a: torch.Tensor, experts: RepackedExperts, K: int, N: int, group_si
     return out
 
 
+def _moe_dense_launch(a: torch.Tensor, w: torch.Tensor, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
+                      topk_weights: Optional[torch.Tensor], out: torch.Tensor, num_routed: int, top_k: int, act: int,
+                      mul_routed_weight: bool) -> None:
+    dev = a.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _moe_dense_launch(a, w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k, act,
+                                     mul_routed_weight)
+    E, N, K = w.shape
+    _lib.check(_lib.load().awq_moe_dense_gemm(
+        a.data_ptr(), a.shape[0], w.data_ptr(), E, N, K, dtype_code(a.dtype), sorted_ids.data_ptr(),
+        sorted_ids.numel(), expert_offsets.data_ptr(), _ptr(topk_weights), num_routed, top_k, act,
+        1 if mul_routed_weight else 0, out.data_ptr(), _stream(dev)), "awq_moe_dense_gemm")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_moe_dense_gemm", mutates_args=("out",), device_types="cuda")
+def _moe_dense_op(a: torch.Tensor, w: torch.Tensor, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
+                  topk_weights: Optional[torch.Tensor], out: torch.Tensor, num_routed: int, top_k: int,
+                  activation: str, mul_routed_weight: bool) -> None:
+    _moe_dense_launch(a, w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k,
+                      _ACT_CODE[_ACT_NAME[activation]], mul_routed_weight)
+
+
+@_moe_dense_op.register_fake
+def _(a, w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k, activation, mul_routed_weight):
+    return None
+
+
+def moe_dense_gemm(a: torch.Tensor, w: torch.Tensor, align: MoeAlignment, topk_weights: Optional[torch.Tensor],
+                   num_routed: int, top_k: int, activation: Optional[str] = None, mul_routed_weight: bool = False,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Grouped product over the expert buckets with dense weights ``w`` [E, N, K].
+
+    Routed row r reads ``a[r // top_k]``; the output has ``num_routed`` rows of ``N`` columns, or ``N / 2`` of
+    ``act(gate) * up`` with an ``activation`` ("silu"/"gelu", gate rows of ``w`` first).  fp32 sums, rounded once.
+    Rows that ``align`` does not hold (ids outside the experts) are not written."""
+    if w.dim() != 3:
+        raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
+    E, N, K = w.shape
+    if a.dim() != 2 or a.shape[1] != K:
+        raise ValueError(f"a must be [rows, {K}], got {tuple(a.shape)}")
+    dtype_code(a.dtype)
+    if a.dtype != w.dtype:
+        raise ValueError(f"activation dtype {a.dtype} does not match the weight dtype {w.dtype}")
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        raise ValueError("w must be contiguous and 16-byte aligned")
+    if activation not in _ACT_CODE:
+        raise ValueError(f"unsupported activation {activation!r}")
+    if mul_routed_weight and topk_weights is None:
+        raise ValueError("mul_routed_weight needs topk_weights")
+    if num_routed < 0 or top_k < 1:
+        raise ValueError(f"num_routed must be at least 0 and top_k at least 1, got {num_routed} and {top_k}")
+    if align.expert_offsets.numel() != E + 1:
+        raise ValueError(f"the rows were aligned for {align.expert_offsets.numel() - 1} experts, w holds {E}")
+    if align.sorted_ids.dtype != torch.int32 or align.expert_offsets.dtype != torch.int32 \
+            or not align.sorted_ids.is_contiguous() or not align.expert_offsets.is_contiguous():
+        raise ValueError("the alignment must be moe_align_block_size's: contiguous int32")
+    ncols = N // 2 if activation is not None else N
+    if topk_weights is not None and topk_weights.numel() < num_routed:
+        raise ValueError(f"topk_weights must hold {num_routed} routed weights, got {topk_weights.numel()}")
+    _require_cuda(a, w, topk_weights, align.sorted_ids, align.expert_offsets)
+    for t in (w, topk_weights, align.sorted_ids, align.expert_offsets):
+        if t is not None and t.device != a.device:
+            raise ValueError("a, w, the weights and the alignment must be on one device")
+    a = _aligned(a)
+    if out is None:
+        out = torch.empty((num_routed, ncols), dtype=a.dtype, device=a.device)
+    else:
+        _check_out(out, (num_routed, ncols), a.dtype, a.device)
+        if out.data_ptr() % 16:
+            raise ValueError("out must be 16-byte aligned")
+        if _overlap(out, a) or _overlap(out, w):
+            raise ValueError("out must not share memory with a or w")
+    if topk_weights is not None:
+        topk_weights = _aligned(topk_weights.float().reshape(-1), 4)
+    if _undispatched(a, w, topk_weights, out, align.sorted_ids, align.expert_offsets):
+        _moe_dense_launch(a, w, align.sorted_ids, align.expert_offsets, topk_weights, out, num_routed, top_k,
+                          _ACT_CODE[activation], mul_routed_weight)
+        return out
+    torch.ops.sglite_awq.awq_moe_dense_gemm(a, w, align.sorted_ids, align.expert_offsets, topk_weights, out,
+                                            num_routed, top_k, "none" if activation is None else activation,
+                                            bool(mul_routed_weight))
+    return out
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_moe_sum_reduce", mutates_args=("out",), device_types="cuda")
 def _moe_sum_op(inp: torch.Tensor, out: torch.Tensor) -> None:
     T, k, H = inp.shape
@@ -1193,16 +1288,6 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
     _require_cuda(y, x, a, b, stack.scaling, stack.ranks, batch.sorted_ids, batch.block_adapters)
 
 
-def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether the address ranges that two tensors' elements span meet."""
-    if s.numel() == 0 or t.numel() == 0:
-        return False
-
-    def end(v: torch.Tensor) -> int:
-        return v.data_ptr() + (sum((n - 1) * st for n, st in zip(v.shape, v.stride())) + 1) * v.element_size()
-    return s.data_ptr() < end(t) and t.data_ptr() < end(s)
-
-
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch, activation: Optional[str] = None,
              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``y + scaling * B (A x)`` of every row's adapter, summed in fp32 and rounded once, on x's current stream.
@@ -1244,5 +1329,5 @@ REGISTERED_OPS: List[str] = [
     "awq_repack_cdna4", "awq_unrepack_cdna4", "awq_dequant", "awq_dequant_repacked", "awq_w4a16_gemm",
     "awq_w4a16_gemm_out", "awq_w4a16_gemm_act", "awq_w4a16_gemm_act_out", "awq_repack_experts",
     "awq_moe_topk_softmax", "awq_moe_align_block_size", "awq_moe_route", "awq_moe_w4a16_gemm", "awq_moe_sum_reduce",
-    "awq_lora_route", "awq_lora_add", "awq_lora_add_",
+    "awq_moe_dense_gemm", "awq_lora_route", "awq_lora_add", "awq_lora_add_",
 ]
