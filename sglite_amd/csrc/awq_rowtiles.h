@@ -59,6 +59,38 @@ struct RowTiles {
     rb = __builtin_amdgcn_readlane(fb, src);
     rows = __builtin_amdgcn_readlane(fn, src);
   }
+
+  // Unit u of the (tile, column group) pairs, the experts in order and inside
+  // an expert its tiles for one column group after the other's: neighbours read
+  // the same weights.  The tiles of an expert are of nearly equal size, rounded
+  // up to `grain` rows.
+  __device__ __forceinline__ void find_unit(int u, int groups, int tile_rows, int grain, int lane, int& e, int& rb,
+                                            int& rows, int& group) const {
+    const uint64_t hit = __ballot(u >= excl * groups && u < incl * groups);
+    if (hit == 0) {
+      e = -1;
+      return;
+    }
+    int fe = 0, fb = 0, fn = 0, fg = 0, pos = excl;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int n = (nr[i] + tile_rows - 1) / tile_rows;
+      if (u >= pos * groups && u < (pos + n) * groups) {
+        const int at = u - pos * groups;
+        fg = at / n;
+        const int per = ((nr[i] + n - 1) / n + grain - 1) / grain * grain;
+        fe = lane * EPL + i;
+        fb = r0[i] + (at - fg * n) * per;
+        fn = min(per, r0[i] + nr[i] - fb);
+      }
+      pos += n;
+    }
+    const int src = __builtin_ctzll(hit);
+    e = __builtin_amdgcn_readlane(fe, src);
+    rb = __builtin_amdgcn_readlane(fb, src);
+    rows = __builtin_amdgcn_readlane(fn, src);
+    group = __builtin_amdgcn_readlane(fg, src);
+  }
 };
 
 }  // namespace sgl_awq
