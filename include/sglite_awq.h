@@ -434,8 +434,9 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  * reference.
  *
  * awq_lora_route sorts the rows by adapter (stable) into 16-row blocks; one
- * call serves every projection of the step.  Ids outside [0, num_adapters)
- * name no adapter.
+ * call serves every projection of the step, and a step of up to
+ * AWQ_LORA_MAX_UNROUTED_ROWS rows can do without.  Ids outside
+ * [0, num_adapters) name no adapter.
  *   adapter_ids [M]
  *   sorted_ids[awq_moe_sorted_capacity(M, num_adapters + 1, 16)]  rows, M in padding
  *   block_adapters[awq_moe_block_capacity(M, num_adapters + 1, 16)]
@@ -454,22 +455,27 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  *          then not touched); AWQ_ACT_SILU / AWQ_ACT_GELU: parts are gate and up
  *          of equal width and out [M, N / 2] = act(y'_gate) * y'_up for every row
  *   N, K, max_rank and every part multiples of 8; y, x, a, b, out 16-byte aligned
- *   ws     awq_lora_workspace_bytes bytes, 16-byte aligned, any content
+ *   sorted_ids, block_adapters  from awq_lora_route, adapter_ids may then be
+ *          null; or both null and adapter_ids [M] read row by row
+ *   ws     awq_lora_workspace_bytes bytes (`routed`: with the tables), 16-byte
+ *          aligned, any content
  * Limits: num_adapters <= AWQ_LORA_MAX_ADAPTERS, max_rank <= AWQ_LORA_MAX_RANK,
  * parts <= AWQ_LORA_MAX_PARTS, M < 2^24; x, one adapter's a and one adapter's b
  * below 2 GiB each. */
 #define AWQ_LORA_MAX_ADAPTERS 511
 #define AWQ_LORA_MAX_RANK 256
 #define AWQ_LORA_MAX_PARTS 4
+#define AWQ_LORA_MAX_UNROUTED_ROWS 256
 int awq_lora_route(const int32_t* adapter_ids, int64_t M, int64_t num_adapters, int32_t* sorted_ids,
                    int32_t* block_adapters, int32_t* num_rows_post_pad, int32_t* adapter_offsets,
                    awq_stream_t stream);
-int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts);
+int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts,
+                                 int routed);
 int awq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling,
                  const int32_t* ranks, void* out, int64_t M, int64_t N, int64_t K, int64_t num_adapters,
                  int64_t max_rank, int parts, const int64_t* part_cols, int dtype, int activation,
-                 const int32_t* sorted_ids, const int32_t* block_adapters, void* ws, int64_t ws_bytes,
-                 awq_stream_t stream);
+                 const int32_t* adapter_ids, const int32_t* sorted_ids, const int32_t* block_adapters, void* ws,
+                 int64_t ws_bytes, awq_stream_t stream);
 
 #ifdef __cplusplus
 }

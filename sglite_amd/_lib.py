@@ -78,9 +78,9 @@ SIGNATURES = {
                                   _vp, _vp]),
     "awq_moe_sum_reduce": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp]),
     "awq_lora_route": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
-    "awq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "awq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int, _int]),
     "awq_lora_add": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,
-                            ctypes.POINTER(_i64), _int, _int, _vp, _vp, _vp, _i64, _vp]),
+                            ctypes.POINTER(_i64), _int, _int, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 AWQ_ACT_SILU = 1
@@ -115,6 +115,7 @@ AWQ_NOALLOC_MAX_N = 1 << 20
 AWQ_LORA_MAX_ADAPTERS = 511
 AWQ_LORA_MAX_RANK = 256
 AWQ_LORA_MAX_PARTS = 4
+AWQ_LORA_MAX_UNROUTED_ROWS = 256
 
 AWQ_MOE_ACT_NONE = 0
 AWQ_MOE_ACT_SILU = 1

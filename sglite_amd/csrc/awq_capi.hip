@@ -889,18 +889,19 @@ int check_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int parts,
 
 }  // namespace
 
-int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts) {
+int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_adapters, int64_t max_rank, int parts,
+                                 int routed) {
   const int st = check_lora(M, N, K, num_adapters, max_rank, parts, "awq_lora_workspace_bytes");
   if (st != 0) return st;
   ok();
-  return M == 0 ? 0 : plan_lora(M, K, num_adapters, max_rank, parts).ws_bytes;
+  return M == 0 ? 0 : plan_lora(M, K, num_adapters, max_rank, parts, routed != 0).ws_bytes;
 }
 
 int awq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling,
                  const int32_t* ranks, void* out, int64_t M, int64_t N, int64_t K, int64_t num_adapters,
                  int64_t max_rank, int parts, const int64_t* part_cols, int dtype, int activation,
-                 const int32_t* sorted_ids, const int32_t* block_adapters, void* ws, int64_t ws_bytes,
-                 awq_stream_t stream) {
+                 const int32_t* adapter_ids, const int32_t* sorted_ids, const int32_t* block_adapters, void* ws,
+                 int64_t ws_bytes, awq_stream_t stream) {
   const TraceRange range("awq_lora_add");
   if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16)
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: dtype must be 0 or 1, got %d", dtype);
@@ -922,13 +923,17 @@ int awq_lora_add(const void* y, const void* x, const void* a, const void* b, con
   if (activation != 0 && (parts != 2 || part_cols[0] != part_cols[1]))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: an activation needs two equal parts, gate and up");
   if (M == 0) return ok();
-  if (!y || !x || !a || !b || !scaling || !ranks || !out || !sorted_ids || !block_adapters)
+  const bool routed = sorted_ids != nullptr;
+  if (!y || !x || !a || !b || !scaling || !ranks || !out || (routed ? !block_adapters : !adapter_ids))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: null pointer argument");
   if (!aligned(y, 16) || !aligned(x, 16) || !aligned(a, 16) || !aligned(b, 16) || !aligned(out, 16))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: y, x, a, b and out must be 16-byte aligned");
   if (activation != 0 && out == y)
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_lora_add: with an activation out must not be y");
-  const int64_t need = plan_lora(M, K, num_adapters, max_rank, parts).ws_bytes;
+  if (!routed && M > AWQ_LORA_MAX_UNROUTED_ROWS)
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_add: more than %d rows need the tables of awq_lora_route",
+                AWQ_LORA_MAX_UNROUTED_ROWS);
+  const int64_t need = plan_lora(M, K, num_adapters, max_rank, parts, routed).ws_bytes;
   if (!ws || ws_bytes < need || !aligned(ws, 16))
     return fail(AWQ_STATUS_WORKSPACE, "awq_lora_add: a 16-byte aligned workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)ws_bytes);
@@ -949,9 +954,10 @@ int awq_lora_add(const void* y, const void* x, const void* a, const void* b, con
   p.part_cols = part_cols;
   p.act = activation;
   p.dtype = dtype;
+  p.ids = adapter_ids;
   p.sorted = sorted_ids;
   p.bucket = block_adapters;
-  p.ws = (float*)ws;
+  p.ws = ws;
   return hip_status(launch_lora(p, (hipStream_t)stream), "awq_lora_add launch");
 }
 

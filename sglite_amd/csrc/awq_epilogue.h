@@ -34,6 +34,15 @@ __device__ __forceinline__ float gated_act(int act, float g) {
   return act == kActSilu ? g / (1.f + expf(-g)) : 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
 }
 
+// The same through the hardware's base-2 exponential and reciprocal (each
+// within an ulp or two of fp32, far below the 16-bit rounding that follows),
+// where a kernel is bound by reading: silu takes 5 vector operations instead of
+// about 25.
+__device__ __forceinline__ float gated_act_fast(int act, float g) {
+  if (act != kActSilu) return gated_act(act, g);
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896f * g));
+}
+
 // Fused gate/up output of four columns o0..o0+3: the gate and up sums are each
 // rounded to the output dtype with their bias added in that dtype (gate bias
 // at o0, up bias nh columns further: the merged projection's two halves),

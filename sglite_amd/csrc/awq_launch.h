@@ -174,15 +174,20 @@ hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s);
 constexpr int kLoraBlock = 16;    // rows of a block of the sorted table
 constexpr int kLoraParts = 4;     // column parts of a projection, at most
 constexpr int kLoraColTiles = 4;  // 16-column tiles of a wave of the expand
+constexpr int kLoraTileRows = 512;  // rows from which the prefill kernels run
+enum : int { kLoraRows = 0, kLoraBlocks = 1, kLoraTiles = 2 };
 struct LoraPlan {
-  int64_t blocks;  // 16-row blocks the grids cover
-  int row_tiles;   // of a workgroup of the shrink
-  int rank_tiles;  // ... and its 16-rank tiles
-  int slices;      // k-slices of the shrink, summed by the expand
-  int per;         // row blocks that a workgroup of the expand takes in turn
+  int mode;           // one of the three above
+  int64_t blocks;     // row blocks the grids cover
+  int64_t positions;  // rows of the shrink's result
+  int rank_tiles;     // 16-rank tiles of a wave of the shrink
+  int slices;         // k-slices of the shrink
+  int per;            // row blocks that a workgroup of the expand takes in turn
+  int64_t v_bytes, vs_bytes, ve_bytes;  // the workspace: partial sums, operands, exponents
   int64_t ws_bytes;
 };
-LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts);
+// routed: with the sorted table of launch_lora_route.
+LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts, bool routed);
 hipError_t launch_lora_route(const int32_t* ids, int64_t n, int64_t L, int32_t* sorted, int32_t* bucket,
                              int32_t* num_post_pad, int32_t* offsets, hipStream_t s);
 struct LoraParams {
@@ -197,9 +202,10 @@ struct LoraParams {
   int parts;
   const int64_t* part_cols;
   int act, dtype;
-  const int32_t* sorted;  // from launch_lora_route
+  const int32_t* ids;     // adapter of each row
+  const int32_t* sorted;  // from launch_lora_route, or null
   const int32_t* bucket;
-  float* ws;
+  void* ws;
 };
 hipError_t launch_lora(const LoraParams& p, hipStream_t s);
 

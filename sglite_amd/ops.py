@@ -1129,12 +1129,19 @@ class LoraStack(NamedTuple):
 
 
 class LoraBatch(NamedTuple):
-    """A step's rows in the order of their adapters (``lora_route``)."""
-    sorted_ids: torch.Tensor      # int32, rows; the row count in padding
-    block_adapters: torch.Tensor  # int32, adapter of each 16-row block (num_adapters: none, -1: past the last)
-    offsets: torch.Tensor         # int32 [num_adapters + 2], padded bucket starts
-    rows: int
+    """A step's rows and their adapters (``lora_route``); the tables are None for the few rows of a small step."""
+    adapter_ids: torch.Tensor               # int32 [rows], as given
+    sorted_ids: Optional[torch.Tensor]      # int32, rows by adapter; the row count in padding
+    block_adapters: Optional[torch.Tensor]  # int32, adapter of each 16-row block (num_adapters: none, -1: past the end)
     num_adapters: int
+
+    @property
+    def rows(self) -> int:
+        return self.adapter_ids.numel()
+
+
+# Rows up to which every row is taken by itself and nothing is sorted.
+LORA_UNSORTED_ROWS = 32
 
 
 def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[int], dtype: torch.dtype,
@@ -1148,102 +1155,102 @@ def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[in
                      torch.zeros(num_adapters, dtype=torch.int32, device=device), tuple(int(n) for n in parts))
 
 
-def _lora_route_launch(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+def _lora_route_launch(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = adapter_ids.device
     if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):
             return _lora_route_launch(adapter_ids, num_adapters)
     M = adapter_ids.numel()
     cap = M + (num_adapters + 1) * 15  # awq_moe_sorted_capacity(M, num_adapters + 1, 16)
+    sorted_ids = torch.empty(cap, dtype=torch.int32, device=dev)
+    # Block adapters, then what the projections do not read: offsets and the padded row count.
     bcap = (cap + 15) // 16
-    # One allocation: sorted ids, block adapters, offsets, the padded row count.
-    n0, n1 = (cap + 3) // 4 * 4, (bcap + 3) // 4 * 4
-    buf = torch.empty(n0 + n1 + num_adapters + 3, dtype=torch.int32, device=dev)
-    sorted_ids, blocks = buf[:cap], buf[n0:n0 + bcap]
-    offsets = buf[n0 + n1:n0 + n1 + num_adapters + 2]
-    p = buf.data_ptr()
-    _lib.check(_lib.load().awq_lora_route(adapter_ids.data_ptr() if M else None, M, num_adapters, p, p + 4 * n0,
-                                          p + 4 * (n0 + n1 + num_adapters + 2), p + 4 * (n0 + n1), _stream(dev)),
-               "awq_lora_route")
-    return sorted_ids, blocks, offsets
+    blocks = torch.empty(bcap + num_adapters + 3, dtype=torch.int32, device=dev)
+    p = blocks.data_ptr()
+    _lib.check(_lib.load().awq_lora_route(adapter_ids.data_ptr() if M else None, M, num_adapters,
+                                          sorted_ids.data_ptr(), p, p + 4 * (bcap + num_adapters + 2), p + 4 * bcap,
+                                          _stream(dev)), "awq_lora_route")
+    return sorted_ids, blocks
 
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_lora_route", mutates_args=(), device_types="cuda")
-def _lora_route_op(adapter_ids: torch.Tensor,
-                   num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    # Outputs of a registered op are tensors of their own.
-    return tuple(t.clone() for t in _lora_route_launch(adapter_ids, num_adapters))
+def _lora_route_op(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _lora_route_launch(adapter_ids, num_adapters)
 
 
 @_lora_route_op.register_fake
 def _(adapter_ids, num_adapters):
     cap = adapter_ids.numel() + (num_adapters + 1) * 15
-    return (adapter_ids.new_empty(cap), adapter_ids.new_empty((cap + 15) // 16),
-            adapter_ids.new_empty(num_adapters + 2))
+    return adapter_ids.new_empty(cap), adapter_ids.new_empty((cap + 15) // 16 + num_adapters + 3)
 
 
 def lora_route(adapter_ids: torch.Tensor, num_adapters: int) -> LoraBatch:
-    """Sort a step's rows by adapter; one call serves every projection of the step.
+    """A step's rows by adapter; one call serves every projection of the step.
 
-    ``adapter_ids`` [M] int32 names each row's slot; an id outside ``[0, num_adapters)``, as -1, names none."""
+    ``adapter_ids`` [M] int32 names each row's slot; an id outside ``[0, num_adapters)``, as -1, names none.  The
+    batch refers to them: they stay as they are until its last use.  Up to ``LORA_UNSORTED_ROWS`` rows nothing is
+    launched, beyond that one kernel sorts the rows."""
     if adapter_ids.dim() != 1 or adapter_ids.dtype != torch.int32:
         raise ValueError(f"adapter_ids must be int32 [M], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
     if not 1 <= num_adapters <= _lib.AWQ_LORA_MAX_ADAPTERS:
         raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
     _require_cuda(adapter_ids)
     ids = _aligned(adapter_ids, 4)
+    if ids.numel() <= LORA_UNSORTED_ROWS:
+        return LoraBatch(ids, None, None, num_adapters)
     if _undispatched(ids):
-        t = _lora_route_launch(ids, num_adapters)
+        tables = _lora_route_launch(ids, num_adapters)
     else:
-        t = torch.ops.sglite_awq.awq_lora_route(ids, num_adapters)
-    return LoraBatch(*t, ids.numel(), num_adapters)
+        tables = torch.ops.sglite_awq.awq_lora_route(ids, num_adapters)
+    return LoraBatch(ids, *tables, num_adapters)
 
 
 def _lora_launch(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
-                 ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor, out: torch.Tensor,
-                 parts: Sequence[int], act: int) -> None:
+                 ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
+                 block_adapters: Optional[torch.Tensor], out: torch.Tensor, parts: Sequence[int], act: int) -> None:
     M, K = x.shape
     if M == 0:
         return
     dev = x.device
     if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
         with torch.cuda.device(dev):  # the C ABI's planning fills the current device's CUs
-            return _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, out, parts, act)
+            return _lora_launch(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, out, parts, act)
     L, N, R = b.shape
     lib = _lib.load()
-    wsb = _lib.check(lib.awq_lora_workspace_bytes(M, N, K, L, R, len(parts)), "awq_lora_workspace_bytes")
+    wsb = _lib.check(lib.awq_lora_workspace_bytes(M, N, K, L, R, len(parts), 0 if sorted_ids is None else 1),
+                     "awq_lora_workspace_bytes")
     ws = _workspace(wsb, dev)
     cols = (ctypes.c_int64 * len(parts))(*parts)
     _lib.check(lib.awq_lora_add(y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), scaling.data_ptr(),
                                 ranks.data_ptr(), out.data_ptr(), M, N, K, L, R, len(parts), cols,
-                                dtype_code(x.dtype), act, sorted_ids.data_ptr(), block_adapters.data_ptr(),
-                                ws.data_ptr(), wsb, _stream(dev)), "awq_lora_add")
+                                dtype_code(x.dtype), act, adapter_ids.data_ptr(), _ptr(sorted_ids),
+                                _ptr(block_adapters), ws.data_ptr(), wsb, _stream(dev)), "awq_lora_add")
 
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_lora_add", mutates_args=(), device_types="cuda")
 def _lora_add_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
-                 ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor, parts: List[int],
-                 activation: str) -> torch.Tensor:
+                 ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
+                 block_adapters: Optional[torch.Tensor], parts: List[int], activation: str) -> torch.Tensor:
     act = _ACT_CODE[_ACT_NAME[activation]]
     out = torch.empty((y.shape[0], y.shape[1] // 2 if act else y.shape[1]), dtype=y.dtype, device=y.device)
-    _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, out, parts, act)
+    _lora_launch(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, out, parts, act)
     return out
 
 
 @_lora_add_op.register_fake
-def _(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, parts, activation):
+def _(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, parts, activation):
     return y.new_empty((y.shape[0], y.shape[1] if activation == "none" else y.shape[1] // 2))
 
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_lora_add_", mutates_args=("y",), device_types="cuda")
 def _lora_add_inplace_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
-                         ranks: torch.Tensor, sorted_ids: torch.Tensor, block_adapters: torch.Tensor,
-                         parts: List[int]) -> None:
-    _lora_launch(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, y, parts, 0)
+                         ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
+                         block_adapters: Optional[torch.Tensor], parts: List[int]) -> None:
+    _lora_launch(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, y, parts, 0)
 
 
 @_lora_add_inplace_op.register_fake
-def _(y, x, a, b, scaling, ranks, sorted_ids, block_adapters, parts):
+def _(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, parts):
     return None
 
 
@@ -1274,7 +1281,7 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
         if not t.is_contiguous() or t.data_ptr() % (16 if t.dtype == x.dtype else 4):
             raise ValueError("the stack's tensors must be contiguous (a and b 16-byte aligned)")
     dev = x.device
-    for t in (y, a, b, stack.scaling, stack.ranks, batch.sorted_ids, batch.block_adapters):
+    for t in (y, a, b, stack.scaling, stack.ranks, batch.adapter_ids):
         if t.device != dev:
             raise ValueError("y, x, the stack and the batch must be on one device")
     if batch.rows != M or batch.num_adapters != L:
@@ -1285,7 +1292,7 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
             raise ValueError(f"unsupported activation {activation!r}")
         if P != 2 or stack.parts[0] != stack.parts[1]:
             raise ValueError(f"an activation needs two equal parts, gate and up, got {stack.parts}")
-    _require_cuda(y, x, a, b, stack.scaling, stack.ranks, batch.sorted_ids, batch.block_adapters)
+    _require_cuda(y, x, a, b, stack.scaling, stack.ranks, batch.adapter_ids)
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch, activation: Optional[str] = None,
@@ -1306,7 +1313,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatc
             raise ValueError("out must not share memory with x, nor with y unless it is y")
     x = _aligned(x)
     a, b, scaling, ranks = stack.a, stack.b, stack.scaling, stack.ranks
-    tables = (batch.sorted_ids, batch.block_adapters)
+    tables = (batch.adapter_ids, batch.sorted_ids, batch.block_adapters)
     if out is not None:
         if out.data_ptr() != y.data_ptr():
             out.copy_(y)

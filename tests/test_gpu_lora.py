@@ -26,6 +26,11 @@ def make(M, K, parts, L, R, dtype, ranks=None, seed=0, scale=1.0):
     return y, x, stack, ids
 
 
+def routed(ids, L):
+    """The sorted tables whatever the row count."""
+    return ops.LoraBatch(ids, *torch.ops.sglite_awq.awq_lora_route(ids, L), L)
+
+
 def deltas(y, x, stack, ids):
     """(y + scaling B A x, a bound of its error before the last rounding), row by row in 64 bits."""
     out, err = y.double().clone(), torch.zeros(y.shape, dtype=torch.float64, device=y.device)
@@ -80,6 +85,9 @@ SHAPES = [
     (700, 640, (328,), 3, 72),
     (1111, 768, (640, 64), 6, 32),
     (2048, 256, (192,), 1, 200),
+    (515, 136, (72, 24), 100, 16),
+    (4100, 2048, (1024, 256, 256), 9, 64),
+    (600, 64, (40, 40, 40, 8), 2, 256),
 ]
 
 
@@ -101,6 +109,15 @@ def test_lora_add(M, K, parts, L, R, dtype):
     assert inplace is y and torch.equal(y, got)
     other = torch.full_like(y0, 7.0)
     assert torch.equal(ops.lora_add(y0, x, stack, batch, out=other), got)
+    # Few rows by the tables of a larger step, a larger step row by row.
+    assert (batch.sorted_ids is None) == (M <= ops.LORA_UNSORTED_ROWS)
+    if M <= 256:
+        for b in (routed(ids, L), ops.LoraBatch(ids, None, None, L)):
+            got = ops.lora_add(y0, x, stack, b)
+            close(got, want, err)
+            assert torch.equal(got[none], y0[none])
+            z = y0.clone()
+            assert torch.equal(ops.lora_add(z, x, stack, b, out=z), got)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
@@ -110,8 +127,11 @@ def test_lora_add(M, K, parts, L, R, dtype):
 def test_lora_add_gated(M, K, half, L, R, act, dtype):
     y, x, stack, ids = make(M, K, (half, half), L, R, dtype, [R - e % 3 for e in range(L)], seed=M)
     batch = ops.lora_route(ids, L)
-    got = ops.lora_add(y, x, stack, batch, activation=act)
-    close(got, *gated(*deltas(y, x, stack, ids), act))
+    want, err = gated(*deltas(y, x, stack, ids), act)
+    close(ops.lora_add(y, x, stack, batch, activation=act), want, err)
+    if M <= 256:
+        for b in (routed(ids, L), ops.LoraBatch(ids, None, None, L)):
+            close(ops.lora_add(y, x, stack, b, activation=act), want, err)
 
 
 def test_every_id_without_an_adapter_names_none():
@@ -125,13 +145,14 @@ def test_every_id_without_an_adapter_names_none():
 
 
 def test_all_rows_without_an_adapter_and_all_on_one():
-    y, x, stack, ids = make(200, 128, (64, 64), 3, 16, torch.bfloat16)
-    ids[:] = -1
-    batch = ops.lora_route(ids, 3)
-    assert torch.equal(ops.lora_add(y, x, stack, batch), y)
-    close(ops.lora_add(y, x, stack, batch, activation="silu"), *gated(*deltas(y, x, stack, ids), "silu"))
-    ids[:] = 2
-    close(ops.lora_add(y, x, stack, ops.lora_route(ids, 3)), *deltas(y, x, stack, ids))
+    for M in (9, 200, 800):
+        y, x, stack, ids = make(M, 128, (64, 64), 3, 16, torch.bfloat16)
+        ids[:] = -1
+        batch = ops.lora_route(ids, 3)
+        assert torch.equal(ops.lora_add(y, x, stack, batch), y)
+        close(ops.lora_add(y, x, stack, batch, activation="silu"), *gated(*deltas(y, x, stack, ids), "silu"))
+        ids[:] = 2
+        close(ops.lora_add(y, x, stack, ops.lora_route(ids, 3)), *deltas(y, x, stack, ids))
 
 
 def test_no_rows():
@@ -142,9 +163,10 @@ def test_no_rows():
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("scale", [2.0 ** -10, 1.0, 2.0 ** 9])
-def test_large_and_small_sums(dtype, scale):
-    """v = A x of 2^12 times x's size: beyond fp16's range in the last case."""
-    y, x, stack, ids = make(20, 512, (64,), 2, 16, dtype, scale=scale)
+@pytest.mark.parametrize("M", [20, 40, 520])
+def test_large_and_small_sums(M, dtype, scale):
+    """v = A x of 2^7 times x's size: beyond fp16's range in the last case."""
+    y, x, stack, ids = make(M, 512, (64,), 2, 16, dtype, scale=scale)
     stack.a.mul_(2.0 ** 7)
     stack.b.mul_(2.0 ** -12)
     close(ops.lora_add(y, x, stack, ops.lora_route(ids, 2)), *deltas(y, x, stack, ids))
@@ -154,7 +176,7 @@ def test_large_and_small_sums(dtype, scale):
 def test_what_lies_past_a_rank_does_not_count(bad):
     """NaN and infinities past an adapter's rank, in other adapters and in rows without one."""
     for dtype in (torch.float16, torch.bfloat16):
-        for M in (3, 90):
+        for M in (3, 90, 600):
             y, x, stack, ids = make(M, 136, (40, 24), 3, 40, dtype, [13, 40, 33])
             ids[:] = torch.arange(M, device=DEV, dtype=torch.int32) % 4 - 1
             ids[ids == 1] = 0
@@ -170,13 +192,13 @@ def test_what_lies_past_a_rank_does_not_count(bad):
 
 
 def test_infinite_and_nan_inputs_stay_in_their_rows():
-    for dtype in (torch.float16, torch.bfloat16):
-        y, x, stack, ids = make(40, 128, (64,), 2, 16, dtype)
+    for dtype, M in ((torch.float16, 30), (torch.bfloat16, 40), (torch.float16, 700)):
+        y, x, stack, ids = make(M, 128, (64,), 2, 16, dtype)
         ids[:] = 1
         want, err = deltas(y, x, stack, ids)
         x[3, 5], x[20, 127] = float("inf"), float("nan")
         got = ops.lora_add(y, x, stack, ops.lora_route(ids, 2))
-        keep = torch.ones(40, dtype=torch.bool, device=DEV)
+        keep = torch.ones(M, dtype=torch.bool, device=DEV)
         keep[3] = keep[20] = False
         close(got[keep], want[keep], err[keep])
         assert got[20].isnan().all() and not got[3].isfinite().any()
@@ -232,12 +254,8 @@ def test_two_graphs_replayed_in_turn_with_new_ids():
 
 def test_registered_ops_and_fakes():
     y, x, stack, ids = make(20, 128, (64, 64), 3, 16, torch.float16)
-    batch = ops.lora_route(ids, 3)
-    tables = torch.ops.sglite_awq.awq_lora_route(ids, 3)
-    for got, want in zip(tables, batch[:3]):
-        assert got.shape == want.shape
-    eager = ops.lora_add(y, x, stack, batch)
-    args = (stack.a, stack.b, stack.scaling, stack.ranks, tables[0], tables[1])
+    eager = ops.lora_add(y, x, stack, routed(ids, 3))
+    args = (stack.a, stack.b, stack.scaling, stack.ranks, *routed(ids, 3)[:3])
     assert torch.equal(torch.ops.sglite_awq.awq_lora_add(y, x, *args, [64, 64], "none"), eager)
     z = y.clone()
     torch.ops.sglite_awq.awq_lora_add_(z, x, *args, [64, 64])

@@ -62,7 +62,7 @@ def test_slot_refusals_change_nothing():
 
 
 def test_layers_without_slots_take_a_batch_and_ignore_it():
-    batch = ops.LoraBatch(*(torch.zeros(1, dtype=torch.int32) for _ in range(3)), 5, 2)
+    batch = ops.LoraBatch(torch.zeros(5, dtype=torch.int32), None, None, 2)
     g = torch.Generator().manual_seed(1)
     o = RowParallelLinear(16, 8, False)
     o.load_state_dict({"weight": torch.randn((8, 16), generator=g)})
@@ -81,8 +81,7 @@ def _stack(L=3, P=2, R=16, K=64, N=48, dtype=torch.float16):
 
 
 def _batch(M=4, L=3):
-    return ops.LoraBatch(torch.zeros(M + 15 * (L + 1), dtype=torch.int32), torch.zeros(8, dtype=torch.int32),
-                         torch.zeros(L + 2, dtype=torch.int32), M, L)
+    return ops.LoraBatch(torch.zeros(M, dtype=torch.int32), None, None, L)
 
 
 def test_python_refusals():
@@ -114,11 +113,11 @@ def test_python_refusals():
 
 def _call(lib, **kw):
     a = dict(y=4096, x=8192, a=16384, b=32768, scaling=64, ranks=128, out=65536, M=4, N=48, K=64, L=3, R=16, parts=2,
-             cols=(24, 24), dtype=0, act=0, sorted=256, blocks=512, ws=1 << 20, wsb=1 << 30)
+             cols=(24, 24), dtype=0, act=0, ids=192, sorted=256, blocks=512, ws=1 << 20, wsb=1 << 30)
     a.update(kw)
     cols = (ctypes.c_int64 * len(a["cols"]))(*a["cols"]) if a["cols"] else None
     return lib.awq_lora_add(a["y"], a["x"], a["a"], a["b"], a["scaling"], a["ranks"], a["out"], a["M"], a["N"], a["K"],
-                            a["L"], a["R"], a["parts"], cols, a["dtype"], a["act"], a["sorted"], a["blocks"],
+                            a["L"], a["R"], a["parts"], cols, a["dtype"], a["act"], a["ids"], a["sorted"], a["blocks"],
                             a["ws"], a["wsb"], None)
 
 
@@ -132,8 +131,9 @@ def test_c_abi_refusals():
             (inv, dict(cols=(20, 28))), (inv, dict(cols=(48, 0))), (inv, dict(cols=(56, -8))),
             (inv, dict(act=1, cols=(16, 32))), (inv, dict(act=1, parts=1, cols=(48,))), (inv, dict(act=1, out=4096)),
             (inv, dict(y=None)), (inv, dict(x=None)), (inv, dict(a=None)), (inv, dict(b=None)),
-            (inv, dict(scaling=None)), (inv, dict(ranks=None)), (inv, dict(out=None)), (inv, dict(sorted=None)),
-            (inv, dict(blocks=None)), (inv, dict(y=4104)), (inv, dict(x=8194)), (inv, dict(a=16392)),
+            (inv, dict(scaling=None)), (inv, dict(ranks=None)), (inv, dict(out=None)),
+            (inv, dict(blocks=None)), (inv, dict(ids=None, sorted=None)),
+            (uns, dict(M=257, sorted=None, blocks=None)), (inv, dict(y=4104)), (inv, dict(x=8194)), (inv, dict(a=16392)),
             (inv, dict(b=32776)), (inv, dict(out=65544)),
             (uns, dict(R=264)), (uns, dict(L=0)), (uns, dict(L=512)), (uns, dict(parts=5, cols=(8,) * 6)),
             (uns, dict(parts=0, cols=(48,))), (uns, dict(M=1 << 24)), (uns, dict(M=1 << 23, K=128)),
@@ -142,10 +142,12 @@ def test_c_abi_refusals():
         assert _call(lib, **kw) == want, kw
         assert lib.awq_last_error()
     assert _call(lib, M=0, y=None, x=None, ws=None) == 0
-    need = lib.awq_lora_workspace_bytes(4, 48, 64, 3, 16, 2)
-    assert need >= (4 + 4 * 15) * 32 * 4 and _call(lib, wsb=need - 1) == wsp
-    assert lib.awq_lora_workspace_bytes(0, 48, 64, 3, 16, 2) == 0
-    assert lib.awq_lora_workspace_bytes(4, 48, 64, 3, 304, 2) == uns
+    for routed, rows in ((1, 4 + 4 * 15), (0, 4)):
+        need = lib.awq_lora_workspace_bytes(4, 48, 64, 3, 16, 2, routed)
+        assert need >= rows * 32 * 4
+        assert _call(lib, wsb=need - 1, **({} if routed else dict(sorted=None, blocks=None))) == wsp
+        assert lib.awq_lora_workspace_bytes(0, 48, 64, 3, 16, 2, routed) == 0
+        assert lib.awq_lora_workspace_bytes(4, 48, 64, 3, 304, 2, routed) == uns
     for want, args in [(uns, (16, 4, 0, 16, 16, 16, 16, None)), (uns, (16, 4, 512, 16, 16, 16, 16, None)),
                        (uns, (16, -1, 3, 16, 16, 16, 16, None)), (uns, (16, 1 << 24, 3, 16, 16, 16, 16, None)),
                        (inv, (None, 4, 3, 16, 16, 16, 16, None)), (inv, (16, 4, 3, None, 16, 16, 16, None)),
