@@ -894,7 +894,7 @@ int64_t awq_lora_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t num_ad
   const int st = check_lora(M, N, K, num_adapters, max_rank, parts, "awq_lora_workspace_bytes");
   if (st != 0) return st;
   ok();
-  return M == 0 ? 0 : plan_lora(M, K, num_adapters, max_rank, parts, routed != 0).ws_bytes;
+  return M == 0 ? 0 : plan_lora(M, N, K, num_adapters, max_rank, parts, routed != 0).ws_bytes;
 }
 
 int awq_lora_add(const void* y, const void* x, const void* a, const void* b, const float* scaling,
@@ -933,7 +933,7 @@ int awq_lora_add(const void* y, const void* x, const void* a, const void* b, con
   if (!routed && M > AWQ_LORA_MAX_UNROUTED_ROWS)
     return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_add: more than %d rows need the tables of awq_lora_route",
                 AWQ_LORA_MAX_UNROUTED_ROWS);
-  const int64_t need = plan_lora(M, K, num_adapters, max_rank, parts, routed).ws_bytes;
+  const int64_t need = plan_lora(M, N, K, num_adapters, max_rank, parts, routed).ws_bytes;
   if (!ws || ws_bytes < need || !aligned(ws, 16))
     return fail(AWQ_STATUS_WORKSPACE, "awq_lora_add: a 16-byte aligned workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)ws_bytes);

@@ -182,12 +182,11 @@ struct LoraPlan {
   int64_t positions;  // rows of the shrink's result
   int rank_tiles;     // 16-rank tiles of a wave of the shrink
   int slices;         // k-slices of the shrink
-  int per;            // row blocks that a workgroup of the expand takes in turn
-  int64_t v_bytes, vs_bytes, ve_bytes;  // the workspace: partial sums, operands, exponents
+  int per;            // column steps of a workgroup of the expand
   int64_t ws_bytes;
 };
 // routed: with the sorted table of launch_lora_route.
-LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts, bool routed);
+LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int parts, bool routed);
 hipError_t launch_lora_route(const int32_t* ids, int64_t n, int64_t L, int32_t* sorted, int32_t* bucket,
                              int32_t* num_post_pad, int32_t* offsets, hipStream_t s);
 struct LoraParams {

@@ -22,8 +22,7 @@
 //              nothing is sorted, and a kernel waits for two loads in a row
 //              (id, then weights) and no more
 //   batches    16-row blocks of the sorted table
-//   prefill    64-row tiles through LDS in the shrink, and v split once into
-//              MFMA operands by a launch of its own, not by every column group
+//   prefill    64-row tiles, what their waves share staged in LDS
 #include <math.h>
 
 #include <algorithm>
@@ -37,7 +36,22 @@ namespace sgl_awq {
 namespace {
 
 constexpr int kLoraWaves = 4;
+constexpr int kLoraSlices = 4;  // k-slices of the shrink, at most
 constexpr int kStepK = 64;  // k per step of the shrink: 128 bytes of a row
+
+// Loads above stay above: the wait counts of the rings below rely on how many
+// a step issues.
+__device__ __forceinline__ void stay_here() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// A value that no kernel writes while this one runs, at an address all lanes
+// share: a scalar load.
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)(uintptr_t)p;
+}
 
 // Rows of block b (16 of the sorted table, or the one row b), their adapter and
 // their positions in v.
@@ -50,9 +64,31 @@ struct BlockArgs {
 
 template <bool ROWS>
 __device__ __forceinline__ int block_adapter(const BlockArgs& a, int b) {
-  if (!ROWS) return a.bucket[b];
-  const int e = a.ids[b];
+  if (!ROWS) return load_uniform(a.bucket + b);
+  const int e = load_uniform(a.ids + b);
   return e >= 0 && e < a.L ? e : a.L;
+}
+// Prefill: workgroup `id` runs on XCD id % 8.  Each XCD takes neighbouring row
+// tiles, so that it reads few adapters' matrices through its L2 (tiles dealt
+// round, every L2 fetched all of them).  False past the last tile.
+__device__ __forceinline__ bool row_tile(int id, int tiles, int& tile, int& rest) {
+  const int per = (tiles + 7) >> 3, j = id >> 3;
+  rest = j / per;
+  tile = (id & 7) * per + j - rest * per;
+  return tile < tiles;
+}
+int row_tile_workgroups(int64_t tiles, int64_t rest) { return (int)((tiles + 7) / 8 * 8 * rest); }
+
+// The adapters of the four blocks from b, lane m's that of block b + m: 64 rows
+// of the prefill kernels in one load.
+__device__ __forceinline__ int four_adapters(const BlockArgs& a, int b, int lane) {
+  return lane < 4 && b + lane < a.blocks ? a.bucket[b + lane] : -1;
+}
+// Past the blocks of adapter e among them, from block m on.
+__device__ __forceinline__ int blocks_end(int adapters, int e, int m) {
+  int n = m + 1;
+  while (n < 4 && __builtin_amdgcn_readlane(adapters, n) == e) ++n;
+  return n;
 }
 template <bool ROWS>
 __device__ __forceinline__ int block_row(const BlockArgs& a, int b, int c) {
@@ -75,7 +111,9 @@ struct ShrinkArgs {
   int rt;                     // rank tiles of 16 per part
   int tiles;                  // P * rt
   int VR;                     // 16 * tiles
-  int steps;                  // k-steps
+  int steps, slices;          // k-steps, and into how many slices they are cut
+  int row_tiles;              // groups of four blocks (prefill)
+  int positions;              // rows of v
   int64_t v_slice;            // positions * VR
 };
 
@@ -88,11 +126,13 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
 // One rank tile of one block; a wave's share of the k-steps with D - 1 of them
 // in flight, straight from global memory: no other wave reads these k.
 // grid: (blocks, k-slices, rank tiles).
+constexpr int kShrinkWaves = 8;
+
 template <bool ROWS, typename DT>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_kernel(ShrinkArgs a) {
+__global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkArgs a) {
   using V8 = typename DT::vec8;
   constexpr int D = 4;
-  __shared__ f32x4 red[kLoraWaves * 64];
+  __shared__ f32x4 red[kShrinkWaves * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int i = lane & 15, g = lane >> 4;
   const int b = blockIdx.x, q = blockIdx.z;
@@ -101,13 +141,13 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_kernel(ShrinkArgs
   const int sid = block_row<ROWS>(a.b, b, i);
   // A row block waits for the rank, to leave out what lies past it; a single
   // row reads it beside the weights (the expand takes no value past the rank).
-  const int rank = ROWS ? a.R : min(a.ranks[e], a.R);
+  const int rank = ROWS ? a.R : min(load_uniform(a.ranks + e), a.R);
   const __amdgpu_buffer_rsrc_t ar = make_rsrc((const char*)a.a + (int64_t)e * a.a_bytes, a.a_bytes);
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, a.x_bytes);
   const uint32_t ao = a_offset(a, q, i, rank, 16 * g);
   const uint32_t xo = sid >= 0 ? ((uint32_t)sid * (uint32_t)a.K + 16u * g) * 2u : kPastEnd;
   // Slice (blockIdx.y, wave) of the k-steps.
-  const int parts = gridDim.y * kLoraWaves, part = blockIdx.y * kLoraWaves + wave;
+  const int parts = gridDim.y * kShrinkWaves, part = blockIdx.y * kShrinkWaves + wave;
   const int s0 = (int)((int64_t)part * a.steps / parts), s1 = (int)((int64_t)(part + 1) * a.steps / parts);
 
   struct Stage {
@@ -143,7 +183,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_kernel(ShrinkArgs
   if (wave != 0 || (ROWS && i != 0)) return;
   f32x4 s = red[lane];
 #pragma unroll
-  for (int w = 1; w < kLoraWaves; ++w) s += red[w * 64 + lane];
+  for (int w = 1; w < kShrinkWaves; ++w) s += red[w * 64 + lane];
   *(f32x4*)(a.v + blockIdx.y * a.v_slice + (int64_t)(ROWS ? b : b * 16 + i) * a.VR + q * 16 + 4 * g) = s;
 }
 
@@ -151,48 +191,54 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_kernel(ShrinkArgs
 // straight into MFMA operands and the rows shared through a ring of LDS slots
 // filled by LDS-DMA, whole 128-byte lines of a row at a time.  Blocks of
 // different adapters in the four are taken in turn, the others' rows as zeros.
-// grid: (groups of four blocks, k-slices, groups of 4 RT rank tiles).
+// grid: (groups of four blocks and k-slices, groups of 4 RT rank tiles).
 constexpr int kShrinkRows = 64;
-constexpr int kShrinkSlots = 4;
+constexpr int shrink_slots(int rt) { return rt <= 2 ? 6 : 4; }
 
 template <int RT, typename DT>
 __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_tile_kernel(ShrinkArgs a) {
   using V8 = typename DT::vec8;
-  constexpr int D = kShrinkSlots - 1;       // steps in flight ahead of the multiply
+  constexpr int SLOTS = shrink_slots(RT);
+  constexpr int D = SLOTS - 1;              // steps in flight ahead of the multiply
   constexpr int VECS = kShrinkRows * 8;     // 16-byte vectors of a slot
   constexpr int LOADS = 2 + 2 * RT;         // a wave's loads of a step
   extern __shared__ u32x4 xs[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
-  const int q0 = (blockIdx.z * kLoraWaves + wave) * RT;
-  const int s0 = (int)((int64_t)blockIdx.y * a.steps / gridDim.y);
-  const int s1 = (int)((int64_t)(blockIdx.y + 1) * a.steps / gridDim.y);
+  const int slice = blockIdx.x / a.row_tiles, tile = blockIdx.x - slice * a.row_tiles;
+  const int q0 = (blockIdx.y * kLoraWaves + wave) * RT;
+  const int s0 = (int)((int64_t)slice * a.steps / a.slices);
+  const int s1 = (int)((int64_t)(slice + 1) * a.steps / a.slices);
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, a.x_bytes);
   // The DMA's lanes: row lane / 8 of eight, the vector that its place holds.
   const int kq = ((lane & 7) ^ (lane >> 3)) * 8;
-  const int b1 = min((int)(blockIdx.x + 1) * 4, a.b.blocks);
-  for (int b = blockIdx.x * 4; b < b1;) {
-    const int e = a.b.bucket[b];
+  const int b0 = tile * 4, adapters = four_adapters(a.b, b0, lane);
+  int sids[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const int pos = b0 * 16 + (n * kLoraWaves + wave) * 8 + (lane >> 3);
+    sids[n] = pos < a.positions ? a.b.sorted[pos] : -1;
+  }
+  for (int m0 = 0; m0 < 4;) {
+    const int e = __builtin_amdgcn_readlane(adapters, m0);
     if (e < 0 || e >= a.b.L) break;  // none and past the end are the last ones
-    int bn = b + 1;
-    while (bn < b1 && a.b.bucket[bn] == e) ++bn;
-    const int rank = min(a.ranks[e], a.R);
+    const int m1 = blocks_end(adapters, e, m0);
+    const int rank = min(load_uniform(a.ranks + e), a.R);
     const __amdgpu_buffer_rsrc_t ar = make_rsrc((const char*)a.a + (int64_t)e * a.a_bytes, a.a_bytes);
     uint32_t ao[RT], xo[2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) ao[t] = a_offset(a, q0 + t, c, rank, 8 * g);
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      const int pos = blockIdx.x * kShrinkRows + (n * kLoraWaves + wave) * 8 + (lane >> 3);
-      const int sid = pos >= 16 * b && pos < 16 * bn ? a.b.sorted[pos] : -1;
+      const int m = (n * kLoraWaves + wave) >> 1, sid = m >= m0 && m < m1 ? sids[n] : -1;
       xo[n] = sid >= 0 && sid < a.b.M ? ((uint32_t)sid * (uint32_t)a.K + (uint32_t)kq) * 2u : kPastEnd;
     }
     u32x4 aw[D + 1][RT][2];
     auto issue = [&](u32x4 (&w)[RT][2], int s, int slot) {
       const uint32_t dead = s < s1 && s * kStepK + kq < a.K ? 0u : kPastEnd;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-        load_lds16(xr, xs + slot * VECS + (n * kLoraWaves + wave) * 64, xo[n] | dead, s * kStepK * 2);
+      for (int i = 0; i < 2; ++i)
+        load_lds16(xr, xs + slot * VECS + (i * kLoraWaves + wave) * 64, xo[i] | dead, s * kStepK * 2);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -201,7 +247,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_tile_kernel(Shrin
         for (int t = 0; t < RT; ++t)
           w[t][h] = __builtin_amdgcn_raw_buffer_load_b128(ar, (ao[t] + 64u * h) | gone, s * kStepK * 2, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      stay_here();
     };
     f32x4 acc[RT][4];
 #pragma unroll
@@ -213,38 +259,35 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_tile_kernel(Shrin
     // wave is done with the slot that step s + D takes -- and issue that one.
 #pragma unroll
     for (int p = 0; p < D; ++p) issue(aw[p], s0 + p, p);
-    [&] {
-      for (int s = s0;;) {
+    for (int s = s0; s < s1; s += SLOTS) {  // (steps past the slice multiply zeros)
 #pragma unroll
-        for (int d = 0; d <= D; ++d) {
-          __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm((D - 1) * LOADS));
-          __builtin_amdgcn_s_barrier();
-          __builtin_amdgcn_sched_barrier(0);
-          issue(aw[(d + D) % (D + 1)], s + D, (d + D) % (D + 1));
+      for (int d = 0; d <= D; ++d) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm((D - 1) * LOADS));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(aw[(d + D) % (D + 1)], s + d + D, (d + D) % (D + 1));
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const V8 x = __builtin_bit_cast(V8, xs[d * VECS + (16 * m + c) * 8 + ((4 * h + g) ^ (c & 7))]);
+          for (int m = 0; m < 4; ++m) {
+            const V8 x = __builtin_bit_cast(V8, xs[d * VECS + (16 * m + c) * 8 + ((4 * h + g) ^ (c & 7))]);
 #pragma unroll
-              for (int t = 0; t < RT; ++t) acc[t][m] = mfma16x16x32(__builtin_bit_cast(V8, aw[d][t][h]), x, acc[t][m]);
-            }
-          if (++s >= s1) return;
-        }
+            for (int t = 0; t < RT; ++t) acc[t][m] = mfma16x16x32(__builtin_bit_cast(V8, aw[d][t][h]), x, acc[t][m]);
+          }
       }
-    }();
+    }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     __syncthreads();  // before the ring is filled again
-    float* v = a.v + blockIdx.y * a.v_slice;
+    float* v = a.v + slice * a.v_slice;
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const int blk = blockIdx.x * 4 + m;
-      if (blk < b || blk >= bn) continue;
+      if (m < m0 || m >= m1) continue;
 #pragma unroll
       for (int t = 0; t < RT; ++t)
-        if (q0 + t < a.tiles) *(f32x4*)(v + (int64_t)(blk * 16 + c) * a.VR + (q0 + t) * 16 + 4 * g) = acc[t][m];
+        if (q0 + t < a.tiles)
+          *(f32x4*)(v + (int64_t)((b0 + m) * 16 + c) * a.VR + (q0 + t) * 16 + 4 * g) = acc[t][m];
     }
-    b = bn;
+    m0 = m1;
   }
 }
 
@@ -261,7 +304,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_tile_kernel(Shrin
 struct VArgs {
   const float* v;    // partial sums [slices][positions][VR]
   int64_t v_slice;
-  int slices, VR, rp;  // rp: ranks of a part in v, a multiple of 16
+  int positions, slices, VR, rp;  // rp: ranks of a part in v, a multiple of 16
 };
 
 // The lane's row of a part: 8 consecutive ranks of each 32, the k-slices added in order.
@@ -272,9 +315,21 @@ __device__ __forceinline__ void load_v(const VArgs& a, int64_t pos, int part, in
   for (int k = 0; k < KC; ++k) {
     v[k][0] = v[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (32 * k + 8 * g >= limit) continue;
-    for (int s = 0; s < a.slices; ++s) {
-      v[k][0] += *(const f32x4*)(p + s * a.v_slice + 32 * k);
-      v[k][1] += *(const f32x4*)(p + s * a.v_slice + 32 * k + 4);
+    // All in flight at once: one by one a wave waited for each in turn.
+    f32x4 t[kLoraSlices][2];
+#pragma unroll
+    for (int s = 0; s < kLoraSlices; ++s) {
+      if (s < a.slices) {
+        t[s][0] = *(const f32x4*)(p + s * a.v_slice + 32 * k);
+        t[s][1] = *(const f32x4*)(p + s * a.v_slice + 32 * k + 4);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < kLoraSlices; ++s) {
+      if (s < a.slices) {
+        v[k][0] += t[s][0];
+        v[k][1] += t[s][1];
+      }
     }
   }
 }
@@ -307,45 +362,12 @@ __device__ __forceinline__ int split_v(const f32x4 (&v)[KC][2], int rank, int g,
   return ex;
 }
 
-// Prefill: the operands of every block and part, once.  One wave each:
-// vs[(block P + part) KC + k][hi, lo][lane], ve[(block P + part) 16 + row].
-struct SplitArgs {
-  BlockArgs b;
-  VArgs v;
-  const int32_t* ranks;
-  u32x4* vs;
-  int32_t* ve;
-  int P, R;
-};
-
-template <int KC, typename DT>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_split_kernel(SplitArgs a) {
-  const int unit = blockIdx.x * kLoraWaves + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int b = unit / a.P, p = unit - b * a.P, c = lane & 15, g = lane >> 4;
-  if (b >= a.b.blocks) return;
-  const int e = a.b.bucket[b];
-  if (e < 0 || e >= a.b.L) return;
-  const int rank = min(a.ranks[e], a.R);
-  f32x4 v[KC][2];
-  typename DT::vec8 hi[KC], lo[KC];
-  load_v<KC>(a.v, b * 16 + c, p, rank, g, v);
-  const int ex = split_v<KC, DT>(v, rank, g, hi, lo);
-#pragma unroll
-  for (int k = 0; k < KC; ++k) {
-    a.vs[((int64_t)unit * KC + k) * 128 + lane] = __builtin_bit_cast(u32x4, hi[k]);
-    a.vs[((int64_t)unit * KC + k) * 128 + 64 + lane] = __builtin_bit_cast(u32x4, lo[k]);
-  }
-  if (g == 0) a.ve[unit * 16 + c] = ex;
-}
-
 // ---------------------------------------------------------------------------
 // Expand.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
   BlockArgs b;
   VArgs v;
-  const u32x4* vs;  // operands from lora_split_kernel (prefill)
-  const int32_t* ve;
   const void* y;
   void* out;
   const void* w;    // B
@@ -353,17 +375,18 @@ struct ExpandArgs {
   const int32_t* ranks;
   uint32_t w_bytes;  // one adapter's B (below 2^31)
   int N, R, P;
-  int per;           // row blocks that a workgroup takes in turn
   int inplace;       // out is y: rows without an adapter stay as they are
+  int per;           // column steps of a group
   int groups;        // column groups
+  int row_tiles;     // groups of four row blocks (prefill)
   int col[kLoraParts + 1];    // first column of each part
   int group[kLoraParts + 1];  // first column group of each part
 };
 
 // One wave's columns: 16 CT of each of H ranges (gate and up with an
 // activation).  Column j of MFMA tile t of the group is column
-// 4 CT (j / 4) + 4 t + j % 4, so that lane (row, g) holds 4 CT consecutive
-// columns of its row.
+// 32 (t / 2) + 8 (j / 4) + 4 (t % 2) + j % 4, so that lane (row, g) holds the 8
+// columns from 8 g of every 32, and the four lanes of a row 64 bytes in a row.
 template <int KC, int CT, int ACT, typename DT>
 struct ExpandCols {
   using E = typename DT::elem;
@@ -374,16 +397,19 @@ struct ExpandCols {
   const ExpandArgs& a;
   int c, g, part, base, end, half, ncols;
 
-  __device__ __forceinline__ ExpandCols(const ExpandArgs& args, int grp, int lane)
+  // Group `grp` of `per` times 16 CT columns.
+  __device__ __forceinline__ ExpandCols(const ExpandArgs& args, int grp, int lane, int per)
       : a(args), c(lane & 15), g(lane >> 4), part(0) {
     if (H == 1)
       while (part + 1 < kLoraParts && grp >= a.group[part + 1]) ++part;
-    base = a.col[part] + (grp - a.group[part]) * 16 * CT;
+    base = a.col[part] + (grp - a.group[part]) * per * 16 * CT;
     end = a.col[part + 1];
     half = a.N >> 1;
     ncols = H == 1 ? a.N : half;
   }
-  __device__ __forceinline__ int first(int q) const { return base + 4 * CT * g + 8 * q; }
+  __device__ __forceinline__ int first(int q) const { return base + 32 * q + 8 * g; }
+  // Column j of tile t, from the group's first.
+  static __device__ __forceinline__ int column(int t, int j) { return 32 * (t >> 1) + 8 * (j >> 2) + 4 * (t & 1) + (j & 3); }
 
   __device__ __forceinline__ void load_y(int sid, u32x4 (&y)[H][VEC]) const {
 #pragma unroll
@@ -403,7 +429,7 @@ struct ExpandCols {
     for (int h = 0; h < H; ++h)
 #pragma unroll
       for (int t = 0; t < CT; ++t) {
-        const int n = base + 4 * CT * (c >> 2) + 4 * t + (c & 3);
+        const int n = base + column(t, c);
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
           const int r0 = 32 * k + 8 * g;
@@ -415,7 +441,7 @@ struct ExpandCols {
   }
 
   // Zeros in place of what lies at and past the rank.
-  __device__ __forceinline__ void cut_b(int rank, u32x4 (&w)[H][CT][KC]) const {
+  __device__ __forceinline__ void cut(int rank, u32x4 (&w)[CT][KC]) const {
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
       const int live = rank - (32 * k + 8 * g);
@@ -423,9 +449,7 @@ struct ExpandCols {
       for (int i = 0; i < 4; ++i) {
         const uint32_t m = live >= 2 * i + 2 ? ~0u : live == 2 * i + 1 ? 0xFFFFu : 0u;
 #pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-          for (int t = 0; t < CT; ++t) w[h][t][k][i] &= m;
+        for (int t = 0; t < CT; ++t) w[t][k][i] &= m;
       }
     }
   }
@@ -444,28 +468,29 @@ struct ExpandCols {
       for (int t = 0; t < CT; ++t) acc[t] = mfma16x16x32(__builtin_bit_cast(V8, w[t][k]), hi[k], acc[t]);
   }
 
-  // Bring the products back and scale them.
-  static __device__ __forceinline__ void scale(f32x4 (&acc)[CT], int ex, float s) {
+  // y plus f times the products, f the scaling and the power of two that
+  // brings them back.
+  __device__ __forceinline__ void combine(int q, const u32x4 (&y)[H][VEC], const f32x4 (&acc)[H][CT],
+                                          const float (&f)[H], V8& r) const {
+
+    const V8 y0 = __builtin_bit_cast(V8, y[0][q]), y1 = __builtin_bit_cast(V8, y[H - 1][q]);
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_ldexpf(acc[t][i], ex) * s;
+    for (int i = 0; i < 8; ++i) {
+      const int t = 2 * q + (i >> 2);
+      const float v = __builtin_fmaf(acc[0][t][i & 3], f[0], (float)y0[i]);
+      if constexpr (ACT == kActNone)
+        r[i] = (E)v;
+      else
+        r[i] = (E)(gated_act_fast(ACT, v) * __builtin_fmaf(acc[H - 1][t][i & 3], f[H - 1], (float)y1[i]));
+    }
   }
 
-  __device__ __forceinline__ void store(int sid, const u32x4 (&y)[H][VEC], const f32x4 (&acc)[H][CT]) const {
+  __device__ __forceinline__ void store(int sid, const u32x4 (&y)[H][VEC], const f32x4 (&acc)[H][CT],
+                                        const float (&f)[H]) const {
 #pragma unroll
     for (int q = 0; q < VEC; ++q) {
       V8 r;
-      const V8 y0 = __builtin_bit_cast(V8, y[0][q]), y1 = __builtin_bit_cast(V8, y[H - 1][q]);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = 2 * q + (i >> 2);
-        const float f = (float)y0[i] + acc[0][t][i & 3];
-        if constexpr (ACT == kActNone)
-          r[i] = (E)f;
-        else
-          r[i] = (E)(gated_act_fast(ACT, f) * ((float)y1[i] + acc[H - 1][t][i & 3]));
-      }
+      combine(q, y, acc, f, r);
       if (sid >= 0 && first(q) < end) *(V8*)((E*)a.out + (int64_t)sid * ncols + first(q)) = r;
     }
   }
@@ -483,7 +508,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs
   const int wgs = (a.groups + kLoraWaves - 1) / kLoraWaves;
   const int b = blockIdx.x / wgs, grp = (blockIdx.x - b * wgs) * kLoraWaves + wave;
   if (grp >= a.groups) return;
-  const Cols cols(a, grp, lane);
+  const Cols cols(a, grp, lane, 1);
   u32x4 y[H][Cols::VEC];
   f32x4 v[H][KC][2];
   if (ROWS) {
@@ -498,148 +523,178 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs
   const int sid = block_row<ROWS>(a.b, b, cols.c);
   if (!ROWS) cols.load_y(sid, y);
   f32x4 acc[H][CT];
+  float f[H];
 #pragma unroll
-  for (int h = 0; h < H; ++h)
+  for (int h = 0; h < H; ++h) {
+    f[h] = 0.f;
 #pragma unroll
     for (int t = 0; t < CT; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   if (adapter) {
     u32x4 w[H][CT][KC];
     if (ROWS) cols.load_b(e, a.R, w);
-    const int rank = min(a.ranks[e], a.R);
+    const int rank = min(load_uniform(a.ranks + e), a.R);
+    const float scale = load_uniform(a.scaling + e);
     if (!ROWS) {
       cols.load_b(e, rank, w);
 #pragma unroll
       for (int h = 0; h < H; ++h) load_v<KC>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
     }
-    if ((ROWS && rank < a.R) || (rank & 7)) cols.cut_b(rank, w);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
+      if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
       typename DT::vec8 hi[KC], lo[KC];
-      const int ex = split_v<KC, DT>(v[h], rank, cols.g, hi, lo);
+      f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi, lo));
       Cols::mul(w[h], hi, lo, acc[h]);
-      Cols::scale(acc[h], ex, a.scaling[e]);
     }
   }
-  cols.store(sid, y, acc);
+  cols.store(sid, y, acc, f);
 }
 
-// Prefill: v comes as operands, and what block b + 1 reads is in flight while
-// block b is computed.
-template <int KC, int CT, int ACT, typename DT>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_tile_kernel(ExpandArgs a) {
+// Prefill: a workgroup is four row blocks, one a wave, and `per` steps of 64
+// columns (32 gate and their 32 up ones).  A wave's v becomes MFMA operands
+// once; the columns' rows of B come through a ring of LDS slots filled by
+// LDS-DMA, shared by the waves, and y into registers, both D steps ahead.
+// Blocks of different adapters in the four are taken in turn.
+constexpr int kExpandSlots = 4;
+
+template <int KC, int ACT, typename DT>
+__global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_tile_kernel(ExpandArgs a) {
+  constexpr int CT = kLoraColTiles / (ACT == kActNone ? 1 : 2);
   using Cols = ExpandCols<KC, CT, ACT, DT>;
   using V8 = typename DT::vec8;
-  constexpr int H = Cols::H;
+  constexpr int H = Cols::H, VEC = Cols::VEC;
+  constexpr int D = kExpandSlots - 1;
+  constexpr int PL = 4 * KC;              // 16-byte places of a column in a slot
+  constexpr int VECS = 64 * PL;           // ... and of a slot
+  constexpr int LOADS = KC + H * VEC;     // a wave's loads of a step
+  extern __shared__ u32x4 bs[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int wgs = (a.groups + kLoraWaves - 1) / kLoraWaves;
-  const int rows = blockIdx.x / wgs, grp = (blockIdx.x - rows * wgs) * kLoraWaves + wave;
-  if (grp >= a.groups) return;
-  const Cols cols(a, grp, lane);
-  const int b0 = rows * a.per, b1 = min(b0 + a.per, a.b.blocks);
-
-  struct Stage {
-    int e, sid;
-    u32x4 y[H][Cols::VEC];
-    u32x4 v[H][KC][2];
-    int ex[H];
-  };
-  auto find = [&](Stage& s, int b) {
-    s.e = b < b1 ? a.b.bucket[b] : -1;
-    if (H == 1 && a.inplace && s.e >= a.b.L) s.e = -1;  // the rows without an adapter are the last ones
-    s.sid = s.e >= 0 ? block_row<false>(a.b, b, cols.c) : -1;
-  };
-  auto load = [&](Stage& s, int b) {
-    cols.load_y(s.sid, s.y);
-    if (s.e < 0 || s.e >= a.b.L) return;
+  int tile, chunk;
+  if (!row_tile(blockIdx.x, a.row_tiles, tile, chunk)) return;
+  const int b0 = tile * 4;
+  Cols cols(a, chunk, lane, a.per);
+  const int c = cols.c, g = cols.g, base = cols.base;
+  const int steps = min(a.per, (cols.end - base + 16 * CT - 1) / (16 * CT));
+  // Place p of slot row r holds the vector p ^ swap(r) of its column: reads of
+  // one vector of 8 rows meet all banks.
+  auto swap = [](int r) { return KC == 1 ? (r >> 1) & 3 : r & 7; };
+  // What does not hang on the adapter is loaded beside it.
+  const int adapters = four_adapters(a.b, b0, lane);
+  const int pos = (b0 + wave) * 16 + c;
+  const bool have = pos < a.v.positions;
+  const int mine = have ? a.b.sorted[pos] : -1;
+  V8 hi[H][KC], lo[H][KC];
+  float f[H];
+  {
+    f32x4 v[H][KC][2];
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const int unit = b * a.P + (H == 1 ? cols.part : h);
+    for (int h = 0; h < H; ++h) load_v<KC>(a.v, have ? pos : 0, H == 1 ? cols.part : h, a.R, g, v[h]);
+    const int e = __builtin_amdgcn_readlane(adapters, wave);  // of the wave's own block
+    const bool adapter = e >= 0 && e < a.b.L;
+    const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
+    const float scale = adapter ? load_uniform(a.scaling + e) : 0.f;
+#pragma unroll
+    for (int h = 0; h < H; ++h) f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, g, hi[h], lo[h]));
+  }
+
+  for (int m0 = 0; m0 < 4;) {
+    const int e = __builtin_amdgcn_readlane(adapters, m0);
+    if (e < 0) break;  // past the last block
+    const bool adapter = e < a.b.L;
+    if (!adapter && H == 1 && a.inplace) break;  // the rows without an adapter are the last ones
+    const int m1 = blocks_end(adapters, e, m0);
+    const int sid = wave >= m0 && wave < m1 && mine < a.b.M ? mine : -1;
+    const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
+    const __amdgpu_buffer_rsrc_t br = make_rsrc((const char*)a.w + (int64_t)(adapter ? e : 0) * a.w_bytes, a.w_bytes);
+
+    // The wave's places in a slot, and what it fills them with at step 0.
+    uint32_t bo[KC];
+    int bn0[KC];
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const int u = (k * kLoraWaves + wave) * 64 + lane, r = u / PL, i = r & 15, t = r >> 4;
+      const int r0 = ((u % PL) ^ swap(r)) * 8;
+      bn0[k] = base + Cols::column(t % CT, i);
+      bo[k] = r0 < rank ? ((uint32_t)(t / CT * cols.half + bn0[k]) * (uint32_t)a.R + (uint32_t)r0) * 2u : kPastEnd;
+    }
+    const typename DT::elem* yrow = (const typename DT::elem*)a.y + (int64_t)max(sid, 0) * a.N;
+    u32x4 y[D + 1][H][VEC];
+    auto issue = [&](u32x4 (&v)[H][VEC], int s, int slot) {
 #pragma unroll
       for (int k = 0; k < KC; ++k) {
-        s.v[h][k][0] = a.vs[((int64_t)unit * KC + k) * 128 + lane];
-        s.v[h][k][1] = a.vs[((int64_t)unit * KC + k) * 128 + 64 + lane];
+        const uint32_t dead = bn0[k] + s * 16 * CT < cols.end ? 0u : kPastEnd;
+        load_lds16(br, bs + slot * VECS + (k * kLoraWaves + wave) * 64, bo[k] | dead, s * 16 * CT * a.R * 2);
       }
-      s.ex[h] = a.ve[unit * 16 + cols.c];
-    }
-  };
-  u32x4 w[H][CT][KC];
-  int prev = -1;
-  float scale = 0.f;
-  auto work = [&](const Stage& s) {
-    f32x4 acc[H][CT];
-    if (s.e < a.b.L) {
-      if (s.e != prev) {
-        prev = s.e;
-        const int rank = min(a.ranks[prev], a.R);
-        scale = a.scaling[prev];
-        cols.load_b(prev, rank, w);
-        if (rank & 7) cols.cut_b(rank, w);
-      }
-#pragma unroll
-      for (int h = 0; h < H; ++h) {
-        V8 hi[KC], lo[KC];
-#pragma unroll
-        for (int k = 0; k < KC; ++k) {
-          hi[k] = __builtin_bit_cast(V8, s.v[h][k][0]);
-          lo[k] = __builtin_bit_cast(V8, s.v[h][k][1]);
-        }
-        Cols::mul(w[h], hi, lo, acc[h]);
-        Cols::scale(acc[h], s.ex[h], scale);
-      }
-    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      // Past the last column the lane's loads repeat it, so that every wave counts the same loads.
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int t = 0; t < CT; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    cols.store(s.sid, s.y, acc);
-  };
-
-  Stage st[2];
-  find(st[0], b0);
-  if (st[0].e < 0) return;
-  load(st[0], b0);
-  find(st[1], b0 + 1);
-  for (int b = b0;;) {
+        for (int q = 0; q < VEC; ++q)
+          v[h][q] = *(const u32x4*)(yrow + h * cols.half + min(base + s * 16 * CT + 32 * q + 8 * g, cols.end - 8));
+      stay_here();
+    };
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
-      Stage next;
-      load(st[1 - d], b + 1);
-      find(next, b + 2);
-      work(st[d]);
-      if (st[1 - d].e < 0) return;
-      st[d].e = next.e;
-      st[d].sid = next.sid;
-      ++b;
+    for (int p = 0; p < D; ++p) issue(y[p], p, p);
+    // Step s: wait until its loads have landed (those of the D - 1 steps after
+    // it may be in flight), meet the other waves and issue step s + D into the
+    // slot that every wave is done with.  Steps past the last store nothing.
+    for (int s0 = 0; s0 < steps; s0 += kExpandSlots) {
+#pragma unroll
+      for (int d = 0; d <= D; ++d) {
+        const int s = s0 + d;
+        __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm((D - 1) * LOADS));
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(y[(d + D) % (D + 1)], s + D, (d + D) % (D + 1));
+        f32x4 acc[H][CT];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          u32x4 w[CT][KC];
+#pragma unroll
+          for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+              w[t][k] = bs[d * VECS + ((h * CT + t) * 16 + c) * PL + ((4 * k + g) ^ swap(c))];
+          if (rank & 7) cols.cut(rank, w);
+          Cols::mul(w, hi[h], lo[h], acc[h]);
+        }
+        cols.base = base + s * 16 * CT;
+        cols.store(sid, y[d], acc, f);
+      }
     }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __syncthreads();  // before the ring is filled again
+    m0 = m1;
   }
 }
 
 template <int KC, int ACT, typename DT>
-hipError_t launch_expand(const ExpandArgs& a, int mode, dim3 grid, hipStream_t s) {
+hipError_t launch_expand(const ExpandArgs& a, int mode, hipStream_t s) {
   constexpr int CT = kLoraColTiles / (ACT == kActNone ? 1 : 2);
   const dim3 block(64 * kLoraWaves);
+  if constexpr (KC <= 4) {
+    if (mode == kLoraTiles) {
+      constexpr int lds = kExpandSlots * 64 * 4 * KC * 16;
+      hipLaunchKernelGGL((lora_expand_tile_kernel<KC, ACT, DT>),
+                         dim3((unsigned)row_tile_workgroups(a.row_tiles, a.groups)), block, lds, s, a);
+      return hipGetLastError();
+    }
+  }
+  const dim3 grid((unsigned)((a.groups + kLoraWaves - 1) / kLoraWaves * a.b.blocks));
   if (mode == kLoraRows)
     hipLaunchKernelGGL((lora_expand_kernel<true, KC, CT, ACT, DT>), grid, block, 0, s, a);
-  else if (mode == kLoraBlocks)
-    hipLaunchKernelGGL((lora_expand_kernel<false, KC, CT, ACT, DT>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((lora_expand_tile_kernel<KC, CT, ACT, DT>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((lora_expand_kernel<false, KC, CT, ACT, DT>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 
 template <int KC, typename DT>
-hipError_t launch_split_expand(const SplitArgs& sp, const ExpandArgs& a, int mode, int act, dim3 grid, hipStream_t s) {
-  if (mode == kLoraTiles) {
-    const int64_t units = (int64_t)sp.b.blocks * sp.P;
-    hipLaunchKernelGGL((lora_split_kernel<KC, DT>), dim3((unsigned)((units + kLoraWaves - 1) / kLoraWaves)),
-                       dim3(64 * kLoraWaves), 0, s, sp);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  if (act == kActSilu) return launch_expand<KC, kActSilu, DT>(a, mode, grid, s);
-  if (act == kActGelu) return launch_expand<KC, kActGelu, DT>(a, mode, grid, s);
-  return launch_expand<KC, kActNone, DT>(a, mode, grid, s);
+hipError_t launch_expand_act(const ExpandArgs& a, int mode, int act, hipStream_t s) {
+  if (act == kActSilu) return launch_expand<KC, kActSilu, DT>(a, mode, s);
+  if (act == kActGelu) return launch_expand<KC, kActGelu, DT>(a, mode, s);
+  return launch_expand<KC, kActNone, DT>(a, mode, s);
 }
 
 template <typename DT>
@@ -649,16 +704,17 @@ hipError_t launch_shrink(const ShrinkArgs& a, const LoraPlan& p, hipStream_t s) 
   if (p.mode != kLoraTiles) {
     const dim3 grid((unsigned)p.blocks, ks, (unsigned)a.tiles);
     if (p.mode == kLoraRows)
-      hipLaunchKernelGGL((lora_shrink_kernel<true, DT>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((lora_shrink_kernel<true, DT>), grid, dim3(64 * kShrinkWaves), 0, s, a);
     else
-      hipLaunchKernelGGL((lora_shrink_kernel<false, DT>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((lora_shrink_kernel<false, DT>), grid, dim3(64 * kShrinkWaves), 0, s, a);
     return hipGetLastError();
   }
   const int rt = p.rank_tiles;
-  const dim3 grid((unsigned)((p.blocks + 3) / 4), ks, (unsigned)((a.tiles + kLoraWaves * rt - 1) / (kLoraWaves * rt)));
-  constexpr int lds = kShrinkSlots * kShrinkRows * 128;
+  const dim3 grid((unsigned)(a.row_tiles * p.slices),
+                  (unsigned)((a.tiles + kLoraWaves * rt - 1) / (kLoraWaves * rt)));
 #define SGL_TILE(RT_) \
-  if (rt == RT_) hipLaunchKernelGGL((lora_shrink_tile_kernel<RT_, DT>), grid, block, lds, s, a)
+  if (rt == RT_)      \
+  hipLaunchKernelGGL((lora_shrink_tile_kernel<RT_, DT>), grid, block, shrink_slots(RT_) * kShrinkRows * 128, s, a)
   SGL_TILE(1);
   SGL_TILE(2);
   SGL_TILE(3);
@@ -667,15 +723,14 @@ hipError_t launch_shrink(const ShrinkArgs& a, const LoraPlan& p, hipStream_t s) 
   return hipGetLastError();
 }
 
-int rank_chunks(int64_t R) { return R <= 32 ? 1 : R <= 64 ? 2 : R <= 128 ? 4 : 8; }
-
 }  // namespace
 
-LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts, bool routed) {
+LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int parts, bool routed) {
   LoraPlan p{};
   const int cus = device_cu_count();
   const int tiles = parts * (int)((R + 15) / 16);
-  p.mode = !routed ? kLoraRows : M < kLoraTileRows ? kLoraBlocks : kLoraTiles;
+  // (Ranks beyond 128 leave the prefill kernels too few registers.)
+  p.mode = !routed ? kLoraRows : M < kLoraTileRows || R > 128 ? kLoraBlocks : kLoraTiles;
   const int64_t cap = moe_sorted_capacity(M, L + 1, kLoraBlock);
   // A block holds a row at least.
   p.blocks = routed ? std::min(moe_block_capacity(M, L + 1, kLoraBlock), M) : M;
@@ -684,19 +739,24 @@ LoraPlan plan_lora(int64_t M, int64_t K, int64_t L, int64_t R, int parts, bool r
   const int per = p.mode == kLoraTiles ? kLoraWaves * p.rank_tiles : 1;
   const int64_t wgs = (int64_t)((tiles + per - 1) / per) * (p.mode == kLoraTiles ? (p.blocks + 3) / 4 : p.blocks);
   const int64_t steps = (K + kStepK - 1) / kStepK;
-  // Two workgroups a CU, two steps a wave at least, and no more than eight partial sums.
-  p.slices = (int)std::max<int64_t>(
-      1, std::min<int64_t>({8, steps / (p.mode == kLoraTiles ? 8 : 2 * kLoraWaves), (2 * cus + wgs - 1) / wgs}));
-  p.per = p.mode == kLoraTiles ? 8 : 1;
-  p.v_bytes = (int64_t)p.slices * p.positions * tiles * 16 * 4;
-  p.vs_bytes = p.mode == kLoraTiles ? p.blocks * parts * rank_chunks(R) * 2048 : 0;
-  p.ve_bytes = p.mode == kLoraTiles ? p.blocks * parts * 16 * 4 : 0;
-  p.ws_bytes = p.v_bytes + p.vs_bytes + p.ve_bytes;
+  // Two workgroups a CU, eight (tiles) or two steps a wave at least, and no more than kLoraSlices partial sums.
+  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({kLoraSlices, steps / (p.mode == kLoraTiles ? 8 : 2 * kShrinkWaves),
+                                                          (2 * cus + wgs - 1) / wgs}));
+  p.per = 1;
+  if (p.mode == kLoraTiles) {
+    // A workgroup waits for its rows, v and the first columns once (as long as
+    // 5 to 8 steps take) however many steps it has, so they are many, as far as
+    // two workgroups a CU remain (8192 rows, rank 64, N = 6144 / 4096 / 28672
+    // gated: 24 steps 72 / 52 / 228 us, 16 71 / 51 / 243, 8 75 / 52 / 304).
+    const int64_t row_tiles = (p.blocks + 3) / 4;
+    for (p.per = 24; p.per > 4 && row_tiles * ((N + 64 * p.per - 1) / (64 * p.per)) < 2 * cus;) p.per -= 4;
+  }
+  p.ws_bytes = (int64_t)p.slices * p.positions * tiles * 16 * 4;
   return p;
 }
 
 hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
-  const LoraPlan plan = plan_lora(p.M, p.K, p.L, p.R, p.parts, p.sorted != nullptr);
+  const LoraPlan plan = plan_lora(p.M, p.N, p.K, p.L, p.R, p.parts, p.sorted != nullptr);
   const int rt = (int)((p.R + 15) / 16), tiles = p.parts * rt;
   ShrinkArgs a{};
   a.b.ids = p.ids;
@@ -717,6 +777,9 @@ hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
   a.tiles = tiles;
   a.VR = 16 * tiles;
   a.steps = (int)((p.K + kStepK - 1) / kStepK);
+  a.slices = plan.slices;
+  a.row_tiles = (int)((plan.blocks + 3) / 4);
+  a.positions = (int)plan.positions;
   a.v_slice = plan.positions * a.VR;
   const hipError_t st = p.dtype == 0 ? launch_shrink<F16>(a, plan, s) : launch_shrink<BF16>(a, plan, s);
   if (st != hipSuccess) return st;
@@ -725,13 +788,10 @@ hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
   x.b = a.b;
   x.v.v = a.v;
   x.v.v_slice = a.v_slice;
+  x.v.positions = (int)plan.positions;
   x.v.slices = plan.slices;
   x.v.VR = a.VR;
   x.v.rp = 16 * rt;
-  u32x4* vs = (u32x4*)((char*)p.ws + plan.v_bytes);
-  int32_t* ve = (int32_t*)((char*)p.ws + plan.v_bytes + plan.vs_bytes);
-  x.vs = vs;
-  x.ve = ve;
   x.y = p.y;
   x.out = p.out;
   x.w = p.b;
@@ -743,7 +803,8 @@ hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
   x.P = p.parts;
   x.per = plan.per;
   x.inplace = p.out == p.y;
-  const int cols = 16 * kLoraColTiles / (p.act ? 2 : 1);
+  x.row_tiles = a.row_tiles;
+  const int cols = plan.per * 16 * kLoraColTiles / (p.act ? 2 : 1);
   for (int i = 0, c = 0, n = 0; i <= kLoraParts; ++i) {
     // With an activation the groups cover the gate half and its up columns.
     const int width = i < p.parts ? (int)p.part_cols[i] : 0;
@@ -754,17 +815,12 @@ hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
     n += (width + cols - 1) / cols;
     x.groups = n;
   }
-  const SplitArgs sp{a.b, x.v, p.ranks, vs, ve, p.parts, a.R};
-  const dim3 grid((unsigned)((x.groups + kLoraWaves - 1) / kLoraWaves * ((plan.blocks + x.per - 1) / x.per)));
-#define SGL_KC(KC_)                                                                    \
-  (p.dtype == 0 ? launch_split_expand<KC_, F16>(sp, x, plan.mode, p.act, grid, s)      \
-                : launch_split_expand<KC_, BF16>(sp, x, plan.mode, p.act, grid, s))
-  switch (rank_chunks(p.R)) {
-    case 1: return SGL_KC(1);
-    case 2: return SGL_KC(2);
-    case 4: return SGL_KC(4);
-    default: return SGL_KC(8);
-  }
+#define SGL_KC(KC_) \
+  (p.dtype == 0 ? launch_expand_act<KC_, F16>(x, plan.mode, p.act, s) : launch_expand_act<KC_, BF16>(x, plan.mode, p.act, s))
+  if (p.R <= 32) return SGL_KC(1);
+  if (p.R <= 64) return SGL_KC(2);
+  if (p.R <= 128) return SGL_KC(4);
+  return SGL_KC(8);
 #undef SGL_KC
 }
 

@@ -179,8 +179,12 @@ struct AlignLds {
   int wtot[kAlignWaves];
 };
 
-// STRAYS: ids outside [0, E - 1) count as expert E - 1 instead of being dropped.
-template <bool STRAYS = false>
+// RUNS: the rows of a batch by their adapters.  Ids outside [0, E - 1) count as
+// expert E - 1 instead of being dropped, and rows come in long runs of one id,
+// where a wave's lanes would all meet at one LDS word (8192 rows of 12 sequences
+// 21 us): they find each other by ballots instead, one round per distinct id of
+// a 64-row group.
+template <bool RUNS = false>
 __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restrict__ ids, int n, int E, int bs,
                                            int32_t* __restrict__ sorted, int32_t* __restrict__ expert_ids,
                                            int blocks_cap, int32_t* __restrict__ num_post_pad,
@@ -205,7 +209,7 @@ __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restr
     for (int r = 0; r < kAlignBatch; ++r) {
       const int i = b0 + r * 64 + lane;
       er[r] = i < r1 ? ids[i] : -1;
-      if (STRAYS && i < r1 && (uint32_t)er[r] >= (uint32_t)E) er[r] = E - 1;
+      if (RUNS && i < r1 && (uint32_t)er[r] >= (uint32_t)E) er[r] = E - 1;
     }
   };
   const bool one_batch = chunk <= 64 * kAlignBatch;  // the ids stay in registers between the passes
@@ -216,8 +220,18 @@ __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restr
   for (int b0 = r0; b0 < r1; b0 += 64 * kAlignBatch) {  // wave-uniform
     if (!one_batch) load_batch(b0);
 #pragma unroll
-    for (int r = 0; r < kAlignBatch; ++r)
-      if (er[r] >= 0 && er[r] < E) atomicAdd(&wpos[wave][er[r]], 1);
+    for (int r = 0; r < kAlignBatch; ++r) {
+      if constexpr (RUNS) {
+        for (uint64_t left = __ballot(er[r] >= 0); left != 0;) {
+          const int e = read_lane(er[r], __builtin_ctzll(left));
+          const uint64_t m = __ballot(er[r] == e);
+          if (lane == 0) wpos[wave][e] += __popcll(m);
+          left &= ~m;
+        }
+      } else {
+        if (er[r] >= 0 && er[r] < E) atomicAdd(&wpos[wave][er[r]], 1);
+      }
+    }
   }
   __syncthreads();
 
@@ -277,6 +291,17 @@ __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restr
     if (!one_batch) load_batch(b0);
 #pragma unroll
     for (int r = 0; r < kAlignBatch; ++r) {
+      if constexpr (RUNS) {
+        for (uint64_t left = __ballot(er[r] >= 0); left != 0;) {
+          const int e = read_lane(er[r], __builtin_ctzll(left));
+          const uint64_t m = __ballot(er[r] == e);
+          const int first = wpos[wave][e];
+          if (er[r] == e) sorted[first + __popcll(m & lanes_below(lane))] = b0 + r * 64 + lane;
+          if (lane == 0) wpos[wave][e] = first + __popcll(m);
+          left &= ~m;
+        }
+        continue;
+      }
       const int e = er[r];
       const bool valid = e >= 0 && e < E;
       if (valid) atomicOr((unsigned long long*)&wmask[wave][e], 1ull << lane);
