@@ -51,17 +51,22 @@ __device__ __forceinline__ void dense_store4(const DenseArgs& a, int sid, float 
   *(typename DT::vec4*)((E*)a.out + (int64_t)sid * a.cols + n) = r;
 }
 
-// Few rows per expert: a workgroup is one tile of up to 16 MT rows and 16 NT
-// columns (of each half, with an activation), its four waves split K and load
-// weights and rows straight into MFMA operands: each wave reads other k, so
-// LDS would share nothing.  Bound by reading each busy expert's weights once.
+// Few rows per expert: a workgroup is one 16-row tile and 16 NT columns (of each
+// half, with an activation), its four waves split K and load weights and rows
+// straight into MFMA operands: each wave reads other k, so LDS would share
+// nothing.  Bound by reading each busy expert's weights once.  What keeps the
+// loads in flight is many short waves, not deep ones: one step ahead against two
+// and three 223 / 229 / 238 us for both products of E = 128, H = 2048, I = 768
+// top-8 at 32 tokens (4.7 TB/s of weights), 31.5 / 32.3 / 32.5 at one; two
+// waves 227 and 32.0, eight 268 and 33.0.
 constexpr int kDenseWaves = 4;
 
-template <int EPL, int MT, int NT, int D, int ACT, typename DT>
+template <int EPL, int NT, int ACT, typename DT>
 __global__ __launch_bounds__(64 * kDenseWaves) void dense_rows_kernel(DenseArgs a) {
   using V8 = typename DT::vec8;
   constexpr int H = ACT == kActNone ? 1 : 2;
-  __shared__ f32x4 red[kDenseWaves * H * NT * MT * 64];
+  constexpr int D = 2;
+  __shared__ f32x4 red[kDenseWaves * H * NT * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
   const int slot = blockIdx.x / a.groups, base = (blockIdx.x - slot * a.groups) * 16 * NT;
@@ -70,23 +75,16 @@ __global__ __launch_bounds__(64 * kDenseWaves) void dense_rows_kernel(DenseArgs 
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, a.x_bytes);
 
   RowTiles<EPL> tiles;
-  tiles.scan(a.offsets, a.E, a.sorted_cap, 16 * MT, lane);
+  tiles.load(a.offsets, a.E, a.sorted_cap, lane);
+  tiles.scan(16, lane);
   for (int t = slot;; t += a.slots) {
     int e, rb, rows;
-    tiles.find(t, 16 * MT, lane, e, rb, rows);
+    tiles.find(t, 16, lane, e, rb, rows);
     if (e < 0) break;  // the same in every wave
-    int sid[MT];
-    uint32_t xo[MT];
-    bool some = false;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      sid[m] = 16 * m + c < rows ? a.sorted[rb + 16 * m + c] : -1;
-      if (sid[m] >= a.num_routed) sid[m] = -1;
-      xo[m] = sid[m] >= 0 ? ((uint32_t)(sid[m] / a.a_div) * (uint32_t)a.K + 16u * g) * 2u : kPastEnd;
-      some |= sid[m] >= 0;
-    }
-    if (__ballot(some) == 0) continue;  // padding alone: the same in every wave
-
+    int sid = c < rows ? a.sorted[rb + c] : -1;
+    if (sid >= a.num_routed) sid = -1;
+    if (__ballot(sid >= 0) == 0) continue;  // padding alone: the same in every wave
+    const uint32_t xo = sid >= 0 ? ((uint32_t)(sid / a.a_div) * (uint32_t)a.K + 16u * g) * 2u : kPastEnd;
     const __amdgpu_buffer_rsrc_t wr = make_rsrc((const char*)a.w + (int64_t)e * a.w_bytes, a.w_bytes);
     uint32_t wo[H][NT];
 #pragma unroll
@@ -97,7 +95,7 @@ __global__ __launch_bounds__(64 * kDenseWaves) void dense_rows_kernel(DenseArgs 
         wo[h][j] = n < a.cols ? ((uint32_t)(h * a.cols + n) * (uint32_t)a.K + 16u * g) * 2u : kPastEnd;
       }
     struct Stage {
-      u32x4 w[H][NT][2], x[MT][2];
+      u32x4 w[H][NT][2], x[2];
     };
     auto load = [&](Stage& st, int s) {
 #pragma unroll
@@ -110,25 +108,20 @@ __global__ __launch_bounds__(64 * kDenseWaves) void dense_rows_kernel(DenseArgs 
           for (int j = 0; j < NT; ++j)
             st.w[h][j][q] = __builtin_amdgcn_raw_buffer_load_b128(wr, (wo[h][j] + 16u * q) | dead, s * kDenseStepK * 2,
                                                                   kCacheStream);
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          st.x[m][q] = __builtin_amdgcn_raw_buffer_load_b128(xr, (xo[m] + 16u * q) | dead, s * kDenseStepK * 2, 0);
+        st.x[q] = __builtin_amdgcn_raw_buffer_load_b128(xr, (xo + 16u * q) | dead, s * kDenseStepK * 2, 0);
       }
     };
-    f32x4 acc[H][NT][MT];
+    f32x4 acc[H][NT];
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[h][j][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NT; ++j) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     Stage st[D];
-#pragma unroll
-    for (int p = 0; p + 1 < D; ++p) load(st[p], s0 + p);
+    load(st[0], s0);
     for (int s = s0; s < s1;) {
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        load(st[(d + D - 1) % D], s + D - 1);
+        load(st[1 - d], s + 1);
         __builtin_amdgcn_sched_barrier(0);  // the prefetch stays ahead of this step's math
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -136,61 +129,87 @@ __global__ __launch_bounds__(64 * kDenseWaves) void dense_rows_kernel(DenseArgs 
           for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int m = 0; m < MT; ++m)
-                acc[h][j][m] = mfma16x16x32(__builtin_bit_cast(V8, st[d].w[h][j][q]),
-                                            __builtin_bit_cast(V8, st[d].x[m][q]), acc[h][j][m]);
+              acc[h][j] = mfma16x16x32(__builtin_bit_cast(V8, st[d].w[h][j][q]), __builtin_bit_cast(V8, st[d].x[q]),
+                                       acc[h][j]);
         if (++s >= s1) break;
       }
     }
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) red[((wave * H + h) * NT * MT + j * MT + m) * 64 + lane] = acc[h][j][m];
+      for (int j = 0; j < NT; ++j) red[((wave * H + h) * NT + j) * 64 + lane] = acc[h][j];
     __syncthreads();
-    auto sum = [&](int h, int u) {
-      f32x4 v = red[(h * NT * MT + u) * 64 + lane];
+    auto sum = [&](int h, int j) {
+      f32x4 v = red[(h * NT + j) * 64 + lane];
 #pragma unroll
-      for (int w = 1; w < kDenseWaves; ++w) v += red[((w * H + h) * NT * MT + u) * 64 + lane];
+      for (int w = 1; w < kDenseWaves; ++w) v += red[((w * H + h) * NT + j) * 64 + lane];
       return v;
     };
-    // Wave w stores the (column tile, m-tile) pairs w, w + 4, ...: lane (row c, columns 4 g .. 4 g + 3).
-    for (int u = wave; u < NT * MT; u += kDenseWaves) {
-      const int j = u / MT, m = u - j * MT;
-      const int n = base + 16 * j + 4 * g;
-      int id = -1;
-#pragma unroll
-      for (int i = 0; i < MT; ++i) id = i == m ? sid[i] : id;
-      const f32x4 v0 = sum(0, u), v1 = sum(H - 1, u);
-      if (id >= 0 && n < a.cols)
-        dense_store4<ACT, DT>(a, id, a.topk_w != nullptr ? a.topk_w[id] : 1.f, n, v0, v1);
+    // Wave j sums and stores column tile j: lane (row c, columns 4 g .. 4 g + 3).
+    const int n = base + 16 * wave + 4 * g;
+    if (wave < NT) {
+      const f32x4 v0 = sum(0, wave), v1 = sum(H - 1, wave);
+      if (sid >= 0 && n < a.cols)
+        dense_store4<ACT, DT>(a, sid, a.topk_w != nullptr ? a.topk_w[sid] : 1.f, n, v0, v1);
     }
     __syncthreads();  // before the next tile's partial sums
   }
 }
 
-// Many rows per expert: a workgroup of eight waves is one tile of up to 256
+template <int EPL, int NT, int ACT>
+hipError_t launch_rows(const DenseArgs& a, int64_t slots, int dtype, hipStream_t s) {
+  const dim3 grid((unsigned)(slots * a.groups));
+  if (dtype == 0)
+    hipLaunchKernelGGL((dense_rows_kernel<EPL, NT, ACT, F16>), grid, dim3(64 * kDenseWaves), 0, s, a);
+  else
+    hipLaunchKernelGGL((dense_rows_kernel<EPL, NT, ACT, BF16>), grid, dim3(64 * kDenseWaves), 0, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_rows_act(const DenseArgs& args, const MoeDenseParams& p, hipStream_t s) {
+  DenseArgs a = args;
+  const int cols = p.act ? 16 : 32;  // a gate and an up tile, or two tiles
+  a.groups = (a.cols + cols - 1) / cols;
+  // Every tile with rows at once, as far as a launch of 2^24 workgroups goes.
+  const int64_t slots = std::min<int64_t>({p.num_routed, p.num_routed / 16 + p.E, ((1 << 24) - 1) / a.groups});
+  a.slots = (int)slots;
+#define SGL_ROWS(ACT_, NT_) \
+  (p.E <= 128 ? launch_rows<2, NT_, ACT_>(a, slots, p.dtype, s) : launch_rows<8, NT_, ACT_>(a, slots, p.dtype, s))
+  if (p.act == kActSilu) return SGL_ROWS(kActSilu, 1);
+  if (p.act == kActGelu) return SGL_ROWS(kActGelu, 1);
+  return SGL_ROWS(kActNone, 2);
+#undef SGL_ROWS
+}
+
+// Many rows per expert: a workgroup of eight waves is one tile of up to 320
 // rows of an expert and 256 rows of its W (with an activation 128 gate and their
 // 128 up rows), both staged through two LDS buffers of 64 k by LDS-DMA.  Wave
-// (wm, wn) of 2 x 4 holds half the tile's rows and 64 columns.
+// (wm, wn) of 2 x 4 holds half the tile's rows and 64 columns.  One workgroup a
+// CU takes unit after unit.
 constexpr int kTileWaves = 8;
-constexpr int kTileM = 256;
+constexpr int kTileM = 320;
 constexpr int kTileN = 256;
-constexpr int kTileVecs = 2048;  // 16-byte vectors of one operand's stage: 256 rows of 128 bytes
-constexpr int kTileLds = 4 * kTileVecs * 16 + kTileM * 4;
+constexpr int kTileGrain = 32;               // a tile's rows come in multiples of two m-tiles
+constexpr int kTileX = kTileM * 8;           // 16-byte vectors of the rows' stage: 128 bytes a row
+constexpr int kTileStage = (kTileM + kTileN) * 8;
+constexpr int kTileLds = 2 * kTileStage * 16 + kTileM * 4;  // and the row ids
+constexpr int kTileXLoads = kTileM / (8 * kTileWaves);      // a wave's DMAs of a stage's rows, at most
+constexpr int kTileMore = 64;  // what a tile takes beside its rows, in rows
 
-// One tile: MT m-tiles of 16 rows a wave.
+// One unit: MT m-tiles of 16 rows a wave.
 //
 // Row r of a stage lies at 128 r, its 16-byte vector q (k = 8 q .. 8 q + 7) in
 // place q ^ (r & 7): the DMA's lanes then read whole lines of a row, and the
 // MFMA operand reads of 8 rows at one q meet all banks.
+//
+// (Starting the following unit's first stage ahead of the epilogue takes the
+// registers that the products need: with what it keeps spilled, 478 against
+// 422 us for both products of E = 128, H = 2048, I = 768 top-8 at 4096 tokens.)
 template <int MT, int ACT, typename DT>
 __device__ __forceinline__ void dense_tile(const DenseArgs& a, u32x4* lds, const int32_t* sids,
                                            const __amdgpu_buffer_rsrc_t& wr, const uint32_t (&wo)[4],
-                                           const __amdgpu_buffer_rsrc_t& xr, const uint32_t (&xo)[4], int base,
-                                           int wave, int lane) {
+                                           const __amdgpu_buffer_rsrc_t& xr, const uint32_t (&xo)[kTileXLoads],
+                                           int base, int wave, int lane) {
   using E = typename DT::elem;
   using V8 = typename DT::vec8;
   constexpr int H = ACT == kActNone ? 1 : 2;
@@ -201,11 +220,11 @@ __device__ __forceinline__ void dense_tile(const DenseArgs& a, u32x4* lds, const
   const int kq = ((lane & 7) ^ (lane >> 3)) * 8;  // the lane's k in a step's DMA
 
   auto issue = [&](int s) {
-    u32x4* buf = lds + (s & 1) * 2 * kTileVecs;
+    u32x4* buf = lds + (s & 1) * kTileStage;
     const uint32_t dead = s * kDenseStepK + kq < a.K ? 0u : kPastEnd;  // K is a multiple of 8
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      load_lds16(wr, buf + kTileVecs + (q * kTileWaves + wave) * 64, wo[q] | dead, s * kDenseStepK * 2);
+      load_lds16(wr, buf + kTileX + (q * kTileWaves + wave) * 64, wo[q] | dead, s * kDenseStepK * 2);
 #pragma unroll
     for (int q = 0; q < (MT + 1) / 2; ++q)
       if (q * kTileWaves + wave < 4 * MT)
@@ -227,21 +246,28 @@ __device__ __forceinline__ void dense_tile(const DenseArgs& a, u32x4* lds, const
     __builtin_amdgcn_sched_barrier(0);
     if (s + 1 < steps) issue(s + 1);
     __builtin_amdgcn_sched_barrier(0);
-    const u32x4* xs = lds + (s & 1) * 2 * kTileVecs + wm * MT * 128 + c * 8;
-    const u32x4* ws = lds + (s & 1) * 2 * kTileVecs + kTileVecs + wn * 512 + c * 8;
+    const u32x4* xs = lds + (s & 1) * kTileStage + wm * MT * 128 + c * 8;
+    const u32x4* ws = lds + (s & 1) * kTileStage + kTileX + wn * 512 + c * 8;
+    const int at0 = g ^ (c & 7), at1 = (4 + g) ^ (c & 7);
+    V8 w[2][4], x[MT];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int at = (k * 4 + g) ^ (c & 7);
-      V8 b[4];
+    for (int j = 0; j < 4; ++j) w[0][j] = __builtin_bit_cast(V8, ws[j * 128 + at0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = __builtin_bit_cast(V8, ws[j * 128 + at]);
+    for (int m = 0; m < MT; ++m) x[m] = __builtin_bit_cast(V8, xs[m * 128 + at0]);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const V8 x = __builtin_bit_cast(V8, xs[m * 128 + at]);
+    for (int j = 0; j < 4; ++j) w[1][j] = __builtin_bit_cast(V8, ws[j * 128 + at1]);
+    // The second half of a row operand follows its first into the same
+    // registers, MT m-tiles of products ahead of its use.
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[m][j] = mfma16x16x32(b[j], x, acc[m][j]);
-      }
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[m][j] = mfma16x16x32(w[0][j], x[m], acc[m][j]);
+      x[m] = __builtin_bit_cast(V8, xs[m * 128 + at1]);
     }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[m][j] = mfma16x16x32(w[1][j], x[m], acc[m][j]);
   }
 
   // Lane (row c of each m-tile) holds 4 NTH consecutive columns of each half.
@@ -255,12 +281,12 @@ __device__ __forceinline__ void dense_tile(const DenseArgs& a, u32x4* lds, const
     for (int v = 0; v < NTH / 2; ++v) {
       V8 r;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const int j = 2 * v + (w >> 2);
+      for (int i = 0; i < 8; ++i) {
+        const int j = 2 * v + (i >> 2);
         if constexpr (ACT == kActNone)
-          r[w] = (E)(acc[m][j][w & 3] * rw);
+          r[i] = (E)(acc[m][j][i & 3] * rw);
         else
-          r[w] = (E)(gated_act(ACT, acc[m][j][w & 3] * rw) * (acc[m][j + NTH][w & 3] * rw));
+          r[i] = (E)(gated_act_fast(ACT, acc[m][j][i & 3] * rw) * (acc[m][j + NTH][i & 3] * rw));
       }
       if (n0 + 8 * v < a.cols) *(V8*)((E*)a.out + (int64_t)sid * a.cols + n0 + 8 * v) = r;
     }
@@ -272,48 +298,80 @@ __global__ __launch_bounds__(64 * kTileWaves) void dense_tile_kernel(DenseArgs a
   constexpr int H = ACT == kActNone ? 1 : 2;
   constexpr int NTH = 4 / H;
   extern __shared__ u32x4 lds[];
-  int32_t* sids = (int32_t*)(lds + 4 * kTileVecs);
+  int32_t* sids = (int32_t*)(lds + 2 * kTileStage);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+
+  // The tile height: with units of nearly equal length the last round of them
+  // leaves CUs idle, so the height is the one with the shortest rounds for
+  // these buckets (every workgroup finds the same).
+  RowTiles<EPL> tiles;
+  tiles.load(a.offsets, a.E, a.sorted_cap, lane);
+  int height = kTileM;
+  float best = INFINITY;
+  for (int h = kTileM; h >= 128; h -= kTileGrain) {
+    int n, work;
+    tiles.weigh(h, kTileGrain, kTileMore, n, work);
+    const int units = n * a.groups, cus = gridDim.x;
+    const float cost = (float)((units + cus - 1) / cus) * (float)work / (float)max(n, 1);
+    if (cost < best) {
+      best = cost;
+      height = h;
+    }
+  }
+  tiles.scan(height, lane);
 
   // Workgroup b runs on XCD b % 8: each XCD takes a run of consecutive units,
   // so that the tiles that read one expert's weights share an L2.
-  RowTiles<EPL> tiles;
-  tiles.scan(a.offsets, a.E, a.sorted_cap, kTileM, lane);
-  const int per_xcd = (tiles.total() * a.groups + 7) >> 3, u = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd) return;
-  int e, rb, rows, group;
-  tiles.find_unit(u, a.groups, kTileM, 32, lane, e, rb, rows, group);
-  if (e < 0) return;  // the same in every wave
-  const int base = group * 64 * NTH;
-
+  const int per_xcd = (tiles.total() * a.groups + 7) >> 3;
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, a.x_bytes);
-  const __amdgpu_buffer_rsrc_t wr = make_rsrc((const char*)a.w + (int64_t)e * a.w_bytes, a.w_bytes);
   const uint32_t kq = ((lane & 7) ^ (lane >> 3)) * 8;
-  uint32_t xo[4], wo[4];
-  bool some = false;
+  for (int at = blockIdx.x >> 3; at < per_xcd; at += gridDim.x >> 3) {
+    int e, rb, rows, group;
+    tiles.find_unit((blockIdx.x & 7) * per_xcd + at, a.groups, height, kTileGrain, lane, e, rb, rows, group);
+    if (e < 0) break;  // the same in every wave
+    const int base = group * 64 * NTH;
+    const __amdgpu_buffer_rsrc_t wr = make_rsrc((const char*)a.w + (int64_t)e * a.w_bytes, a.w_bytes);
+    uint32_t xo[kTileXLoads], wo[4];
+    int sid[kTileXLoads];
+    bool some = false;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int r = (q * kTileWaves + wave) * 8 + (lane >> 3);
-    int sid = r < rows ? a.sorted[rb + r] : -1;
-    if (sid >= a.num_routed) sid = -1;
-    some |= sid >= 0;
-    if ((lane & 7) == 0) sids[r] = sid;
-    xo[q] = sid >= 0 ? ((uint32_t)(sid / a.a_div) * (uint32_t)a.K + kq) * 2u : kPastEnd;
-    // Row 64 wn + 16 j + i of the stage: column 4 NTH (i / 4) + 4 (j % NTH) + i % 4 of half j / NTH of
-    // wave wn's columns, so that a lane's MFMA outputs are consecutive columns.
-    const int i = r & 15, j = (r >> 4) & 3;
-    const int n = base + (r >> 6) * 16 * NTH + 4 * NTH * (i >> 2) + 4 * (j % NTH) + (i & 3);
-    wo[q] = n < a.cols ? ((uint32_t)(j / NTH * a.cols + n) * (uint32_t)a.K + kq) * 2u : kPastEnd;
+    for (int q = 0; q < kTileXLoads; ++q) {
+      const int r = (q * kTileWaves + wave) * 8 + (lane >> 3);
+      sid[q] = r < rows ? a.sorted[rb + r] : -1;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      // Row 64 wn + 16 j + i of the stage: column 4 NTH (i / 4) + 4 (j % NTH) + i % 4 of half j / NTH of
+      // wave wn's columns, so that a lane's MFMA outputs are consecutive columns.
+      const int r = (q * kTileWaves + wave) * 8 + (lane >> 3), i = r & 15, j = (r >> 4) & 3;
+      const int n = base + (r >> 6) * 16 * NTH + 4 * NTH * (i >> 2) + 4 * (j % NTH) + (i & 3);
+      wo[q] = n < a.cols ? ((uint32_t)(j / NTH * a.cols + n) * (uint32_t)a.K + kq) * 2u : kPastEnd;
+    }
+    __syncthreads();  // the unit before is done with LDS
+#pragma unroll
+    for (int q = 0; q < kTileXLoads; ++q) {
+      if (sid[q] >= a.num_routed) sid[q] = -1;
+      some |= sid[q] >= 0;
+      if ((lane & 7) == 0) sids[(q * kTileWaves + wave) * 8 + (lane >> 3)] = sid[q];
+      xo[q] = sid[q] >= 0 ? ((uint32_t)(sid[q] / a.a_div) * (uint32_t)a.K + kq) * 2u : kPastEnd;
+    }
+    if (!__syncthreads_or(some)) continue;  // padding alone
+#define SGL_MT(MT_) \
+  case MT_: dense_tile<MT_, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane); break
+    switch ((rows + kTileGrain - 1) / kTileGrain) {
+      SGL_MT(1);
+      SGL_MT(2);
+      SGL_MT(3);
+      SGL_MT(4);
+      SGL_MT(5);
+      SGL_MT(6);
+      SGL_MT(7);
+      SGL_MT(8);
+      SGL_MT(9);
+      default: dense_tile<10, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane);
+    }
+#undef SGL_MT
   }
-  if (!__syncthreads_or(some)) return;  // padding alone
-  if (rows <= 64)
-    dense_tile<2, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane);
-  else if (rows <= 128)
-    dense_tile<4, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane);
-  else if (rows <= 192)
-    dense_tile<6, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane);
-  else
-    dense_tile<8, ACT, DT>(a, lds, sids, wr, wo, xr, xo, base, wave, lane);
 }
 
 template <int EPL, int ACT, typename DT>
@@ -327,16 +385,16 @@ int tile_groups(const MoeDenseParams& p) {
   return (int)((cols + bn - 1) / bn);
 }
 
-// Workgroups that every (tile, column group) pair fits in: of the buckets' rows,
-// padding included, each expert has one tile more than its full ones at most.
+// (Tile, column group) pairs, counted in 32 bits: of the buckets' rows, padding
+// included, each expert has one tile more than its full ones at most.
 int64_t tile_units(const MoeDenseParams& p) {
-  return (p.sorted_cap / kTileM + std::min(p.num_routed, p.E)) * tile_groups(p);
+  return (p.sorted_cap / 128 + std::min(p.num_routed, p.E)) * tile_groups(p);
 }
 
 hipError_t launch_tile_act(const DenseArgs& args, const MoeDenseParams& p, hipStream_t s) {
   DenseArgs a = args;
   a.groups = tile_groups(p);
-  const dim3 grid((unsigned)((tile_units(p) + 7) / 8 * 8));
+  const dim3 grid((unsigned)std::max(8, device_cu_count() / 8 * 8));
 #define SGL_TILE(ACT_, DT_) (p.E <= 128 ? launch_tile<2, ACT_, DT_>(a, grid, s) : launch_tile<8, ACT_, DT_>(a, grid, s))
 #define SGL_TILE_A(ACT_) (p.dtype == 0 ? SGL_TILE(ACT_, F16) : SGL_TILE(ACT_, BF16))
   if (p.act == kActSilu) return SGL_TILE_A(kActSilu);
@@ -344,35 +402,6 @@ hipError_t launch_tile_act(const DenseArgs& args, const MoeDenseParams& p, hipSt
   return SGL_TILE_A(kActNone);
 #undef SGL_TILE_A
 #undef SGL_TILE
-}
-
-template <int EPL, int MT, int NT, int D, int ACT>
-hipError_t launch_rows(const DenseArgs& a, int64_t slots, int dtype, hipStream_t s) {
-  const dim3 grid((unsigned)(slots * a.groups));
-  if (dtype == 0)
-    hipLaunchKernelGGL((dense_rows_kernel<EPL, MT, NT, D, ACT, F16>), grid, dim3(64 * kDenseWaves), 0, s, a);
-  else
-    hipLaunchKernelGGL((dense_rows_kernel<EPL, MT, NT, D, ACT, BF16>), grid, dim3(64 * kDenseWaves), 0, s, a);
-  return hipGetLastError();
-}
-
-template <int MT, int NT, int D>
-hipError_t launch_rows_act(const DenseArgs& args, const MoeDenseParams& p, hipStream_t s) {
-  // With an activation a workgroup's tiles are half gate and half up.
-  constexpr int NA = NT / 2;
-  DenseArgs a = args;
-  const int nt = p.act ? NA : NT;
-  a.groups = (a.cols + 16 * nt - 1) / (16 * nt);
-  // Every tile with rows at once, as far as a launch of 2^24 workgroups goes.
-  const int64_t slots = std::min<int64_t>({p.num_routed, p.num_routed / (16 * MT) + p.E, ((1 << 24) - 1) / a.groups});
-  a.slots = (int)slots;
-#define SGL_ROWS(ACT_, NT_)                                                              \
-  (p.E <= 128 ? launch_rows<2, MT, NT_, D, ACT_>(a, slots, p.dtype, s)                   \
-              : launch_rows<8, MT, NT_, D, ACT_>(a, slots, p.dtype, s))
-  if (p.act == kActSilu) return SGL_ROWS(kActSilu, NA);
-  if (p.act == kActGelu) return SGL_ROWS(kActGelu, NA);
-  return SGL_ROWS(kActNone, NT);
-#undef SGL_ROWS
 }
 
 }  // namespace
@@ -394,9 +423,12 @@ hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s) {
   a.N = (int)p.N;
   a.K = (int)p.K;
   a.cols = (int)(p.act ? p.N / 2 : p.N);
-  if (p.num_routed <= 4 * p.E) return launch_rows_act<1, 2, 4>(a, p, s);
-  if (p.num_routed >= 64 * p.E && tile_units(p) < (1 << 24)) return launch_tile_act(a, p, s);
-  return launch_rows_act<4, 4, 2>(a, p, s);
+  // From a few rows per expert the tiles read weights no slower and follow
+  // uneven buckets better: E = 128, H = 2048, I = 768 top-8 at 4 rows an expert
+  // 269 us both ways, at 8 260 against 306 (with 64-row tiles); E = 64, I = 1408
+  // top-6 at 3 rows 220 row by row against 225, at 6 247 against 259.
+  if (p.num_routed <= 4 * p.E || tile_units(p) >= (1 << 30)) return launch_rows_act(a, p, s);
+  return launch_tile_act(a, p, s);
 }
 
 }  // namespace sgl_awq
