@@ -20,7 +20,9 @@
 // Three sizes of batch:
 //   few rows   every row is a block of its own, its adapter read from the ids:
 //              nothing is sorted, and a kernel waits for two loads in a row
-//              (id, then weights) and no more
+//              (id, then weights) and no more.  (Both steps in one launch,
+//              every workgroup computing v for itself, took as long: a CU by
+//              itself draws the 80 to 160 KB of A in 4 us and more.)
 //   batches    16-row blocks of the sorted table
 //   prefill    64-row tiles, what their waves share staged in LDS
 #include <math.h>
@@ -36,7 +38,9 @@ namespace sgl_awq {
 namespace {
 
 constexpr int kLoraWaves = 4;
-constexpr int kLoraSlices = 4;  // k-slices of the shrink, at most
+// k-slices of the shrink at most, for few rows and batches, and for prefill.
+constexpr int kLoraSlices = 8;
+constexpr int kTileSlices = 4;
 constexpr int kStepK = 64;  // k per step of the shrink: 128 bytes of a row
 
 // Loads above stay above: the wait counts of the rings below rely on how many
@@ -126,7 +130,7 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
 // One rank tile of one block; a wave's share of the k-steps with D - 1 of them
 // in flight, straight from global memory: no other wave reads these k.
 // grid: (blocks, k-slices, rank tiles).
-constexpr int kShrinkWaves = 8;
+constexpr int kShrinkWaves = 4;
 
 template <bool ROWS, typename DT>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkArgs a) {
@@ -308,7 +312,7 @@ struct VArgs {
 };
 
 // The lane's row of a part: 8 consecutive ranks of each 32, the k-slices added in order.
-template <int KC>
+template <int KC, int S>
 __device__ __forceinline__ void load_v(const VArgs& a, int64_t pos, int part, int limit, int g, f32x4 (&v)[KC][2]) {
   const float* p = a.v + pos * a.VR + part * a.rp + 8 * g;
 #pragma unroll
@@ -316,16 +320,16 @@ __device__ __forceinline__ void load_v(const VArgs& a, int64_t pos, int part, in
     v[k][0] = v[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (32 * k + 8 * g >= limit) continue;
     // All in flight at once: one by one a wave waited for each in turn.
-    f32x4 t[kLoraSlices][2];
+    f32x4 t[S][2];
 #pragma unroll
-    for (int s = 0; s < kLoraSlices; ++s) {
+    for (int s = 0; s < S; ++s) {
       if (s < a.slices) {
         t[s][0] = *(const f32x4*)(p + s * a.v_slice + 32 * k);
         t[s][1] = *(const f32x4*)(p + s * a.v_slice + 32 * k + 4);
       }
     }
 #pragma unroll
-    for (int s = 0; s < kLoraSlices; ++s) {
+    for (int s = 0; s < S; ++s) {
       if (s < a.slices) {
         v[k][0] += t[s][0];
         v[k][1] += t[s][1];
@@ -514,7 +518,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs
   if (ROWS) {
     cols.load_y(block_row<true>(a.b, b, cols.c), y);
 #pragma unroll
-    for (int h = 0; h < H; ++h) load_v<KC>(a.v, b, H == 1 ? cols.part : h, a.R, cols.g, v[h]);
+    for (int h = 0; h < H; ++h) load_v<KC, kLoraSlices>(a.v, b, H == 1 ? cols.part : h, a.R, cols.g, v[h]);
   }
   const int e = block_adapter<ROWS>(a.b, b);
   if (e < 0) return;  // past the last block
@@ -538,7 +542,7 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs
     if (!ROWS) {
       cols.load_b(e, rank, w);
 #pragma unroll
-      for (int h = 0; h < H; ++h) load_v<KC>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
+      for (int h = 0; h < H; ++h) load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
     }
 #pragma unroll
     for (int h = 0; h < H; ++h) {
@@ -589,7 +593,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_
   {
     f32x4 v[H][KC][2];
 #pragma unroll
-    for (int h = 0; h < H; ++h) load_v<KC>(a.v, have ? pos : 0, H == 1 ? cols.part : h, a.R, g, v[h]);
+    for (int h = 0; h < H; ++h) load_v<KC, kTileSlices>(a.v, have ? pos : 0, H == 1 ? cols.part : h, a.R, g, v[h]);
     const int e = __builtin_amdgcn_readlane(adapters, wave);  // of the wave's own block
     const bool adapter = e >= 0 && e < a.b.L;
     const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
@@ -739,9 +743,11 @@ LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int pa
   const int per = p.mode == kLoraTiles ? kLoraWaves * p.rank_tiles : 1;
   const int64_t wgs = (int64_t)((tiles + per - 1) / per) * (p.mode == kLoraTiles ? (p.blocks + 3) / 4 : p.blocks);
   const int64_t steps = (K + kStepK - 1) / kStepK;
-  // Two workgroups a CU, eight (tiles) or two steps a wave at least, and no more than kLoraSlices partial sums.
-  p.slices = (int)std::max<int64_t>(1, std::min<int64_t>({kLoraSlices, steps / (p.mode == kLoraTiles ? 8 : 2 * kShrinkWaves),
-                                                          (2 * cus + wgs - 1) / wgs}));
+  // Two workgroups a CU, and eight (tiles) or two steps a wave at least.
+  const bool tile = p.mode == kLoraTiles;
+  p.slices = (int)std::max<int64_t>(
+      1, std::min<int64_t>({tile ? kTileSlices : kLoraSlices, steps / (tile ? 8 : 2 * kShrinkWaves),
+                            (2 * cus + wgs - 1) / wgs}));
   p.per = 1;
   if (p.mode == kLoraTiles) {
     // A workgroup waits for its rows, v and the first columns once (as long as
