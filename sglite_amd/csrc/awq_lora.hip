@@ -504,7 +504,7 @@ struct ExpandCols {
 // itself.  A single row's loads go out beside its id as far as they do not
 // hang on it: v's partial sums and y; the weights follow the id alone.
 template <bool ROWS, int KC, int CT, int ACT, typename DT>
-__global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs a) {
+__global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 : 3) void lora_expand_kernel(ExpandArgs a) {
   using Cols = ExpandCols<KC, CT, ACT, DT>;
   constexpr int H = Cols::H;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -539,13 +539,10 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_expand_kernel(ExpandArgs
     if (ROWS) cols.load_b(e, a.R, w);
     const int rank = min(load_uniform(a.ranks + e), a.R);
     const float scale = load_uniform(a.scaling + e);
-    if (!ROWS) {
-      cols.load_b(e, rank, w);
-#pragma unroll
-      for (int h = 0; h < H; ++h) load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
-    }
+    if (!ROWS) cols.load_b(e, rank, w);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
+      if (!ROWS) load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
       if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
       typename DT::vec8 hi[KC], lo[KC];
       f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi, lo));

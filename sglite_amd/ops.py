@@ -1140,8 +1140,13 @@ class LoraBatch(NamedTuple):
         return self.adapter_ids.numel()
 
 
-# Rows up to which every row is taken by itself and nothing is sorted.
-LORA_UNSORTED_ROWS = 32
+def _lora_unsorted(rows: int, num_adapters: int) -> bool:
+    """Whether every row is taken by itself and nothing is sorted: a row then reads its adapter alone, and two rows
+    of one adapter both read it.  32 projections of four decode layers (us, sorted against not): 8 rows over 4
+    adapters of rank 16 155 / 145, over 64 of rank 64 271 / 198; 32 rows over 4 of rank 16 160 / 193, over 32 209 /
+    198, over 64 of rank 64 386 / 331; 64 rows over 4 of rank 16 165 / 261, over 32 253 / 274."""
+    return rows <= 16 or (rows <= 32 and 2 * num_adapters >= rows)
+
 
 
 def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[int], dtype: torch.dtype,
@@ -1188,15 +1193,15 @@ def lora_route(adapter_ids: torch.Tensor, num_adapters: int) -> LoraBatch:
     """A step's rows by adapter; one call serves every projection of the step.
 
     ``adapter_ids`` [M] int32 names each row's slot; an id outside ``[0, num_adapters)``, as -1, names none.  The
-    batch refers to them: they stay as they are until its last use.  Up to ``LORA_UNSORTED_ROWS`` rows nothing is
-    launched, beyond that one kernel sorts the rows."""
+    batch refers to them: they stay as they are until its last use.  For few rows nothing is launched, beyond that
+    one kernel sorts them."""
     if adapter_ids.dim() != 1 or adapter_ids.dtype != torch.int32:
         raise ValueError(f"adapter_ids must be int32 [M], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
     if not 1 <= num_adapters <= _lib.AWQ_LORA_MAX_ADAPTERS:
         raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
     _require_cuda(adapter_ids)
     ids = _aligned(adapter_ids, 4)
-    if ids.numel() <= LORA_UNSORTED_ROWS:
+    if _lora_unsorted(ids.numel(), num_adapters):
         return LoraBatch(ids, None, None, num_adapters)
     if _undispatched(ids):
         tables = _lora_route_launch(ids, num_adapters)
