@@ -36,6 +36,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .. import ops
 from ..linear import div_even
 from .fused import AWQMoeWeights, MoeWeights, process_awq_moe_weights
 
@@ -225,7 +226,7 @@ class MoELayer(_MoEBlock):
             assert param.shape == item.shape and param.dtype == item.dtype, (
                 f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
         for name, key in keys.items():
-            setattr(self, name, state_dict.pop(key).contiguous())
+            setattr(self, name, ops._aligned(state_dict.pop(key)))
         if not _internal and state_dict:
             raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
 

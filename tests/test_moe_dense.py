@@ -42,6 +42,15 @@ def test_layer_loads_what_ingestion_yields(tp):
             layer(torch.zeros(2, H).half(), torch.zeros(2, E))
 
 
+def test_misaligned_checkpoint_tensors_are_moved():
+    layer = MoELayer(2, 1, 16, 24)
+    flat = torch.arange(2 * 48 * 16 + 2 * 16 * 24 + 1, dtype=torch.float16)[1:]
+    up, down = flat[:2 * 48 * 16].view(2, 48, 16), flat[2 * 48 * 16:].view(2, 16, 24)
+    layer.load_state_dict({"gate_up_proj": up, "down_proj": down})
+    assert layer.gate_up_proj.data_ptr() % 16 == 0 and torch.equal(layer.gate_up_proj, up)
+    assert layer.down_proj.data_ptr() % 16 == 0 and torch.equal(layer.down_proj, down)
+
+
 def test_layer_and_backend_refusals():
     for kw in (dict(intermediate_size=20), dict(hidden_size=36), dict(params_dtype=torch.float32),
                dict(top_k=0), dict(top_k=5), dict(activation="relu"), dict(intermediate_size=40, tp_size=3)):
