@@ -1286,12 +1286,18 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
         if not t.is_contiguous() or t.data_ptr() % (16 if t.dtype == x.dtype else 4):
             raise ValueError("the stack's tensors must be contiguous (a and b 16-byte aligned)")
     dev = x.device
-    for t in (y, a, b, stack.scaling, stack.ranks, batch.adapter_ids):
-        if t.device != dev:
+    for t in (y, a, b, stack.scaling, stack.ranks, batch.adapter_ids, batch.sorted_ids, batch.block_adapters):
+        if t is not None and t.device != dev:
             raise ValueError("y, x, the stack and the batch must be on one device")
     if batch.rows != M or batch.num_adapters != L:
         raise ValueError(f"the batch was routed for {batch.rows} rows and {batch.num_adapters} adapters, "
                          f"not {M} and {L}")
+    for t, n in ((batch.adapter_ids, M), (batch.sorted_ids, M + 15 * (L + 1)),
+                 (batch.block_adapters, (M + 15 * (L + 1) + 15) // 16)):
+        if t is not None and (t.dtype != torch.int32 or t.numel() < n or not t.is_contiguous()):
+            raise ValueError("the batch must be lora_route's: contiguous int32 ids and tables")
+    if (batch.sorted_ids is None) != (batch.block_adapters is None):
+        raise ValueError("the batch must have both tables or neither")
     if activation is not None:
         if activation not in _GATED_ACT:
             raise ValueError(f"unsupported activation {activation!r}")

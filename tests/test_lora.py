@@ -97,7 +97,13 @@ def test_python_refusals():
             (y, x, st._replace(ranks=st.ranks.long()), _batch(), None),
             (y, x, st._replace(b=torch.zeros(3, 16, 48, dtype=h).transpose(1, 2)), _batch(), None),
             (y, x, st._replace(a=torch.zeros(3 * 32 * 64 + 1, dtype=h)[1:].view(3, 32, 64)), _batch(), None),
-            (y, x, st, _batch(M=5), None), (y, x, st, _batch(L=4), None), (y, x, st, _batch(), "relu"),
+            (y, x, st, _batch(M=5), None), (y, x, st, _batch(L=4), None),
+            (y, x, st, _batch()._replace(adapter_ids=torch.zeros(4, dtype=torch.int64)), None),
+            (y, x, st, _batch()._replace(sorted_ids=torch.zeros(64, dtype=torch.int32)), None),
+            (y, x, st, _batch()._replace(sorted_ids=torch.zeros(63, dtype=torch.int32),
+                                         block_adapters=torch.zeros(4, dtype=torch.int32)), None),
+            (y, x, st, _batch()._replace(sorted_ids=torch.zeros(64, dtype=torch.int32),
+                                         block_adapters=torch.zeros(3, dtype=torch.int32)), None), (y, x, st, _batch(), "relu"),
             (y, x, st._replace(parts=(16, 32)), _batch(), "silu")]:
         with pytest.raises(ValueError):
             ops.lora_add(bad_y, bad_x, bad_stack, bad_batch, activation=act)
@@ -133,7 +139,8 @@ def test_c_abi_refusals():
             (inv, dict(y=None)), (inv, dict(x=None)), (inv, dict(a=None)), (inv, dict(b=None)),
             (inv, dict(scaling=None)), (inv, dict(ranks=None)), (inv, dict(out=None)),
             (inv, dict(blocks=None)), (inv, dict(ids=None, sorted=None)),
-            (uns, dict(M=257, sorted=None, blocks=None)), (inv, dict(y=4104)), (inv, dict(x=8194)), (inv, dict(a=16392)),
+            (uns, dict(M=257, sorted=None, blocks=None)),
+            (uns, dict(M=256, N=1 << 24, R=8, cols=(1 << 23, 1 << 23), sorted=None, blocks=None)), (inv, dict(y=4104)), (inv, dict(x=8194)), (inv, dict(a=16392)),
             (inv, dict(b=32776)), (inv, dict(out=65544)),
             (uns, dict(R=264)), (uns, dict(L=0)), (uns, dict(L=512)), (uns, dict(parts=5, cols=(8,) * 6)),
             (uns, dict(parts=0, cols=(48,))), (uns, dict(M=1 << 24)), (uns, dict(M=1 << 23, K=128)),
