@@ -68,7 +68,55 @@ SHAPES = [
     (777, 5, 2, 520, 400, "skewed"),
     (1030, 3, 1, 384, 1040, "one"),
     (2048, 16, 4, 512, 528, "skewed"),
+    (300, 200, 8, 64, 48, "even"),
+    (1500, 300, 2, 72, 272, "skewed"),
+    (700, 2, 1, 8, 16, "even"),
 ]
+
+
+@pytest.mark.parametrize("E,n", [(4, 700), (2, 1), (300, 1300)])
+def test_buckets_padded_to_long_blocks(E, n):
+    """Tiles of padding alone in front of other experts' rows."""
+    a, w, ids, _ = make(n, E, 1, 136, 48, torch.bfloat16, load="skewed")
+    align = ops.moe_align_block_size(ids, 1024, E)
+    close(ops.moe_dense_gemm(a, w, align, None, n, 1), *formula(a, w, ids, 1, None, None))
+
+
+def test_weights_and_rows_on_another_stream():
+    a, w, ids, weights = make(900, 4, 2, 512, 256, torch.float16)
+    want, err = formula(a, w, ids, 2, weights, "silu")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        align = ops.moe_align_block_size(ids, 16, 4)
+        got = [ops.moe_dense_gemm(a, w, align, weights, 1800, 2, "silu", True) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[0], t) for t in got)
+    close(got[0], want, err)
+
+
+def test_layers_share_a_graph_with_adapters_between():
+    """A step's projections with adapters and expert products in one graph, replayed with other ids."""
+    a, w, ids, weights = make(40, 8, 2, 256, 128, torch.float16)
+    stack = ops.make_lora_stack(3, 16, 256, (256,), torch.float16, torch.device(DEV))
+    stack.a.normal_(std=0.05), stack.b.normal_(std=0.2), stack.scaling.fill_(1.0), stack.ranks.fill_(16)
+    slots = torch.randint(-1, 3, (40,), dtype=torch.int32, device=DEV)
+
+    def step():
+        x = ops.lora_add(a, a, stack, ops.lora_route(slots, 3))
+        return ops.moe_dense_gemm(x, w, ops.moe_align_block_size(ids, 16, 8), weights, 80, 2, "gelu", True)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        ids.copy_(torch.randint(0, 8, ids.shape, dtype=torch.int32, device=DEV))
+        slots.copy_(torch.randint(-1, 3, slots.shape, dtype=torch.int32, device=DEV))
+        want = step()
+        graph.replay()
+        assert torch.equal(out, want)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
