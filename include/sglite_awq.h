@@ -461,7 +461,7 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  *          aligned, any content
  * Limits: num_adapters <= AWQ_LORA_MAX_ADAPTERS, max_rank <= AWQ_LORA_MAX_RANK,
  * parts <= AWQ_LORA_MAX_PARTS, M < 2^24; x, one adapter's a and one adapter's b
- * below 2 GiB each. */
+ * below 2 GiB each; without the tables (N / 128 + parts) * M < 2^24. */
 #define AWQ_LORA_MAX_ADAPTERS 511
 #define AWQ_LORA_MAX_RANK 256
 #define AWQ_LORA_MAX_PARTS 4

@@ -934,7 +934,7 @@ int awq_lora_add(const void* y, const void* x, const void* a, const void* b, con
     return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_add: more than %d rows need the tables of awq_lora_route",
                 AWQ_LORA_MAX_UNROUTED_ROWS);
   if (!routed && (N / 128 + parts) * M >= (int64_t(1) << 24))
-    return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_add: M * N must be below 2^31 without the tables");
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_lora_add: (N / 128 + parts) * M must be below 2^24 without the tables");
   const int64_t need = plan_lora(M, N, K, num_adapters, max_rank, parts, routed).ws_bytes;
   if (!ws || ws_bytes < need || !aligned(ws, 16))
     return fail(AWQ_STATUS_WORKSPACE, "awq_lora_add: a 16-byte aligned workspace of %lld bytes needed, %lld given",

@@ -129,6 +129,9 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
 
 // One rank tile of one block; a wave's share of the k-steps with D - 1 of them
 // in flight, straight from global memory: no other wave reads these k.
+// Bound by the chain id -> weights -> sum for single rows (Qwen3-4B qkv, rank 16,
+// 0.25 MB of A: 3.3 us under the profiler), by the loads of A for batches
+// (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 17.3 us, 2.9 TB/s).
 // grid: (blocks, k-slices, rank tiles).
 constexpr int kShrinkWaves = 4;
 
@@ -195,6 +198,9 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
 // straight into MFMA operands and the rows shared through a ring of LDS slots
 // filled by LDS-DMA, whole 128-byte lines of a row at a time.  Blocks of
 // different adapters in the four are taken in turn, the others' rows as zeros.
+// 8192 rows over 8 adapters of rank 64, Llama-3-8B qkv / o / gate_up / down: 57 /
+// 27 / 43 / 87 us, x at 1.2 to 2.7 TB/s.  Bound by the reads of A through L2,
+// three times x's bytes for qkv's 192 ranks, and the wait for them at each step.
 // grid: (groups of four blocks and k-slices, groups of 4 RT rank tiles).
 constexpr int kShrinkRows = 64;
 constexpr int shrink_slots(int rt) { return rt <= 2 ? 6 : 4; }
@@ -503,6 +509,10 @@ struct ExpandCols {
 // Few rows and batches: row block after row block, v split by every wave for
 // itself.  A single row's loads go out beside its id as far as they do not
 // hang on it: v's partial sums and y; the weights follow the id alone.
+// Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 5.0 us
+// under the profiler); for batches by it and by the waves that the operands'
+// registers leave room for (Llama-3-8B gate_up, 128 rows over 32 adapters of
+// rank 64: 128 MB in 49.8 us, 2.6 TB/s).
 template <bool ROWS, int KC, int CT, int ACT, typename DT>
 __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 : 3) void lora_expand_kernel(ExpandArgs a) {
   using Cols = ExpandCols<KC, CT, ACT, DT>;
@@ -556,7 +566,9 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
 // columns (32 gate and their 32 up ones).  A wave's v becomes MFMA operands
 // once; the columns' rows of B come through a ring of LDS slots filled by
 // LDS-DMA, shared by the waves, and y into registers, both D steps ahead.
-// Blocks of different adapters in the four are taken in turn.
+// Blocks of different adapters in the four are taken in turn.  Bound by reading
+// y and writing the output, and by each workgroup's start: 8192 rows of rank 64,
+// Llama-3-8B gate_up with silu 242 us for 705 MB, 2.9 TB/s; qkv 77 us, o 57 us.
 constexpr int kExpandSlots = 4;
 
 template <int KC, int ACT, typename DT>
