@@ -552,7 +552,9 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
     if (!ROWS) cols.load_b(e, rank, w);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      if (!ROWS) load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, rank, cols.g, v[h]);
+      // Padding rows take none: with all 16 rows v was more bytes than B.
+      if (!ROWS)
+        load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, sid >= 0 ? rank : 0, cols.g, v[h]);
       if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
       typename DT::vec8 hi[KC], lo[KC];
       f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi, lo));
