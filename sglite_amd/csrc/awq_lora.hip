@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
   // Sum over the waves; lane (row i, ranks 4 g .. 4 g + 3).
   red[wave * 64 + lane] = acc;
   __syncthreads();
-  if (wave != 0 || (ROWS && i != 0)) return;
+  if (wave != 0 || sid < 0) return;  // (the expand reads no padding)
   f32x4 s = red[lane];
 #pragma unroll
   for (int w = 1; w < kShrinkWaves; ++w) s += red[w * 64 + lane];
@@ -506,13 +506,15 @@ struct ExpandCols {
   }
 };
 
-// Few rows and batches: row block after row block, v split by every wave for
-// itself.  A single row's loads go out beside its id as far as they do not
-// hang on it: v's partial sums and y; the weights follow the id alone.
+// Few rows and batches: a wave is a row block and one or two column steps, v
+// split by every wave for itself.  A single row's loads go out beside its id as
+// far as they do not hang on it: v's partial sums and y; the weights follow the
+// id alone.  A block's go out ahead of its v, the second step's ahead of the
+// first one's stores.
 // Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 5.0 us
 // under the profiler); for batches by it and by the waves that the operands'
 // registers leave room for (Llama-3-8B gate_up, 128 rows over 32 adapters of
-// rank 64: 128 MB in 49.8 us, 2.6 TB/s).
+// rank 64: 128 MB in 34.8 us, 3.7 TB/s).
 template <bool ROWS, int KC, int CT, int ACT, typename DT>
 __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 : 3) void lora_expand_kernel(ExpandArgs a) {
   using Cols = ExpandCols<KC, CT, ACT, DT>;
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
   const int wgs = (a.groups + kLoraWaves - 1) / kLoraWaves;
   const int b = blockIdx.x / wgs, grp = (blockIdx.x - b * wgs) * kLoraWaves + wave;
   if (grp >= a.groups) return;
-  const Cols cols(a, grp, lane, 1);
+  Cols cols(a, grp, lane, ROWS ? 1 : a.per);
   u32x4 y[H][Cols::VEC];
   f32x4 v[H][KC][2];
   if (ROWS) {
@@ -535,33 +537,45 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
   const bool adapter = e < a.b.L;
   if (!adapter && H == 1 && a.inplace) return;
   const int sid = block_row<ROWS>(a.b, b, cols.c);
+  u32x4 w[H][CT][KC];
+  if (ROWS && adapter) cols.load_b(e, a.R, w);
   if (!ROWS) cols.load_y(sid, y);
-  f32x4 acc[H][CT];
+  const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
+  const float scale = adapter ? load_uniform(a.scaling + e) : 0.f;
+  if (!ROWS && adapter) cols.load_b(e, rank, w);
+  typename DT::vec8 hi[H][KC], lo[H][KC];
   float f[H];
 #pragma unroll
   for (int h = 0; h < H; ++h) {
-    f[h] = 0.f;
-#pragma unroll
-    for (int t = 0; t < CT; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // Padding rows take none: with all 16 rows v was more bytes than B.
+    if (!ROWS)
+      load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, sid >= 0 ? rank : 0, cols.g, v[h]);
+    f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi[h], lo[h]));
   }
-  if (adapter) {
-    u32x4 w[H][CT][KC];
-    if (ROWS) cols.load_b(e, a.R, w);
-    const int rank = min(load_uniform(a.ranks + e), a.R);
-    const float scale = load_uniform(a.scaling + e);
-    if (!ROWS) cols.load_b(e, rank, w);
+  for (int s = 0;;) {
+    f32x4 acc[H][CT];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      // Padding rows take none: with all 16 rows v was more bytes than B.
-      if (!ROWS)
-        load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, sid >= 0 ? rank : 0, cols.g, v[h]);
-      if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
-      typename DT::vec8 hi[KC], lo[KC];
-      f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi, lo));
-      Cols::mul(w[h], hi, lo, acc[h]);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (adapter) {
+        if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
+        Cols::mul(w[h], hi[h], lo[h], acc[h]);
+      }
     }
+    const bool more = !ROWS && ++s < a.per && cols.base + 16 * CT < cols.end;
+    if (!more) {
+      cols.store(sid, y, acc, f);
+      return;
+    }
+    cols.base += 16 * CT;
+    if (adapter) cols.load_b(e, rank, w);
+    __builtin_amdgcn_sched_barrier(0);
+    cols.base -= 16 * CT;
+    cols.store(sid, y, acc, f);
+    cols.base += 16 * CT;
+    cols.load_y(sid, y);
   }
-  cols.store(sid, y, acc, f);
 }
 
 // Prefill: a workgroup is four row blocks, one a wave, and `per` steps of 64
@@ -760,6 +774,12 @@ LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int pa
       1, std::min<int64_t>({tile ? kTileSlices : kLoraSlices, steps / (tile ? 8 : 2 * kShrinkWaves),
                             (2 * cus + wgs - 1) / wgs}));
   p.per = 1;
+  // Two column steps for each split of v once there are four waves a SIMD with
+  // one step each (a projection alone, both steps of it; one / two / three steps,
+  // us: rank 64, N = 28672 gated, 64 rows over 8 adapters 32.4 / 22.9 / 24.4, 128
+  // over 32 58.3 / 48.5 / 48.1; N = 6144 128 over 32 21.8 / 21.8 / 23.5, 64 over 8
+  // 13.2 / 14.3 / 15.7; rank 16, N = 4096, 40 rows over 4 9.2 / 10.0 / 10.6).
+  if (p.mode == kLoraBlocks && p.blocks * N / (16 * kLoraColTiles) >= 16 * cus) p.per = 2;
   if (p.mode == kLoraTiles) {
     // A workgroup waits for its rows, v and the first columns once (as long as
     // 5 to 8 steps take) however many steps it has, so they are many, as far as

@@ -134,6 +134,26 @@ def test_lora_add_gated(M, K, half, L, R, act, dtype):
             close(ops.lora_add(y, x, stack, b, activation=act), want, err)
 
 
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("L,R", [(9, 16), (9, 64), (6, 128), (5, 200)])
+def test_blocks_of_many_columns(L, R, act):
+    """Row blocks with two column steps a wave; the last one of a part, and its columns, are cut short."""
+    parts = (9000, 9000) if act else (12872, 4104, 40)
+    y, x, stack, ids = make(270, 64, parts, L, R, torch.float16, [(R, R - 3, 0, 1)[e % 4] for e in range(L)], seed=R)
+    ids[:20] = -1
+    y0 = y.clone()
+    batch = ops.lora_route(ids, L)
+    assert batch.sorted_ids is not None
+    want, err = deltas(y, x, stack, ids)
+    if act:
+        close(ops.lora_add(y, x, stack, batch, activation=act), *gated(want, err, act))
+        return
+    got = ops.lora_add(y, x, stack, batch)
+    close(got, want, err)
+    assert torch.equal(got[ids < 0], y0[ids < 0])
+    assert torch.equal(ops.lora_add(y, x, stack, batch, out=y), got)
+
+
 def test_every_id_without_an_adapter_names_none():
     y, x, stack, ids = make(50, 128, (64,), 4, 16, torch.float16)
     ids[::2] = torch.tensor([-1, 4, 5, -7, 2 ** 31 - 1, -2 ** 31, 1000, 511, 512, 4, -1, -2, 99, 4, 5, 6, 7, 8, 9, 10,
