@@ -127,8 +127,12 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
   return q < a.tiles && r < rank ? ((uint32_t)(p * a.R + r) * (uint32_t)a.K + (uint32_t)k) * 2u : kPastEnd;
 }
 
-// One rank tile of one block; a wave's share of the k-steps with D - 1 of them
-// in flight, straight from global memory: no other wave reads these k.
+// One rank tile of one block; a wave's share of the k-steps, one step ahead,
+// straight from global memory: no other wave reads these k.  The waves of other
+// workgroups fill the time; loads further ahead mostly lie past the short slices
+// (layers of Qwen3-4B at 1 row / 32 rows over 16 adapters of rank 32 / Llama-3-8B at
+// 128 over 32 of 64: one step ahead 263 / 424 / 484 us, two 266 / 435 / 491, three
+// 270 / 444 / 500, five 275 / 460 / 513).
 // Bound by the chain id -> weights -> sum for single rows (Qwen3-4B qkv, rank 16,
 // 0.25 MB of A: 3.3 us under the profiler), by the loads of A for batches
 // (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 17.3 us, 2.9 TB/s).
@@ -138,7 +142,7 @@ constexpr int kShrinkWaves = 4;
 template <bool ROWS, typename DT>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkArgs a) {
   using V8 = typename DT::vec8;
-  constexpr int D = 4;
+  constexpr int D = 2;
   __shared__ f32x4 red[kShrinkWaves * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int i = lane & 15, g = lane >> 4;
