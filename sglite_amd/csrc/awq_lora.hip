@@ -130,12 +130,12 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
 // One rank tile of one block; a wave's share of the k-steps, one step ahead,
 // straight from global memory: no other wave reads these k.  The waves of other
 // workgroups fill the time; loads further ahead mostly lie past the short slices
-// (layers of Qwen3-4B at 1 row / 32 rows over 16 adapters of rank 32 / Llama-3-8B at
-// 128 over 32 of 64: one step ahead 263 / 424 / 484 us, two 266 / 435 / 491, three
+// (layers of Qwen3-4B at 1 row / 32 rows unsorted / Llama-3-8B at 128 rows over 32
+// adapters of rank 64: one step ahead 263 / 424 / 484 us, two 266 / 435 / 491, three
 // 270 / 444 / 500, five 275 / 460 / 513).
 // Bound by the chain id -> weights -> sum for single rows (Qwen3-4B qkv, rank 16,
-// 0.25 MB of A: 3.3 us under the profiler), by the loads of A for batches
-// (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 17.3 us, 2.9 TB/s).
+// 0.25 MB of A: 3.2 us under the profiler), by the loads of A for batches
+// (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 15.5 us, 3.2 TB/s).
 // grid: (blocks, k-slices, rank tiles).
 constexpr int kShrinkWaves = 4;
 
@@ -515,10 +515,10 @@ struct ExpandCols {
 // far as they do not hang on it: v's partial sums and y; the weights follow the
 // id alone.  A block's go out ahead of its v, the second step's ahead of the
 // first one's stores.
-// Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 5.0 us
+// Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 5.2 us
 // under the profiler); for batches by it and by the waves that the operands'
 // registers leave room for (Llama-3-8B gate_up, 128 rows over 32 adapters of
-// rank 64: 128 MB in 34.8 us, 3.7 TB/s).
+// rank 64: 128 MB in 34.6 us, 3.7 TB/s).
 template <bool ROWS, int KC, int CT, int ACT, typename DT>
 __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 : 3) void lora_expand_kernel(ExpandArgs a) {
   using Cols = ExpandCols<KC, CT, ACT, DT>;

@@ -1140,13 +1140,13 @@ class LoraBatch(NamedTuple):
         return self.adapter_ids.numel()
 
 
-def _lora_unsorted(rows: int, num_adapters: int) -> bool:
+def _lora_unsorted(rows: int) -> bool:
     """Whether every row is taken by itself and nothing is sorted: a row then reads its adapter alone, and two rows
     of one adapter both read it.  32 projections of four decode layers (us, sorted against not): 8 rows over 4
-    adapters of rank 16 155 / 145, over 64 of rank 64 271 / 198; 32 rows over 4 of rank 16 160 / 193, over 32 209 /
-    198, over 64 of rank 64 386 / 331; 64 rows over 4 of rank 16 165 / 261, over 32 253 / 274."""
-    return rows <= 16 or (rows <= 32 and 2 * num_adapters >= rows)
-
+    adapters of rank 16 149 / 141, over 64 of rank 64 217 / 198; 16 rows over 4 of rank 16 149 / 152, over 32 162 /
+    154, over 64 of rank 64 258 / 264; 24 rows over 16 of rank 32 183 / 186; 32 rows 190 / 199, over 4 of rank 16
+    156 / 178."""
+    return rows <= 16
 
 
 def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[int], dtype: torch.dtype,
@@ -1201,7 +1201,7 @@ def lora_route(adapter_ids: torch.Tensor, num_adapters: int) -> LoraBatch:
         raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
     _require_cuda(adapter_ids)
     ids = _aligned(adapter_ids, 4)
-    if _lora_unsorted(ids.numel(), num_adapters):
+    if _lora_unsorted(ids.numel()):
         return LoraBatch(ids, None, None, num_adapters)
     if _undispatched(ids):
         tables = _lora_route_launch(ids, num_adapters)

@@ -110,7 +110,7 @@ def test_lora_add(M, K, parts, L, R, dtype):
     other = torch.full_like(y0, 7.0)
     assert torch.equal(ops.lora_add(y0, x, stack, batch, out=other), got)
     # Few rows by the tables of a larger step, a larger step row by row.
-    assert (batch.sorted_ids is None) == (M <= 16 or (M <= 32 and 2 * L >= M))
+    assert (batch.sorted_ids is None) == (M <= 16)
     if M <= 256:
         for b in (routed(ids, L), ops.LoraBatch(ids, None, None, L)):
             got = ops.lora_add(y0, x, stack, b)
