@@ -430,8 +430,9 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  * and the projection's `parts` column parts (q, k, v of a fused qkv; gate, up),
  *   v[p, j]  = sum_k x[m, k] * a[e][p * max_rank + j, k]
  *   y'[m, n] = y[m, n] + scaling[e] * sum_{j < r} v[part of n, j] * b[e][n, j]
- * in fp32 and rounded once; rows that name none keep y.  No counterpart in the
- * reference.
+ * in fp32 and rounded once; rows that name none keep y.  (v enters the second
+ * product whole in bf16, and with 23 of its 24 bits in fp16, down to 2^-39 of
+ * the row's largest.)  No counterpart in the reference.
  *
  * awq_lora_route sorts the rows by adapter (stable) into 16-row blocks; one
  * call serves every projection of the step, and a step of up to

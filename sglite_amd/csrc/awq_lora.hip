@@ -308,13 +308,22 @@ __global__ __launch_bounds__(64 * kLoraWaves) void lora_shrink_tile_kernel(Shrin
 // ---------------------------------------------------------------------------
 // v as MFMA operands.
 //
-// v enters the expand's MFMAs as two values of the operand type, the second
-// the first one's remainder: together 22 (fp16) or 16 (bf16) bits of the row's
-// largest, so that the rounding stays far below the output's.  A part's row is
+// v enters the expand's MFMAs as a sum of values of the operand type, each the
+// remainder of those before: three in bf16, which hold all 24 bits of the fp32
+// sum, two in fp16, which hold 23 of them (down to 2^-39 of the row's largest).
+// (Two in bf16 hold 16 bits: where B takes the difference of two sums, outputs
+// were off by whole percents; of a qkv of 32 rows 5.9e-4 of the outputs rounded
+// the other way than the exact value, with three terms 2.5e-5, in torch's fp32
+// products 5.1e-5.)  A part's row is
 // brought to a largest value in [2^14, 2^15) by a power of two first: fp16
 // holds no more than 65504, and the remainders stay normal numbers.  A row with
 // an infinity or NaN keeps those, and its finite values no longer count.
 // ---------------------------------------------------------------------------
+template <typename DT>
+constexpr int kTerms = 3;
+template <>
+constexpr int kTerms<F16> = 2;
+
 struct VArgs {
   const float* v;    // partial sums [slices][positions][VR]
   int64_t v_slice;
@@ -350,8 +359,8 @@ __device__ __forceinline__ void load_v(const VArgs& a, int64_t pos, int part, in
 
 // Its operands, and the exponent that brings the products back.
 template <int KC, typename DT>
-__device__ __forceinline__ int split_v(const f32x4 (&v)[KC][2], int rank, int g, typename DT::vec8 (&hi)[KC],
-                                       typename DT::vec8 (&lo)[KC]) {
+__device__ __forceinline__ int split_v(const f32x4 (&v)[KC][2], int rank, int g,
+                                       typename DT::vec8 (&t)[kTerms<DT>][KC]) {
   using E = typename DT::elem;
   float f[KC][8], top = 0.f;
 #pragma unroll
@@ -369,9 +378,12 @@ __device__ __forceinline__ int split_v(const f32x4 (&v)[KC][2], int rank, int g,
   for (int k = 0; k < KC; ++k)
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const float t = __builtin_ldexpf(f[k][w], -ex);
-      hi[k][w] = (E)t;
-      lo[k][w] = finite ? (E)(t - (float)hi[k][w]) : (E)0.f;
+      float rest = __builtin_ldexpf(f[k][w], -ex);
+#pragma unroll
+      for (int i = 0; i < kTerms<DT>; ++i) {
+        t[i][k][w] = (E)rest;
+        rest = finite ? rest - (float)t[i][k][w] : 0.f;
+      }
     }
   return ex;
 }
@@ -468,18 +480,17 @@ struct ExpandCols {
     }
   }
 
-  static __device__ __forceinline__ void mul(const u32x4 (&w)[CT][KC], const V8 (&hi)[KC], const V8 (&lo)[KC],
+  // The smallest terms of v first.
+  static __device__ __forceinline__ void mul(const u32x4 (&w)[CT][KC], const V8 (&v)[kTerms<DT>][KC],
                                              f32x4 (&acc)[CT]) {
 #pragma unroll
     for (int t = 0; t < CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < KC; ++k)
+    for (int i = kTerms<DT> - 1; i >= 0; --i)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) acc[t] = mfma16x16x32(__builtin_bit_cast(V8, w[t][k]), lo[k], acc[t]);
+      for (int k = 0; k < KC; ++k)
 #pragma unroll
-    for (int k = 0; k < KC; ++k)
-#pragma unroll
-      for (int t = 0; t < CT; ++t) acc[t] = mfma16x16x32(__builtin_bit_cast(V8, w[t][k]), hi[k], acc[t]);
+        for (int t = 0; t < CT; ++t) acc[t] = mfma16x16x32(__builtin_bit_cast(V8, w[t][k]), v[i][k], acc[t]);
   }
 
   // y plus f times the products, f the scaling and the power of two that
@@ -547,14 +558,14 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
   const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
   const float scale = adapter ? load_uniform(a.scaling + e) : 0.f;
   if (!ROWS && adapter) cols.load_b(e, rank, w);
-  typename DT::vec8 hi[H][KC], lo[H][KC];
+  typename DT::vec8 vt[H][kTerms<DT>][KC];
   float f[H];
 #pragma unroll
   for (int h = 0; h < H; ++h) {
     // Padding rows take none: with all 16 rows v was more bytes than B.
     if (!ROWS)
       load_v<KC, kLoraSlices>(a.v, b * 16 + cols.c, H == 1 ? cols.part : h, sid >= 0 ? rank : 0, cols.g, v[h]);
-    f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, hi[h], lo[h]));
+    f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, cols.g, vt[h]));
   }
   for (int s = 0;;) {
     f32x4 acc[H][CT];
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
       for (int t = 0; t < CT; ++t) acc[h][t] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (adapter) {
         if ((ROWS && rank < a.R) || (rank & 7)) cols.cut(rank, w[h]);
-        Cols::mul(w[h], hi[h], lo[h], acc[h]);
+        Cols::mul(w[h], vt[h], acc[h]);
       }
     }
     const bool more = !ROWS && ++s < a.per && cols.base + 16 * CT < cols.end;
@@ -591,8 +602,12 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
 // Llama-3-8B gate_up with silu 242 us for 705 MB, 2.9 TB/s; qkv 77 us, o 57 us.
 constexpr int kExpandSlots = 4;
 
+// Waves a SIMD: with three terms of 64 ranks two, since three spill 8 to 9
+// registers (8192 rows of a Llama-3-8B layer, bf16, rank 64: 635 us against 661).
+constexpr int expand_tile_waves(int kc, int terms) { return kc * terms <= 4 ? 3 : kc <= 2 ? 2 : 1; }
+
 template <int KC, int ACT, typename DT>
-__global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_tile_kernel(ExpandArgs a) {
+__global__ __launch_bounds__(64 * kLoraWaves, expand_tile_waves(KC, kTerms<DT>)) void lora_expand_tile_kernel(ExpandArgs a) {
   constexpr int CT = kLoraColTiles / (ACT == kActNone ? 1 : 2);
   using Cols = ExpandCols<KC, CT, ACT, DT>;
   using V8 = typename DT::vec8;
@@ -617,7 +632,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_
   const int pos = (b0 + wave) * 16 + c;
   const bool have = pos < a.v.positions;
   const int mine = have ? a.b.sorted[pos] : -1;
-  V8 hi[H][KC], lo[H][KC];
+  V8 vt[H][kTerms<DT>][KC];
   float f[H];
   {
     f32x4 v[H][KC][2];
@@ -628,7 +643,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_
     const int rank = adapter ? min(load_uniform(a.ranks + e), a.R) : 0;
     const float scale = adapter ? load_uniform(a.scaling + e) : 0.f;
 #pragma unroll
-    for (int h = 0; h < H; ++h) f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, g, hi[h], lo[h]));
+    for (int h = 0; h < H; ++h) f[h] = __builtin_ldexpf(scale, split_v<KC, DT>(v[h], rank, g, vt[h]));
   }
 
   for (int m0 = 0; m0 < 4;) {
@@ -691,7 +706,7 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC <= 2 ? 3 : 1) void lora_expand_
             for (int k = 0; k < KC; ++k)
               w[t][k] = bs[d * VECS + ((h * CT + t) * 16 + c) * PL + ((4 * k + g) ^ swap(c))];
           if (rank & 7) cols.cut(rank, w);
-          Cols::mul(w, hi[h], lo[h], acc[h]);
+          Cols::mul(w, vt[h], acc[h]);
         }
         cols.base = base + s * 16 * CT;
         cols.store(sid, y[d], acc, f);

@@ -1308,7 +1308,8 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch, activation: Optional[str] = None,
              out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """``y + scaling * B (A x)`` of every row's adapter, summed in fp32 and rounded once, on x's current stream.
+    """``y + scaling * B (A x)`` of every row's adapter, summed in fp32 and rounded once, on x's current stream (for
+    fp16, ``A x`` keeps 23 of the 24 bits of its fp32 sum, for bf16 all).
 
     ``y`` [M, N] is the projection's output for ``x`` [M, K]; rows that name no adapter keep it.  ``out`` may be
     ``y`` itself: then only rows with an adapter are written.  With ``activation`` ("silu" or "gelu") the two
