@@ -120,7 +120,9 @@ int awq_dequant_repacked(const void* w, const void* s, const void* z, int dtype,
  * (python/sglite/srt/model_executor/layers/quantization/marlin_utils.py:388-415).
  *
  * Split-K scratch: `ws` must hold awq_workspace_bytes(M, N, K, G) bytes (any
- * content; may be NULL when that is 0).  `counters` (int32, counter_bytes
+ * content; may be NULL when that is 0; a call may be two launches that pass
+ * their sums through it, so calls that other threads or streams make meanwhile
+ * need a ws of their own).  `counters` (int32, counter_bytes
  * long, 128-byte aligned) must hold at least awq_counter_bytes(N) bytes that
  * are zero before the first call on them; every call leaves them valid for
  * the next (the decode kernels' per-column-tile counters zero again, the
@@ -459,7 +461,9 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  *   sorted_ids, block_adapters  from awq_lora_route, adapter_ids may then be
  *          null; or both null and adapter_ids [M] read row by row
  *   ws     awq_lora_workspace_bytes bytes (`routed`: with the tables), 16-byte
- *          aligned, any content
+ *          aligned, any content.  The call is two launches that pass v through
+ *          it: calls that other threads or streams make meanwhile need a ws of
+ *          their own
  * Limits: num_adapters <= AWQ_LORA_MAX_ADAPTERS, max_rank <= AWQ_LORA_MAX_RANK,
  * parts <= AWQ_LORA_MAX_PARTS, M < 2^24; x, one adapter's a and one adapter's b
  * below 2 GiB each; without the tables (N / 128 + parts) * M < 2^24. */

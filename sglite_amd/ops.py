@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import threading
 from typing import Dict, Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
@@ -368,13 +369,21 @@ def counters_settled(counters: torch.Tensor) -> bool:
 
 
 # ---------------------------------------------------------------------------
-# Split-K workspace: one growing buffer per (device, stream) for eager calls
-# (the reference sizes its Marlin workspace once at load, awq_marlin.py:298);
-# a call being captured into a graph takes a fresh buffer from the graph's
-# pool instead, so that replays never share eager memory.
+# Workspace of split-K sums and of the adapters' A x: one growing buffer per
+# (device, stream) of a thread for eager calls (the reference sizes its Marlin
+# workspace once at load, awq_marlin.py:298).  A call may launch two kernels,
+# and another thread's launch on the same stream may come between them (the C
+# call runs without the interpreter's lock): with a buffer of its own it leaves
+# the first one's sums alone.  A call being captured into a graph takes a fresh
+# buffer from the graph's pool instead, so that replays never share eager memory.
 # ---------------------------------------------------------------------------
 
-_WS_CACHE: Dict[Tuple[int, int], torch.Tensor] = {}
+class _Workspaces(threading.local):
+    def __init__(self) -> None:
+        self.buffers: Dict[Tuple[int, int], torch.Tensor] = {}
+
+
+_WS = _Workspaces()
 
 
 def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -383,10 +392,10 @@ def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index if device.index is not None else torch.cuda.current_device(), _stream(device))
-    buf = _WS_CACHE.get(key)
+    buf = _WS.buffers.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        _WS_CACHE[key] = buf
+        _WS.buffers[key] = buf
     return buf
 
 
