@@ -25,6 +25,7 @@ import threading
 from typing import Dict, Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch._subclasses.fake_tensor import is_fake
 
 from . import _lib
 
@@ -491,13 +492,13 @@ def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, de
 
 
 def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
-    """Whether the address ranges that two tensors' elements span meet."""
-    if s.numel() == 0 or t.numel() == 0:
+    """Whether the address ranges that two tensors' elements span meet (the tensors of a trace have none)."""
+    if torch.compiler.is_compiling() or s.numel() == 0 or t.numel() == 0:
         return False
 
     def end(v: torch.Tensor) -> int:
         return v.data_ptr() + (sum((n - 1) * st for n, st in zip(v.shape, v.stride())) + 1) * v.element_size()
-    return s.data_ptr() < end(t) and t.data_ptr() < end(s)
+    return s.data_ptr() < end(t) and t.data_ptr() < end(s) and not (is_fake(s) or is_fake(t))
 
 
 def _check_counters(counters: torch.Tensor, N: int, device: torch.device) -> None:
