@@ -103,6 +103,8 @@ def fused_experts_impl(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeigh
 def _check_experts(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, activation: str) -> None:
     if activation not in ("silu", "gelu"):
         raise ValueError(f"unsupported activation {activation!r}")
+    if isinstance(w1, torch.Tensor) != isinstance(w2, torch.Tensor):
+        raise ValueError("w1 and w2 must both be dense or both repacked AWQ experts")
     (E1, K1, N1), (E2, K2, N2) = _expert_dims(w1), _expert_dims(w2)
     assert hidden_states.shape[1] == K1, "Hidden size mismatch"
     assert hidden_states.is_contiguous(), "Hidden_states must be contiguous"
@@ -147,27 +149,35 @@ class BaseMoeBackend(ABC):
         ...
 
 
+def _route_and_run(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, gating_output: torch.Tensor,
+                   topk: int, renormalize: bool, activation: str, apply_router_weight_on_input: bool) -> torch.Tensor:
+    T, E = gating_output.shape
+    E1, K1, N1 = _expert_dims(w1)
+    if T > 0 and hidden_states.shape[0] == T and E == E1:
+        _check_experts(hidden_states, w1, w2, activation)
+        config = get_default_config(T, E, N1, K1, topk)
+        topk_weights, _, align = ops.moe_route(gating_output, topk, renormalize, config["BLOCK_SIZE_M"])
+        return _run_experts(hidden_states, w1, w2, topk_weights, topk, align, activation,
+                            apply_router_weight_on_input)
+    topk_weights, topk_ids = fused_topk(hidden_states=hidden_states, gating_output=gating_output, topk=topk,
+                                        renormalize=renormalize)
+    return fused_experts_impl(hidden_states, w1, w2, topk_weights, topk_ids, activation,
+                              apply_router_weight_on_input=apply_router_weight_on_input)
+
+
 class AWQFusedMoe(BaseMoeBackend):
     """Fused MoE backend over AWQ expert stacks (FusedMoe, fused.py:205-233)."""
 
-    def forward(self, hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, gating_output: torch.Tensor,
+    def forward(self, hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, gating_output: torch.Tensor,
                 topk: int, renormalize: bool, activation: str = "silu",
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
-        T, E = gating_output.shape
-        E1, K1, N1 = _expert_dims(w1)
-        if T > 0 and hidden_states.shape[0] == T and E == E1:
-            _check_experts(hidden_states, w1, w2, activation)
-            config = get_default_config(T, E, N1, K1, topk)
-            topk_weights, _, align = ops.moe_route(gating_output, topk, renormalize, config["BLOCK_SIZE_M"])
-            return _run_experts(hidden_states, w1, w2, topk_weights, topk, align, activation,
-                                apply_router_weight_on_input)
-        topk_weights, topk_ids = fused_topk(hidden_states=hidden_states, gating_output=gating_output, topk=topk,
-                                            renormalize=renormalize)
-        return fused_experts_impl(hidden_states, w1, w2, topk_weights, topk_ids, activation,
-                                  apply_router_weight_on_input=apply_router_weight_on_input)
+        if isinstance(w1, torch.Tensor) or isinstance(w2, torch.Tensor):
+            raise ValueError("the awq_fused backend takes repacked AWQ experts; dense ones go to fused")
+        return _route_and_run(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
+                              apply_router_weight_on_input)
 
 
-class FusedMoe(AWQFusedMoe):
+class FusedMoe(BaseMoeBackend):
     """The same backend over dense experts, w1 [E, 2I, H] and w2 [E, H, I] (FusedMoe, fused.py:205-233)."""
 
     def forward(self, hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, gating_output: torch.Tensor,
@@ -175,5 +185,5 @@ class FusedMoe(AWQFusedMoe):
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
         if not (isinstance(w1, torch.Tensor) and isinstance(w2, torch.Tensor)):
             raise ValueError("the fused backend takes dense expert weights; repacked AWQ ones go to awq_fused")
-        return super().forward(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
-                               apply_router_weight_on_input)
+        return _route_and_run(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
+                              apply_router_weight_on_input)
