@@ -32,13 +32,13 @@ products read as they are.
 
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, Optional, Tuple, Type
 
 import torch
 
 from .. import ops
 from ..linear import div_even
-from .fused import AWQMoeWeights, MoeWeights, process_awq_moe_weights
+from .fused import AWQFusedMoe, AWQMoeWeights, BaseMoeBackend, FusedMoe, MoeWeights, process_awq_moe_weights
 
 _AWQ_NAMES = ("qweight", "qzeros", "scales")
 
@@ -103,6 +103,8 @@ class _MoEBlock:
 
     # Columns of the gate (and up) projection come in multiples of this.
     _COLUMNS = 16
+    # Of the backends here, the one for the other kind of experts.
+    _NOT_FOR: Type[BaseMoeBackend] = FusedMoe
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int, renormalize: bool,
                  activation: str, apply_router_weight_on_input: bool, tp_size: int, process_group, backend: str):
@@ -127,6 +129,8 @@ class _MoEBlock:
         from . import create_moe_backend
 
         self._backend = create_moe_backend(backend)
+        if isinstance(self._backend, self._NOT_FOR):
+            raise ValueError(f"the {backend!r} backend does not take the experts of {type(self).__name__}")
 
     def _expert_weights(self) -> Tuple[MoeWeights, MoeWeights]:
         raise NotImplementedError
@@ -190,6 +194,7 @@ class MoELayer(_MoEBlock):
     """Experts of one MoE block with dense weights (MoELayer, moe_layer.py:11-64)."""
 
     _COLUMNS = 8  # rows of the weights are whole 16-byte vectors
+    _NOT_FOR = AWQFusedMoe
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
                  renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,

@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from sglite_amd import ops
-from sglite_amd.moe import AWQFusedMoe, AWQMoeWeights, FusedMoe, create_moe_backend, fused_experts_impl
+from sglite_amd.moe import (SUPPORTED_MOE_BACKENDS, AWQFusedMoe, AWQMoELayer, AWQMoeWeights, BaseMoeBackend, FusedMoe,
+                            MoELayer, create_moe_backend, fused_experts_impl)
 
 E, H, I, T = 4, 64, 48, 3
 
@@ -43,3 +44,22 @@ def test_backends_refuse_the_other_kind_and_mixed_pairs():
             call(create_moe_backend(f), *pair)
     with pytest.raises(ValueError, match="device tensors"):
         call(fused_experts_impl, d1, d2)
+
+
+def test_layers_refuse_the_other_kinds_backend_at_once():
+    for layer, name, other in ((AWQMoELayer, "awq_fused", "fused"), (MoELayer, "fused", "awq_fused")):
+        with pytest.raises(ValueError, match="backend"):
+            layer(E, 2, 128, 128, backend=other)
+        with pytest.raises(ValueError, match="unknown"):
+            layer(E, 2, 128, 128, backend="none")
+        assert layer(E, 2, 128, 128)._backend.__class__ is layer(E, 2, 128, 128, backend=name)._backend.__class__
+
+
+def test_layers_take_a_backend_of_ones_own(monkeypatch):
+    class Mine(BaseMoeBackend):
+        def forward(self, hidden_states, **kw):
+            return hidden_states
+
+    monkeypatch.setitem(SUPPORTED_MOE_BACKENDS, "mine", Mine)
+    for layer in (AWQMoELayer, MoELayer):
+        assert isinstance(layer(E, 2, 128, 128, backend="mine")._backend, Mine)
