@@ -102,14 +102,19 @@ class _TPLinearBase:
     def add_adapters(self, num_adapters: int, max_rank: int, dtype: torch.dtype,
                      device: Optional[torch.device] = None) -> None:
         """Make ``num_adapters`` empty adapter slots (an empty slot adds nothing) of ranks up to ``max_rank``,
-        rounded up to a multiple of 8.  Replaces slots made before."""
+        rounded up to a multiple of 8, on ``device`` (that of the loaded weights if None; before they are loaded, the
+        current GPU).  Replaces slots made before: a step captured with those is captured anew.  Layers whose sizes
+        the adapters' kernels cannot take (input and every merged projection in multiples of 8, at most four merged)
+        are refused."""
         if not 1 <= num_adapters <= ops.LORA_MAX_ADAPTERS:
             raise ValueError(f"num_adapters must be in [1, {ops.LORA_MAX_ADAPTERS}], got {num_adapters}")
         rank = (max_rank + 7) // 8 * 8
         if not 8 <= rank <= ops.LORA_MAX_RANK:
             raise ValueError(f"max_rank must be in [1, {ops.LORA_MAX_RANK}], got {max_rank}")
-        self._lora = ops.make_lora_stack(num_adapters, rank, self.local_input_size, self._parts, dtype,
-                                         torch.device("cuda") if device is None else device)
+        if device is None:
+            loaded = [t for t in self._weights.values() if isinstance(t, torch.Tensor)] if self._weights_processed else []
+            device = loaded[0].device if loaded else torch.device("cuda")
+        self._lora = ops.make_lora_stack(num_adapters, rank, self.local_input_size, self._parts, dtype, device)
 
     def _lora_slot(self, slot: int) -> ops.LoraStack:
         if self._lora is None:

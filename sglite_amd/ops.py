@@ -1161,9 +1161,21 @@ def _lora_unsorted(rows: int) -> bool:
 
 def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[int], dtype: torch.dtype,
                     device: torch.device) -> LoraStack:
-    """An empty stack (every slot of rank 0, which adds nothing)."""
+    """An empty stack (every slot of rank 0, which adds nothing).  Sizes that ``lora_add`` cannot take are refused."""
     dtype_code(dtype)
-    N = sum(parts)
+    N, P = sum(parts), len(parts)
+    if not 1 <= num_adapters <= LORA_MAX_ADAPTERS:
+        raise ValueError(f"num_adapters must be in [1, {LORA_MAX_ADAPTERS}], got {num_adapters}")
+    if not 1 <= P <= _lib.AWQ_LORA_MAX_PARTS or any(n <= 0 or n % 8 for n in parts):
+        raise ValueError(f"the projection must have 1 to {_lib.AWQ_LORA_MAX_PARTS} parts, their columns positive "
+                         f"multiples of 8, got {tuple(parts)}")
+    if K <= 0 or K % 8:
+        raise ValueError(f"the projection's input size must be a positive multiple of 8, got {K}")
+    if not 8 <= max_rank <= LORA_MAX_RANK or max_rank % 8:
+        raise ValueError(f"max_rank must be a multiple of 8 in [8, {LORA_MAX_RANK}], got {max_rank}")
+    if max(P * K, N) * max_rank * 2 >= 1 << 31 or K >= 1 << 24:
+        raise ValueError(f"one adapter's A and B must each span below 2 GiB, got rank {max_rank}, {P} parts, K {K}, "
+                         f"N {N}")
     return LoraStack(torch.zeros((num_adapters, len(parts) * max_rank, K), dtype=dtype, device=device),
                      torch.zeros((num_adapters, N, max_rank), dtype=dtype, device=device),
                      torch.zeros(num_adapters, dtype=torch.float32, device=device),
