@@ -123,11 +123,13 @@ class _TPLinearBase:
             raise ValueError(f"slot must be in [0, {self._lora.ranks.numel()}), got {slot}")
         return self._lora
 
+    @torch.no_grad()
     def load_adapter(self, slot: int, lora_a: Union[torch.Tensor, Sequence[Optional[torch.Tensor]]],
                      lora_b: Union[torch.Tensor, Sequence[Optional[torch.Tensor]]], scaling: float = 1.0) -> None:
         """Fill a slot with an adapter: A [rank, K] and B [columns, rank] for every merged projection in order (one
         tensor each for a layer of one projection, None where the adapter leaves a projection alone), each the
-        layer's own shard.  ``scaling`` is alpha / rank.  Copies on the current stream: the caller orders it
+        layer's own shard.  ``scaling`` is alpha / rank.  The slot holds values alone: trained Parameters are copied
+        without their gradients' graph.  Copies on the current stream: the caller orders it
         against steps on other streams."""
         stack = self._lora_slot(slot)
         a_list = [lora_a] if isinstance(lora_a, torch.Tensor) else list(lora_a)

@@ -44,3 +44,14 @@ def test_slots_lie_with_the_loaded_weights():
     assert layer._lora.a.device == CPU
     layer.load_adapter(1, torch.ones(4, 64), torch.ones(32, 4))
     assert layer._lora.ranks.tolist() == [0, 4]
+
+
+def test_trained_parameters_leave_no_graph_in_the_slots():
+    layer = ReplicatedLinear(64, 32, False)
+    layer.add_adapters(2, 8, torch.float16, CPU)
+    a, b = torch.nn.Parameter(torch.ones(4, 64)), torch.nn.Parameter(torch.ones(32, 4))
+    assert torch.is_grad_enabled()
+    layer.load_adapter(0, a, b, 0.5)
+    assert not any(t.requires_grad or t.grad_fn is not None for t in layer._lora[:4])
+    assert torch.equal(layer._lora.a[0, :4].float(), torch.ones(4, 64)) and layer._lora.ranks.tolist() == [4, 0]
+    assert a.requires_grad and a.grad is None
