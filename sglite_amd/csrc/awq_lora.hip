@@ -400,7 +400,7 @@ struct ExpandArgs {
   const float* scaling;
   const int32_t* ranks;
   uint32_t w_bytes;  // one adapter's B (below 2^31)
-  int N, R, P;
+  int N, R;
   int inplace;       // out is y: rows without an adapter stay as they are
   int per;           // column steps of a group
   int groups;        // column groups
@@ -856,7 +856,6 @@ hipError_t launch_lora(const LoraParams& p, hipStream_t s) {
   x.w_bytes = (uint32_t)(p.N * p.R * 2);
   x.N = (int)p.N;
   x.R = a.R;
-  x.P = p.parts;
   x.per = plan.per;
   x.inplace = p.out == p.y;
   x.row_tiles = a.row_tiles;

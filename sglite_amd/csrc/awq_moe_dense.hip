@@ -34,7 +34,7 @@ struct DenseArgs {
   void* out;
   uint32_t x_bytes, w_bytes;  // of the activation rows, and of one expert's W (both below 2^31)
   int a_div, num_routed, sorted_cap, E;
-  int N, K;
+  int K;
   int cols;   // output columns: N, or N / 2 with an activation
   int groups; // column groups of a row tile
   int slots;  // row tiles the grid covers at a time
@@ -424,7 +424,6 @@ hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s) {
   a.num_routed = (int)p.num_routed;
   a.sorted_cap = (int)p.sorted_cap;
   a.E = (int)p.E;
-  a.N = (int)p.N;
   a.K = (int)p.K;
   a.cols = (int)(p.act ? p.N / 2 : p.N);
   // From a few rows per expert the tiles read weights no slower and follow
