@@ -174,7 +174,20 @@ hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s);
 constexpr int kLoraBlock = 16;    // rows of a block of the sorted table
 constexpr int kLoraParts = 4;     // column parts of a projection, at most
 constexpr int kLoraColTiles = 4;  // 16-column tiles of a wave of the expand
-constexpr int kLoraTileRows = 512;  // rows from which the prefill kernels run
+// Rows from which the prefill kernels run.  What they save is A and B read for 64
+// rows of an adapter at a time in place of 16, so the line hangs on the rank; what
+// they lose is the adapters of a 64-row tile taken in turn.  Llama-3-8B's qkv,
+// gate_up with silu and down, fp16, blocks / tiles in us, the rows in sequences
+// of 250 | each with an adapter of its own choice:
+//   rank 8, of 8       1024 rows  78 /  89 |  83 / 122   2048 121 / 109 | 126 / 145
+//   rank 16, of 8      1024       87 /  91 |  93 / 124   2048 131 / 110 | 136 / 149
+//   rank 16, of 100     512       74 /  97 |  91 / 209   2048 145 / 132 | 185 / 259
+//   rank 32, of 32     1024      105 / 105 | 133 / 184   1536 143 / 110 | 154 / 164
+//   rank 64, of 8       384       93 / 127 | 105 / 179    768 148 / 112 | 159 / 164
+//   rank 64, of 32      512      129 / 110 | 144 / 269   1024 176 / 131 | 213 / 247
+//   rank 128, of 8      512      185 / 226 | 195 / 333   1024 314 / 250 | 347 / 360
+// The host knows the rows, not their ids; so many rows are mostly a prefill's.
+constexpr int lora_tile_rows(int64_t max_rank) { return max_rank > 32 ? 512 : 1536; }
 enum : int { kLoraRows = 0, kLoraBlocks = 1, kLoraTiles = 2 };
 struct LoraPlan {
   int mode;           // one of the three above

@@ -778,7 +778,7 @@ LoraPlan plan_lora(int64_t M, int64_t N, int64_t K, int64_t L, int64_t R, int pa
   const int cus = device_cu_count();
   const int tiles = parts * (int)((R + 15) / 16);
   // (Ranks beyond 128 leave the prefill kernels too few registers.)
-  p.mode = !routed ? kLoraRows : M < kLoraTileRows || R > 128 ? kLoraBlocks : kLoraTiles;
+  p.mode = !routed ? kLoraRows : M < lora_tile_rows(R) || R > 128 ? kLoraBlocks : kLoraTiles;
   const int64_t cap = moe_sorted_capacity(M, L + 1, kLoraBlock);
   // A block holds a row at least.
   p.blocks = routed ? std::min(moe_block_capacity(M, L + 1, kLoraBlock), M) : M;

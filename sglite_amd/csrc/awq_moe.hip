@@ -182,8 +182,7 @@ struct AlignLds {
 // STRAYS: ids outside [0, E - 1) count as expert E - 1 instead of being dropped.
 // RUNS: rows come in long runs of one id, where a wave's lanes would all meet at
 // one LDS word: they find each other by ballots instead, one round per distinct
-// id of a 64-row group (8192 rows of 12 sequences 21 -> 11 us; 128 rows of 32
-// different ids 4.6 -> 8.6).
+// id of a 64-row group.
 template <bool STRAYS = false, bool RUNS = false>
 __device__ __forceinline__ void align_rows(AlignLds& lds, const int32_t* __restrict__ ids, int n, int E, int bs,
                                            int32_t* __restrict__ sorted, int32_t* __restrict__ expert_ids,
@@ -936,11 +935,16 @@ hipError_t launch_moe_align(const int32_t* ids, int64_t n, int64_t E, int64_t bs
 
 hipError_t launch_lora_route(const int32_t* ids, int64_t n, int64_t L, int32_t* sorted, int32_t* bucket,
                              int32_t* num_post_pad, int32_t* offsets, hipStream_t s) {
-  // A prefill's rows come sequence by sequence, a decode batch's each with its own id.
+  // A prefill's rows come sequence by sequence, a decode batch's each with its
+  // own id (LDS atomics / ballots, us, in sequences of 250 rows | of 8 adapters |
+  // of 32 at random: 512 rows 4.7 / 4.2 | 4.2 / 5.3 | 4.4 / 8.8, 1024 5.5 / 4.3 |
+  // 4.4 / 5.4 | 4.5 / 9.2, 2048 7.0 / 4.5 | 4.7 / 6.9 | 4.7 / 15, 8192 18.5 / 7.7 |
+  // 8.7 / 18.7 | 8.3 / 51).
+  constexpr int kRunRows = 1024;
 #define SGL_ROUTE_L(RUNS_)                                                                                          \
   hipLaunchKernelGGL((lora_route_kernel<RUNS_>), dim3(1), dim3(kAlignThreads), 0, s, ids, (int)n, (int)(L + 1),     \
                      kLoraBlock, sorted, bucket, (int)moe_block_capacity(n, L + 1, kLoraBlock), num_post_pad, offsets)
-  if (n >= kLoraTileRows)
+  if (n >= kRunRows)
     SGL_ROUTE_L(true);
   else
     SGL_ROUTE_L(false);

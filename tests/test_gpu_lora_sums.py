@@ -10,7 +10,7 @@ DEV = "cuda"
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("R", [8, 64, 128, 256])
-@pytest.mark.parametrize("M", [1, 16, 40, 600])
+@pytest.mark.parametrize("M", [1, 16, 40, 600, 1600])
 def test_differences_of_large_sums_are_exact(M, R, dtype):
     """Each sum is a whole number of 23 bits, its digits in A and their places in x, so that fp32 adds them exactly;
     B takes the difference, at most 127, of two of them: every value on the way is exact, and so is the output."""
