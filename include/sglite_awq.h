@@ -63,7 +63,8 @@ const char* awq_version(void);
  *      calls) is new.
  * Calls added since without a change to an existing one keep the revision
  * (awq_moe_route with AWQ_DTYPE_FP32, awq_gemm_plan_ring, awq_gemm_launch_info,
- * the AWQ_PLAN_RING knobs): a caller that binds them by name finds out there.
+ * the AWQ_PLAN_RING knobs, awq_moe_dense_gemm, awq_lora_route,
+ * awq_lora_workspace_bytes, awq_lora_add): a caller that binds them by name finds out there.
  * No counterpart in the reference (its kernels are Python and Triton). */
 #define AWQ_ABI_VERSION 4
 int awq_abi_version(void);

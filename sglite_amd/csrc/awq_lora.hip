@@ -19,10 +19,11 @@
 //
 // Three sizes of batch:
 //   few rows   every row is a block of its own, its adapter read from the ids:
-//              nothing is sorted, and a kernel waits for two loads in a row
-//              (id, then weights) and no more.  (Both steps in one launch,
-//              every workgroup computing v for itself, took as long: a CU by
-//              itself draws the 80 to 160 KB of A in 4 us and more.)
+//              nothing is sorted, and the shrink waits for two loads in a row
+//              (id, then weights) and no more; the expand, as compiled, for v
+//              first.  (Both steps in one launch, every workgroup computing v
+//              for itself, took as long: a CU by itself draws the 80 to 160 KB
+//              of A in 4 us and more.)
 //   batches    16-row blocks of the sorted table
 //   prefill    64-row tiles, what their waves share staged in LDS
 #include <math.h>
@@ -129,13 +130,16 @@ __device__ __forceinline__ uint32_t a_offset(const ShrinkArgs& a, int q, int i, 
 
 // One rank tile of one block; a wave's share of the k-steps, one step ahead,
 // straight from global memory: no other wave reads these k.  The waves of other
-// workgroups fill the time; loads further ahead mostly lie past the short slices
-// (layers of Qwen3-4B at 1 row / 32 rows unsorted / Llama-3-8B at 128 rows over 32
-// adapters of rank 64: one step ahead 263 / 424 / 484 us, two 266 / 435 / 491, three
-// 270 / 444 / 500, five 275 / 460 / 513).
+// workgroups fill the time.  Depths measured on this loop (layers of Qwen3-4B at
+// 1 row / 32 rows unsorted / Llama-3-8B at 128 rows over 32 adapters of rank 64):
+// one step ahead 263 / 424 / 484 us, two 266 / 435 / 491, three 270 / 444 / 500,
+// five 275 / 460 / 513.  (The break between the two steps of its body gives the
+// loop two ways back to its head, where the compiler waits for three of the four
+// loads in flight: every second step starts nearly empty.  What a loop without
+// it would gain from depth is not known.)
 // Bound by the chain id -> weights -> sum for single rows (Qwen3-4B qkv, rank 16,
-// 0.25 MB of A: 3.2 us under the profiler), by the loads of A for batches
-// (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 15.5 us, 3.2 TB/s).
+// 0.25 MB of A: 2.2 to 4.6 us under the profiler), by the loads of A for batches
+// (Llama-3-8B qkv, 128 rows over 32 adapters of rank 64: 50 MB in 16 us, 3.1 TB/s).
 // grid: (blocks, k-slices, rank tiles).
 constexpr int kShrinkWaves = 4;
 
@@ -202,8 +206,8 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
 // straight into MFMA operands and the rows shared through a ring of LDS slots
 // filled by LDS-DMA, whole 128-byte lines of a row at a time.  Blocks of
 // different adapters in the four are taken in turn, the others' rows as zeros.
-// 8192 rows over 8 adapters of rank 64, Llama-3-8B qkv / o / gate_up / down: 57 /
-// 27 / 43 / 87 us, x at 1.2 to 2.7 TB/s.  Bound by the reads of A through L2,
+// 8192 rows over 8 adapters of rank 64, Llama-3-8B qkv / o / gate_up / down: 55 /
+// 29 / 44 / 87 us, x at 1.2 to 2.7 TB/s.  Bound by the reads of A through L2,
 // three times x's bytes for qkv's 192 ranks, and the wait for them at each step.
 // grid: (groups of four blocks and k-slices, groups of 4 RT rank tiles).
 constexpr int kShrinkRows = 64;
@@ -338,7 +342,10 @@ __device__ __forceinline__ void load_v(const VArgs& a, int64_t pos, int part, in
   for (int k = 0; k < KC; ++k) {
     v[k][0] = v[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (32 * k + 8 * g >= limit) continue;
-    // All in flight at once: one by one a wave waited for each in turn.
+    // Asked for ahead of the first sum.  The compiler keeps a branch for each
+    // slice and waits at joins: up to 32 ranks of a block have all slices in
+    // flight, further ranks and the prefill kernel's slices mostly come one after
+    // the other, a single row's first slice by itself.
     f32x4 t[S][2];
 #pragma unroll
     for (int s = 0; s < S; ++s) {
@@ -522,14 +529,15 @@ struct ExpandCols {
 };
 
 // Few rows and batches: a wave is a row block and one or two column steps, v
-// split by every wave for itself.  A single row's loads go out beside its id as
-// far as they do not hang on it: v's partial sums and y; the weights follow the
-// id alone.  A block's go out ahead of its v, the second step's ahead of the
-// first one's stores.
-// Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 5.2 us
+// split by every wave for itself.  A single row's y and v are asked for first;
+// the compiled code adds v's slices before it loads the id, and the weights
+// follow that.  A block's y and weights go out ahead of its v, whose waits
+// (load_v) take them in too; the second step's go out ahead of the first one's
+// stores.
+// Bound by that chain for single rows (Qwen3-4B gate_up, rank 16, silu: 4.7 us
 // under the profiler); for batches by it and by the waves that the operands'
 // registers leave room for (Llama-3-8B gate_up, 128 rows over 32 adapters of
-// rank 64: 128 MB in 34.6 us, 3.7 TB/s).
+// rank 64: 128 MB in 34.8 us, 3.7 TB/s).
 template <bool ROWS, int KC, int CT, int ACT, typename DT>
 __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 : 3) void lora_expand_kernel(ExpandArgs a) {
   using Cols = ExpandCols<KC, CT, ACT, DT>;
@@ -596,10 +604,13 @@ __global__ __launch_bounds__(64 * kLoraWaves, KC > 2 ? 1 : ROWS || KC == 1 ? 4 :
 // Prefill: a workgroup is four row blocks, one a wave, and `per` steps of 64
 // columns (32 gate and their 32 up ones).  A wave's v becomes MFMA operands
 // once; the columns' rows of B come through a ring of LDS slots filled by
-// LDS-DMA, shared by the waves, and y into registers, both D steps ahead.
-// Blocks of different adapters in the four are taken in turn.  Bound by reading
-// y and writing the output, and by each workgroup's start: 8192 rows of rank 64,
-// Llama-3-8B gate_up with silu 242 us for 705 MB, 2.9 TB/s; qkv 77 us, o 57 us.
+// LDS-DMA, shared by the waves, and y into registers, both issued D steps ahead.
+// (The wait leaves room for D - 1 steps' loads; the stores in between count among
+// them, so that it takes in the next step's loads too, half of them with an
+// activation.)  Blocks of different adapters in the four are taken in turn.  Bound
+// by reading y and writing the output, and by each workgroup's start, most of it
+// v's slices one after the other (load_v): 8192 rows of rank 64, bf16, Llama-3-8B
+// gate_up with silu 246 us for 705 MB, 2.9 TB/s; qkv 84 us, o 52 us.
 constexpr int kExpandSlots = 4;
 
 // Waves a SIMD: with three terms of 64 ranks two, since three spill 8 to 9
@@ -685,9 +696,10 @@ __global__ __launch_bounds__(64 * kLoraWaves, expand_tile_waves(KC, kTerms<DT>))
     };
 #pragma unroll
     for (int p = 0; p < D; ++p) issue(y[p], p, p);
-    // Step s: wait until its loads have landed (those of the D - 1 steps after
-    // it may be in flight), meet the other waves and issue step s + D into the
-    // slot that every wave is done with.  Steps past the last store nothing.
+    // Step s: wait until its loads have landed (with no stores between, those of
+    // the D - 1 steps after it may be in flight), meet the other waves and issue
+    // step s + D into the slot that every wave is done with.  Steps past the last
+    // store nothing.
     for (int s0 = 0; s0 < steps; s0 += kExpandSlots) {
 #pragma unroll
       for (int d = 0; d <= D; ++d) {

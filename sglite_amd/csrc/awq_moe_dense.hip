@@ -54,11 +54,13 @@ __device__ __forceinline__ void dense_store4(const DenseArgs& a, int sid, float 
 // Few rows per expert: a workgroup is one 16-row tile and 16 NT columns (of each
 // half, with an activation), its four waves split K and load weights and rows
 // straight into MFMA operands: each wave reads other k, so LDS would share
-// nothing.  Bound by reading each busy expert's weights once.  What keeps the
-// loads in flight is many short waves, not deep ones: one step ahead against two
-// and three 223 / 229 / 238 us for both products of E = 128, H = 2048, I = 768
-// top-8 at 32 tokens (4.7 TB/s of weights), 31.5 / 32.3 / 32.5 at one; two
-// waves 227 and 32.0, eight 268 and 33.0.
+// nothing.  Bound by reading each busy expert's weights once; the loads in flight
+// are those of many short waves.  One step ahead against two and three took 223 /
+// 229 / 238 us for both products of E = 128, H = 2048, I = 768 top-8 at 32 tokens
+// (4.7 TB/s of weights), 31.5 / 32.3 / 32.5 at one; two waves 227 and 32.0, eight
+// 268 and 33.0.  (Measured on this loop, whose break between the two steps of its
+// body gives it two ways back to its head: the compiler waits there for all loads,
+// and every second step starts with none in flight.)
 constexpr int kDenseWaves = 4;
 
 template <int EPL, int NT, int ACT, typename DT>
@@ -188,8 +190,12 @@ hipError_t launch_rows_act(const DenseArgs& args, const MoeDenseParams& p, hipSt
 // CU takes unit after unit.  Bound by the weights' bytes where experts are short
 // (E = 128, H = 2048, I = 768 top-8 at 512 tokens: gate/up and down 196 + 95 us,
 // 4.2 TB/s) and by the MFMA loop and the last round of units where they are long
-// (E = 16, H = 4096, I = 1408 top-4 at 4001 tokens: 555 GFLOP in 417 + 232 us under
-// the profiler, 0.94 PFLOP/s of both in a captured step).
+// (E = 16, H = 4096, I = 1408 top-4 at 4001 tokens: 555 GFLOP in 419 + 233 us under
+// the profiler; an eager pass of both and the alignment takes 592 us, 0.94 PFLOP/s).
+// The form for more than 128 experts (EPL = 8) keeps 16 registers of buckets a lane
+// and spills 26 (44 with gelu), outside the loop over k: E = 256, H = 2048, I = 768
+// top-8 at 512 / 4096 tokens 553 / 693 us, E = 512 of I = 384 566 / 682 us, for
+// 2.4 GB of weights (4.4 and 4.3 TB/s at 512 tokens).
 constexpr int kTileWaves = 8;
 constexpr int kTileM = 320;
 constexpr int kTileN = 256;
