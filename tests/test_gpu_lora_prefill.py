@@ -16,7 +16,6 @@ TYPES = [torch.float16, torch.bfloat16]
                                            (1601, 72, (264,), 511, 8), (1700, 256, (64, 40, 24), 5, 32)])
 def test_both_sides_of_the_lines(M, K, parts, L, R, dtype):
     y, x, stack, ids = make(M, K, parts, L, R, dtype, [(R, R // 2 + 1, 1, 0, R - 1)[e % 5] for e in range(L)], seed=M)
-    want, err = deltas(y, x, stack, ids)
     for order in (ids, ids.sort().values, ids.sort(descending=True).values):  # scattered and in sequences
         ids.copy_(order)
         want, err = deltas(y, x, stack, ids)
@@ -28,8 +27,9 @@ def test_both_sides_of_the_lines(M, K, parts, L, R, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ["silu", "gelu"])
-def test_gated(act, dtype):
-    y, x, stack, ids = make(1550, 264, (72, 72), 6, 24, dtype, [24, 1, 13, 0, 23, 8])
+@pytest.mark.parametrize("M,R", [(1550, 24), (600, 40), (600, 104)])
+def test_gated(M, R, act, dtype):
+    y, x, stack, ids = make(M, 264, (72, 72), 6, R, dtype, [R, 1, R // 2 + 1, 0, R - 1, 8])
     want, err = gated(*deltas(y, x, stack, ids), act)
     close(ops.lora_add(y, x, stack, ops.lora_route(ids, 6), activation=act), want, err)
 
