@@ -427,6 +427,52 @@ int awq_moe_dense_gemm(const void* a, int64_t a_rows, const void* w, int64_t E, 
 int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64_t H, int dtype,
                        awq_stream_t stream);
 
+/* ---- microscaled 4-bit floating point (MXFP4) ---------------------------------
+ * 32 consecutive k share a power of two:
+ *   value = (-1)^s {0, 0.5, 1, 1.5, 2, 3, 4, 6}[code & 7] * 2^(byte - 127)
+ * Two codes a byte, the lower k in the low bits; a byte of 255 makes its block
+ * NaN.  No counterpart in the reference.
+ *
+ * awq_mx4_quantize    x [rows, K] (dtype AWQ_DTYPE_*, fp32 too) -> codes
+ *   [rows, K / 2], scales [rows, K / 32]: byte = max(floor(log2(max |x|)) + 125, 0)
+ *   over the block, each x 2^(127 - byte) to the nearest value, ties to the even
+ *   code, beyond 6 to 6; a block with an infinity or NaN gets the byte 255
+ * awq_mx4_dequantize  the values, each rounded once to dtype
+ * awq_mx4_weight_bytes, awq_mx4_repack, awq_mx4_unrepack
+ *   E weights [N, K] (codes [E, N, K / 2], scales [E, N, K / 32]) to the layout
+ *   that the products read (w: E weight_bytes, s: E scale_bytes, each weight's
+ *   contiguous) and back
+ * awq_mx4_gemm        out[m, n] = sum_k Q(x)[m, k] W[n, k] (+ bias[n]), Q the
+ *   quantisation above; with an activation (AWQ_ACT_*) N = 2I, gate columns
+ *   first, and out[m, j] = act(gate) * up, [M, I].  fp32 sums, the bias (dtype)
+ *   added to them, one rounding.  ws: awq_mx4_workspace_bytes bytes of any
+ *   content, which no other thread's or stream's call may use meanwhile
+ * awq_mx4_moe_gemm    the same over the expert buckets (awq_moe_dense_gemm's
+ *   arguments and order; w and s of E weights), without a bias; with
+ *   mul_routed_weight each sum times topk_weights[r] first.  Rows that the
+ *   sorted table does not hold are not written
+ * K % 32 == 0, N % 8 == 0, with an activation I % 32 == 0; x, a, w, bias, out and
+ * ws 16-byte aligned.  Limits: K, N and M below 2^24, E <= 512, x of a product
+ * below 2^34 elements, the routed activation rows below 2 GiB. */
+int awq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                     awq_stream_t stream);
+int awq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,
+                       awq_stream_t stream);
+int awq_mx4_weight_bytes(int64_t N, int64_t K, int64_t* weight_bytes, int64_t* scale_bytes);
+int awq_mx4_repack(const void* codes, const void* scales, int64_t E, int64_t N, int64_t K, void* w, void* s,
+                   awq_stream_t stream);
+int awq_mx4_unrepack(const void* w, const void* s, int64_t E, int64_t N, int64_t K, void* codes, void* scales,
+                     awq_stream_t stream);
+int64_t awq_mx4_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation);
+int awq_mx4_gemm(const void* x, const void* w, const void* s, const void* bias, void* out, int64_t M, int64_t N,
+                 int64_t K, int dtype, int activation, void* ws, int64_t ws_bytes, awq_stream_t stream);
+int64_t awq_mx4_moe_workspace_bytes(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K,
+                                    int activation);
+int awq_mx4_moe_gemm(const void* a, int64_t a_rows, const void* w, const void* s, int64_t E, int64_t N, int64_t K,
+                     int dtype, const int32_t* sorted_ids, int64_t sorted_cap, const int32_t* expert_offsets,
+                     const float* topk_weights, int64_t num_routed, int64_t top_k, int activation,
+                     int mul_routed_weight, void* out, void* ws, int64_t ws_bytes, awq_stream_t stream);
+
 /* ---- low-rank adapters beside a projection -----------------------------------
  * Adapters of many requests on one projection's output, in one call for the
  * whole batch.  Row m names adapter e(m); with the adapter's rank r <= max_rank

@@ -77,6 +77,16 @@ SIGNATURES = {
     "awq_moe_dense_gemm": (_int, [_vp, _i64, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64, _int, _int,
                                   _vp, _vp]),
     "awq_moe_sum_reduce": (_int, [_vp, _vp, _i64, _i64, _i64, _int, _vp]),
+    "awq_mx4_quantize": (_int, [_vp, _int, _i64, _i64, _vp, _vp, _vp]),
+    "awq_mx4_dequantize": (_int, [_vp, _vp, _i64, _i64, _int, _vp, _vp]),
+    "awq_mx4_weight_bytes": (_int, [_i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
+    "awq_mx4_repack": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "awq_mx4_unrepack": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "awq_mx4_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "awq_mx4_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _i64, _vp]),
+    "awq_mx4_moe_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "awq_mx4_moe_gemm": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64, _int,
+                                _int, _vp, _vp, _i64, _vp]),
     "awq_lora_route": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "awq_lora_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int, _int]),
     "awq_lora_add": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _int,

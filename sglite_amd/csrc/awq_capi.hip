@@ -18,6 +18,7 @@
 #include "awq_epilogue.h"
 #include "awq_fixup.h"
 #include "awq_launch.h"
+#include "awq_mx4.h"
 
 using namespace sgl_awq;
 
@@ -840,6 +841,237 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
   if (!aligned(in, 16) || !aligned(out, 16))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_sum_reduce: in and out must be 16-byte aligned");
   return hip_status(launch_moe_sum(in, out, T, topk, H, dtype, (hipStream_t)stream), "awq_moe_sum_reduce launch");
+}
+
+namespace {
+
+// Shapes of MXFP4 tensors [rows, K] and weights [N, K].
+int check_mx4(int64_t rows, int64_t K, const char* who) {
+  if (rows < 0 || K <= 0 || K % kMxBlock != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: K must be a positive multiple of %d (rows=%lld, K=%lld)", who,
+                kMxBlock, (long long)rows, (long long)K);
+  if (K >= (int64_t(1) << 24)) return fail(AWQ_STATUS_UNSUPPORTED, "%s: K must be below 2^24, got %lld", who, (long long)K);
+  return AWQ_STATUS_OK;
+}
+
+int check_mx4_weight(int64_t N, int64_t K, int activation, const char* who) {
+  const int st = check_mx4(0, K, who);
+  if (st != 0) return st;
+  if (N <= 0 || N % 8 != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: N must be a positive multiple of 8, got %lld", who, (long long)N);
+  if (activation != 0 && activation != AWQ_ACT_SILU && activation != AWQ_ACT_GELU)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: unknown activation %d", who, activation);
+  if (activation != 0 && N % 64 != 0)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: gate/up pairing needs N = 2I with I %% 32 == 0, got N=%lld", who,
+                (long long)N);
+  if (N >= (int64_t(1) << 24)) return fail(AWQ_STATUS_UNSUPPORTED, "%s: N must be below 2^24, got %lld", who, (long long)N);
+  return AWQ_STATUS_OK;
+}
+
+int check_mx4_workspace(const Mx4Plan& p, const void* ws, int64_t ws_bytes, const char* who) {
+  if (p.grid > kMx4MaxGrid) return fail(AWQ_STATUS_UNSUPPORTED, "%s: too many rows and columns for one launch", who);
+  if (p.ws_bytes == 0) return AWQ_STATUS_OK;
+  if (!ws || ws_bytes < p.ws_bytes)
+    return fail(AWQ_STATUS_WORKSPACE, "%s: workspace of %lld bytes needed, %lld given", who, (long long)p.ws_bytes,
+                (long long)(ws ? ws_bytes : 0));
+  if (!aligned(ws, 16)) return fail(AWQ_STATUS_WORKSPACE, "%s: ws must be 16-byte aligned", who);
+  return AWQ_STATUS_OK;
+}
+
+// Rows that a launch of their own quantises: its threads are counted in 32 bits.
+int check_mx4_rows(int64_t rows, int64_t K, const char* who) {
+  if (rows >= (int64_t(1) << 24) || rows * mx4_ksteps(K) >= (int64_t(1) << 25))
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: x must have below 2^24 rows and 2^34 elements", who);
+  return AWQ_STATUS_OK;
+}
+
+}  // namespace
+
+int awq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                     awq_stream_t stream) {
+  const TraceRange range("awq_mx4_quantize");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16 && dtype != AWQ_DTYPE_FP32)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_quantize: dtype must be 0, 1 or 2, got %d", dtype);
+  const int st = check_mx4(rows, K, "awq_mx4_quantize");
+  if (st != 0) return st;
+  if (rows >= (int64_t(1) << 31) || rows * K >= (int64_t(1) << 35))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_quantize: x must have below 2^35 elements");
+  if (rows == 0) return ok();
+  if (!x || !codes || !scales) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_quantize: null pointer argument");
+  if (!aligned(x, 16) || !aligned(codes, 4))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_quantize: x must be 16-byte and codes 4-byte aligned");
+  return hip_status(launch_mx4_quantize(x, dtype, rows, K, codes, scales, (hipStream_t)stream),
+                    "awq_mx4_quantize launch");
+}
+
+int awq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,
+                       awq_stream_t stream) {
+  const TraceRange range("awq_mx4_dequantize");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16 && dtype != AWQ_DTYPE_FP32)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_dequantize: dtype must be 0, 1 or 2, got %d", dtype);
+  const int st = check_mx4(rows, K, "awq_mx4_dequantize");
+  if (st != 0) return st;
+  if (rows >= (int64_t(1) << 31) || rows * K >= (int64_t(1) << 35))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_dequantize: the tensor must have below 2^35 elements");
+  if (rows == 0) return ok();
+  if (!codes || !scales || !out) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_dequantize: null pointer argument");
+  if (!aligned(codes, 4) || !aligned(out, 16))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_dequantize: codes must be 4-byte and out 16-byte aligned");
+  return hip_status(launch_mx4_dequantize(codes, scales, rows, K, dtype, out, (hipStream_t)stream),
+                    "awq_mx4_dequantize launch");
+}
+
+int awq_mx4_weight_bytes(int64_t N, int64_t K, int64_t* weight_bytes, int64_t* scale_bytes) {
+  const int st = check_mx4_weight(N, K, 0, "awq_mx4_weight_bytes");
+  if (st != 0) return st;
+  if (!weight_bytes || !scale_bytes)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_weight_bytes: null pointer argument");
+  *weight_bytes = mx4_weight_bytes(N, K);
+  *scale_bytes = mx4_scale_bytes(N, K);
+  return ok();
+}
+
+namespace {
+
+int mx4_repack(void* codes, void* scales, int64_t E, int64_t N, int64_t K, void* w, void* ws, bool back,
+               awq_stream_t stream, const char* who) {
+  const TraceRange range(who);
+  const int st = check_mx4_weight(N, K, 0, who);
+  if (st != 0) return st;
+  if (E < 0 || E > 65536)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: E must be in [0, 65536], got %lld", who, (long long)E);
+  if (E > 0 && mx4_tiles(N) * mx4_ksteps(K) >= (int64_t(1) << 24) / E)
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: too many weights for one call", who);
+  if (E == 0) return ok();
+  if (!codes || !scales || !w || !ws) return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: null pointer argument", who);
+  if (!aligned(codes, 16) || !aligned(w, 16) || !aligned(ws, 4))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: codes and w must be 16-byte and s 4-byte aligned", who);
+  return hip_status(launch_mx4_repack(codes, scales, w, ws, E, N, K, back, (hipStream_t)stream), who);
+}
+
+}  // namespace
+
+int awq_mx4_repack(const void* codes, const void* scales, int64_t E, int64_t N, int64_t K, void* w, void* s,
+                   awq_stream_t stream) {
+  return mx4_repack((void*)codes, (void*)scales, E, N, K, w, s, false, stream, "awq_mx4_repack");
+}
+
+int awq_mx4_unrepack(const void* w, const void* s, int64_t E, int64_t N, int64_t K, void* codes, void* scales,
+                     awq_stream_t stream) {
+  return mx4_repack(codes, scales, E, N, K, (void*)w, (void*)s, true, stream, "awq_mx4_unrepack");
+}
+
+int64_t awq_mx4_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation) {
+  int st = check_mx4_weight(N, K, activation, "awq_mx4_workspace_bytes");
+  if (st != 0) return st;
+  if (M < 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_workspace_bytes: M must be non-negative");
+  st = check_mx4_rows(M, K, "awq_mx4_workspace_bytes");
+  if (st != 0) return st;
+  ok();
+  return M == 0 ? 0 : plan_mx4(M, N, K, activation).ws_bytes;
+}
+
+int awq_mx4_gemm(const void* x, const void* w, const void* s, const void* bias, void* out, int64_t M, int64_t N,
+                 int64_t K, int dtype, int activation, void* ws, int64_t ws_bytes, awq_stream_t stream) {
+  const TraceRange range("awq_mx4_gemm");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_gemm: dtype must be 0 or 1, got %d", dtype);
+  int st = check_mx4_weight(N, K, activation, "awq_mx4_gemm");
+  if (st != 0) return st;
+  if (M < 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_gemm: M must be non-negative, got %lld", (long long)M);
+  st = check_mx4_rows(M, K, "awq_mx4_gemm");
+  if (st != 0) return st;
+  if (M == 0) return ok();
+  if (!x || !w || !s || !out) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_gemm: null pointer argument");
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(s, 4) || !aligned(out, 16) || (bias && !aligned(bias, 16)))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_gemm: x, w, bias and out must be 16-byte and s 4-byte aligned");
+  const Mx4Plan plan = plan_mx4(M, N, K, activation);
+  st = check_mx4_workspace(plan, ws, ws_bytes, "awq_mx4_gemm");
+  if (st != 0) return st;
+  Mx4Params p{};
+  p.x = x;
+  p.w = w;
+  p.s = s;
+  p.bias = bias;
+  p.out = out;
+  p.rows = M;
+  p.N = N;
+  p.K = K;
+  p.act = activation;
+  p.dtype = dtype;
+  p.ws = ws;
+  return hip_status(launch_mx4_gemm(p, plan, (hipStream_t)stream), "awq_mx4_gemm launch");
+}
+
+namespace {
+
+int check_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int activation, const char* who) {
+  const int st = check_mx4_weight(N, K, activation, who);
+  if (st != 0) return st;
+  if (E <= 0 || E > 512) return fail(AWQ_STATUS_UNSUPPORTED, "%s: E must be in [1, 512], got %lld", who, (long long)E);
+  if (top_k <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: top_k must be positive", who);
+  if (num_routed < 0 || num_routed >= (int64_t(1) << 24))
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: num_routed must be in [0, 2^24)", who);
+  const int64_t rows = (num_routed + top_k - 1) / top_k;
+  // Row offsets inside one buffer range are 32-bit, past-the-end ones bit 31.
+  if (rows * K * 2 >= (int64_t(1) << 31) || rows * mx4_ksteps(K) * 16 >= (int64_t(1) << 31))
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: the routed activation rows must span below 2 GiB", who);
+  return AWQ_STATUS_OK;
+}
+
+}  // namespace
+
+int64_t awq_mx4_moe_workspace_bytes(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K,
+                                    int activation) {
+  const int st = check_mx4_moe(num_routed, top_k, E, N, K, activation, "awq_mx4_moe_workspace_bytes");
+  if (st != 0) return st;
+  ok();
+  return num_routed == 0 ? 0 : plan_mx4_moe(num_routed, top_k, E, N, K, activation).ws_bytes;
+}
+
+int awq_mx4_moe_gemm(const void* a, int64_t a_rows, const void* w, const void* s, int64_t E, int64_t N, int64_t K,
+                     int dtype, const int32_t* sorted_ids, int64_t sorted_cap, const int32_t* expert_offsets,
+                     const float* topk_weights, int64_t num_routed, int64_t top_k, int activation,
+                     int mul_routed_weight, void* out, void* ws, int64_t ws_bytes, awq_stream_t stream) {
+  const TraceRange range("awq_mx4_moe_gemm");
+  if (dtype != AWQ_DTYPE_FP16 && dtype != AWQ_DTYPE_BF16)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_moe_gemm: dtype must be 0 or 1, got %d", dtype);
+  int st = check_mx4_moe(num_routed, top_k, E, N, K, activation, "awq_mx4_moe_gemm");
+  if (st != 0) return st;
+  if (sorted_cap < 0 || sorted_cap >= (int64_t(1) << 30))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_moe_gemm: sorted_cap must be in [0, 2^30)");
+  const int64_t rows = (num_routed + top_k - 1) / top_k;
+  if (rows > a_rows)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT,
+                "awq_mx4_moe_gemm: %lld routed rows with top_k %lld need %lld activation rows, a has %lld",
+                (long long)num_routed, (long long)top_k, (long long)rows, (long long)a_rows);
+  if (num_routed == 0 || sorted_cap == 0) return ok();
+  if (!a || !w || !s || !sorted_ids || !expert_offsets || !out || (mul_routed_weight && !topk_weights))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_moe_gemm: null pointer argument");
+  if (!aligned(a, 16) || !aligned(w, 16) || !aligned(s, 4) || !aligned(out, 16))
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_moe_gemm: a, w and out must be 16-byte and s 4-byte aligned");
+  const Mx4Plan plan = plan_mx4_moe(num_routed, top_k, E, N, K, activation);
+  st = check_mx4_workspace(plan, ws, ws_bytes, "awq_mx4_moe_gemm");
+  if (st != 0) return st;
+  Mx4Params p{};
+  p.x = a;
+  p.w = w;
+  p.s = s;
+  p.out = out;
+  p.rows = rows;
+  p.N = N;
+  p.K = K;
+  p.act = activation;
+  p.dtype = dtype;
+  p.ws = ws;
+  p.sorted = sorted_ids;
+  p.offsets = expert_offsets;
+  p.topk_w = mul_routed_weight ? topk_weights : nullptr;
+  p.E = E;
+  p.a_div = top_k;
+  p.num_routed = num_routed;
+  p.sorted_cap = sorted_cap;
+  return hip_status(launch_mx4_gemm(p, plan, (hipStream_t)stream), "awq_mx4_moe_gemm launch");
 }
 
 int awq_lora_route(const int32_t* adapter_ids, int64_t M, int64_t num_adapters, int32_t* sorted_ids,

@@ -170,6 +170,45 @@ struct MoeDenseParams {
 };
 hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s);
 
+// Microscaled 4-bit floating point (awq_mx4.h): blocks, values and the weights'
+// tile layout (awq_mx4.hip), products (awq_mx4_gemm.hip).
+hipError_t launch_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                               hipStream_t s);
+// Scales in the rows' order of the products.
+hipError_t launch_mx4_rows_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                                    hipStream_t s);
+hipError_t launch_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,
+                                 hipStream_t s);
+// back: tiles to a checkpoint's order.
+hipError_t launch_mx4_repack(void* codes, void* scales, void* w, void* ws, int64_t E, int64_t N, int64_t K, bool back,
+                             hipStream_t s);
+constexpr int64_t kMx4MaxGrid = 1 << 22;  // workgroups of up to 1024 threads
+struct Mx4Plan {
+  bool pre;            // the rows are quantised by a launch of their own
+  int mt, ntw, waves;  // m-tiles and column tiles of a workgroup, its waves
+  int64_t groups;      // column groups
+  int64_t slots;       // row blocks, for experts those the grid covers at a time
+  int64_t grid, ws_bytes;
+};
+Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act);
+Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act);
+struct Mx4Params {
+  const void* x;
+  const void* w;
+  const void* s;
+  const void* bias;
+  void* out;
+  int64_t rows, N, K;  // rows of x
+  int act, dtype;
+  void* ws;
+  // Experts alone:
+  const int32_t* sorted;   // from launch_moe_align, else null
+  const int32_t* offsets;
+  const float* topk_w;     // null: not multiplied
+  int64_t E, a_div, num_routed, sorted_cap;
+};
+hipError_t launch_mx4_gemm(const Mx4Params& p, const Mx4Plan& plan, hipStream_t s);
+
 // Low-rank adapters beside a projection (awq_lora.hip).
 constexpr int kLoraBlock = 16;    // rows of a block of the sorted table
 constexpr int kLoraParts = 4;     // column parts of a projection, at most

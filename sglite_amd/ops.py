@@ -1119,6 +1119,376 @@ def moe_sum_reduce(inp: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------------------
+# Microscaled 4-bit floating point (MXFP4): blocks of 32 values along the last
+# axis that share a power of two.
+# ---------------------------------------------------------------------------
+
+MX4_BLOCK = 32
+_MX4_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+class Mx4(NamedTuple):
+    """A tensor [..., K] in MXFP4, as checkpoints hold it: the value of code c in a block with byte b is
+    ``(-1)^(c >> 3) * (0, 0.5, 1, 1.5, 2, 3, 4, 6)[c & 7] * 2^(b - 127)``, NaN for b = 255."""
+    codes: torch.Tensor   # uint8 [..., K / 2], the lower k in the low bits
+    scales: torch.Tensor  # uint8 [..., K / 32]
+
+
+class Mx4Weight(NamedTuple):
+    """A weight [N, K], or a stack of experts' [E, N, K], in the layout that the products read (``mx4_repack``)."""
+    w: torch.Tensor  # uint8 [bytes] or [E, bytes]
+    s: torch.Tensor  # uint8 [bytes] or [E, bytes]
+    N: int
+    K: int
+
+    @property
+    def num_experts(self) -> int:
+        if self.w.dim() != 2:
+            raise ValueError("this weight is one linear's, not a stack of experts'")
+        return self.w.shape[0]
+
+    def expert(self, e: int) -> "Mx4Weight":
+        return Mx4Weight(self.w[e], self.s[e], self.N, self.K)
+
+
+def _mx4_rows(K: int) -> None:
+    if K <= 0 or K % MX4_BLOCK:
+        raise ValueError(f"the last axis must be a positive multiple of {MX4_BLOCK}, got {K}")
+
+
+def _check_mx4(q: Mx4) -> Tuple[int, ...]:
+    """Shape of the tensor that q holds."""
+    codes, scales = q
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
+    if codes.dim() < 1 or codes.dim() != scales.dim():
+        raise ValueError("codes and scales must have the same, at least one, axes")
+    K = codes.shape[-1] * 2
+    _mx4_rows(K)
+    if tuple(scales.shape) != tuple(codes.shape[:-1]) + (K // MX4_BLOCK,):
+        raise ValueError(f"scales must be {tuple(codes.shape[:-1]) + (K // MX4_BLOCK,)} beside codes "
+                         f"{tuple(codes.shape)}, got {tuple(scales.shape)}")
+    if codes.device != scales.device:
+        raise ValueError("codes and scales must be on one device")
+    return tuple(codes.shape[:-1]) + (K,)
+
+
+def _mx4_quantize_launch(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    x = _aligned(x)
+    K, dev = x.shape[-1], x.device
+    codes = torch.empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8, device=dev)
+    scales = torch.empty(x.shape[:-1] + (K // MX4_BLOCK,), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().awq_mx4_quantize(x.data_ptr(), _LOGITS_CODE[x.dtype], x.numel() // K, K,
+                                                codes.data_ptr(), scales.data_ptr(), _stream(dev)),
+                   "awq_mx4_quantize")
+    return codes, scales
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_quantize", mutates_args=(), device_types="cuda")
+def _mx4_quantize_op(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _mx4_quantize_launch(x)
+
+
+@_mx4_quantize_op.register_fake
+def _(x):
+    K = x.shape[-1]
+    return (x.new_empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8),
+            x.new_empty(x.shape[:-1] + (K // MX4_BLOCK,), dtype=torch.uint8))
+
+
+def mx4_quantize(x: torch.Tensor) -> Mx4:
+    """x [..., K] (float16, bfloat16 or float32, K a multiple of 32) in MXFP4.
+
+    A block's byte is that of 2^e, e the exponent of its largest magnitude less 2 (at least -127); each value goes to
+    the nearest one, ties to the even code, and beyond 6 * 2^e to that.  A block that holds an infinity or NaN becomes
+    NaN whole."""
+    if x.dtype not in _MX4_DTYPES:
+        raise ValueError(f"MXFP4 is made from float16, bfloat16 or float32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
+    _mx4_rows(x.shape[-1])
+    _require_cuda(x)
+    if _undispatched(x):
+        return Mx4(*_mx4_quantize_launch(x))
+    return Mx4(*torch.ops.sglite_awq.awq_mx4_quantize(x))
+
+
+def _mx4_dequantize_launch(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    codes, scales = _aligned(codes, 4), scales.contiguous()
+    K, dev = codes.shape[-1] * 2, codes.device
+    out = torch.empty(codes.shape[:-1] + (K,), dtype=dtype, device=dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().awq_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), out.numel() // K, K,
+                                                  _LOGITS_CODE[dtype], out.data_ptr(), _stream(dev)),
+                   "awq_mx4_dequantize")
+    return out
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_dequantize", mutates_args=(), device_types="cuda")
+def _mx4_dequantize_op(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return _mx4_dequantize_launch(codes, scales, dtype)
+
+
+@_mx4_dequantize_op.register_fake
+def _(codes, scales, dtype):
+    return codes.new_empty(codes.shape[:-1] + (codes.shape[-1] * 2,), dtype=dtype)
+
+
+def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of q, [..., K], each rounded once to ``dtype`` (float16, bfloat16 or float32)."""
+    _check_mx4(q)
+    if dtype not in _MX4_DTYPES:
+        raise ValueError(f"values are float16, bfloat16 or float32, got {dtype}")
+    _require_cuda(*q)
+    if _undispatched(*q):
+        return _mx4_dequantize_launch(q.codes, q.scales, dtype)
+    return torch.ops.sglite_awq.awq_mx4_dequantize(q.codes, q.scales, dtype)
+
+
+def mx4_weight_bytes(N: int, K: int) -> Tuple[int, int]:
+    """Bytes of one weight [N, K] and of its scales in the products' layout."""
+    w, s = ctypes.c_int64(), ctypes.c_int64()
+    _lib.check(_lib.load().awq_mx4_weight_bytes(N, K, ctypes.byref(w), ctypes.byref(s)), "awq_mx4_weight_bytes")
+    return w.value, s.value
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_repack", mutates_args=(), device_types="cuda")
+def _mx4_repack_op(codes: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    lead, N, K, dev = tuple(codes.shape[:-2]), codes.shape[-2], codes.shape[-1] * 2, codes.device
+    wb, sb = mx4_weight_bytes(N, K)
+    codes, scales = _aligned(codes), scales.contiguous()
+    w = torch.empty(lead + (wb,), dtype=torch.uint8, device=dev)
+    s = torch.empty(lead + (sb,), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().awq_mx4_repack(codes.data_ptr(), scales.data_ptr(), lead[0] if lead else 1, N, K,
+                                              w.data_ptr(), s.data_ptr(), _stream(dev)), "awq_mx4_repack")
+    return w, s
+
+
+@_mx4_repack_op.register_fake
+def _(codes, scales):
+    wb, sb = mx4_weight_bytes(codes.shape[-2], codes.shape[-1] * 2)
+    return codes.new_empty(codes.shape[:-2] + (wb,)), codes.new_empty(codes.shape[:-2] + (sb,))
+
+
+def mx4_repack(q: Mx4) -> Mx4Weight:
+    """A weight [N, K], or a stack of experts' [E, N, K], laid out for ``mx4_gemm`` and ``mx4_moe_gemm``, once."""
+    shape = _check_mx4(q)
+    if len(shape) not in (2, 3):
+        raise ValueError(f"the weight must be [N, K] or [E, N, K], got {shape}")
+    mx4_weight_bytes(shape[-2], shape[-1])  # refuses sizes that the products cannot take
+    _require_cuda(*q)
+    return Mx4Weight(*torch.ops.sglite_awq.awq_mx4_repack(q.codes, q.scales), shape[-2], shape[-1])
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_unrepack", mutates_args=(), device_types="cuda")
+def _mx4_unrepack_op(w: torch.Tensor, s: torch.Tensor, N: int, K: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    lead, dev = tuple(w.shape[:-1]), w.device
+    codes = torch.empty(lead + (N, K // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty(lead + (N, K // MX4_BLOCK), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().awq_mx4_unrepack(w.data_ptr(), s.data_ptr(), lead[0] if lead else 1, N, K,
+                                                codes.data_ptr(), scales.data_ptr(), _stream(dev)),
+                   "awq_mx4_unrepack")
+    return codes, scales
+
+
+@_mx4_unrepack_op.register_fake
+def _(w, s, N, K):
+    return w.new_empty(w.shape[:-1] + (N, K // 2)), w.new_empty(w.shape[:-1] + (N, K // MX4_BLOCK))
+
+
+def _check_mx4_weight(weight: Mx4Weight, dims: int) -> None:
+    """A weight that mx4_repack made, of one linear (dims 1) or a stack of experts (2)."""
+    if weight.w.dim() != dims or weight.s.dim() != dims or weight.w.shape[:-1] != weight.s.shape[:-1]:
+        raise ValueError("the weight must be " + ("one linear's [N, K]" if dims == 1 else "a stack of experts' [E, N, K]")
+                         + " from mx4_repack")
+    if (weight.w.shape[-1], weight.s.shape[-1]) != mx4_weight_bytes(weight.N, weight.K):
+        raise ValueError(f"the weight does not hold [{weight.N}, {weight.K}]")
+    for t in weight[:2]:
+        if t.dtype != torch.uint8 or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError("the weight must be mx4_repack's: contiguous, 16-byte aligned uint8")
+    if weight.w.device != weight.s.device:
+        raise ValueError("the weight must be on one device")
+
+
+def mx4_unrepack(weight: Mx4Weight) -> Mx4:
+    """The codes and scales that ``mx4_repack`` was given."""
+    _check_mx4_weight(weight, 2 if weight.w.dim() == 2 else 1)
+    _require_cuda(weight.w, weight.s)
+    return Mx4(*torch.ops.sglite_awq.awq_mx4_unrepack(weight.w, weight.s, weight.N, weight.K))
+
+
+def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
+                     out: torch.Tensor, N: int, K: int, act: int) -> None:
+    M = x.shape[0]
+    if M == 0:
+        return
+    dev = x.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _mx4_gemm_launch(x, w, s, bias, out, N, K, act)
+    lib = _lib.load()
+    wsb = _lib.check(lib.awq_mx4_workspace_bytes(M, N, K, act), "awq_mx4_workspace_bytes")
+    ws = _workspace(wsb, dev)
+    _lib.check(lib.awq_mx4_gemm(x.data_ptr(), w.data_ptr(), s.data_ptr(), _ptr(bias), out.data_ptr(), M, N, K,
+                                dtype_code(x.dtype), act, _ptr(ws), wsb, _stream(dev)), "awq_mx4_gemm")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_gemm", mutates_args=(), device_types="cuda")
+def _mx4_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor], N: int, K: int,
+                 activation: str) -> torch.Tensor:
+    act = _ACT_CODE[_ACT_NAME[activation]]
+    out = torch.empty((x.shape[0], N // 2 if act else N), dtype=x.dtype, device=x.device)
+    _mx4_gemm_launch(x, w, s, bias, out, N, K, act)
+    return out
+
+
+@_mx4_gemm_op.register_fake
+def _(x, w, s, bias, N, K, activation):
+    return x.new_empty((x.shape[0], N if activation == "none" else N // 2))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_gemm_out", mutates_args=("out",), device_types="cuda")
+def _mx4_gemm_out_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
+                     out: torch.Tensor, N: int, K: int, activation: str) -> None:
+    _mx4_gemm_launch(x, w, s, bias, out, N, K, _ACT_CODE[_ACT_NAME[activation]])
+
+
+@_mx4_gemm_out_op.register_fake
+def _(x, w, s, bias, out, N, K, activation):
+    return None
+
+
+def _check_mx4_product(x: torch.Tensor, weight: Mx4Weight, activation: Optional[str], dims: int) -> None:
+    _check_mx4_weight(weight, dims)
+    if x.dim() != 2 or x.shape[1] != weight.K:
+        raise ValueError(f"the activations must be [rows, {weight.K}], got {tuple(x.shape)}")
+    if x.dtype not in _DTYPE_CODE:
+        raise ValueError(f"MXFP4 products take float16 and bfloat16 activations, got {x.dtype}")
+    if activation not in _ACT_CODE:
+        raise ValueError(f"unsupported activation {activation!r}")
+    if activation is not None and weight.N % (2 * MX4_BLOCK):
+        raise ValueError(f"gate and up must have a multiple of {MX4_BLOCK} columns each, the weight has {weight.N}")
+    if weight.w.device != x.device:
+        raise ValueError("the activations and the weight must be on one device")
+
+
+def _check_mx4_out(out: torch.Tensor, shape: Tuple[int, ...], x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    _check_out(out, shape, x.dtype, x.device)
+    if out.data_ptr() % 16:
+        raise ValueError("out must be 16-byte aligned")
+    if any(t is not None and _overlap(out, t) for t in (x,) + others):
+        raise ValueError("out must not share memory with an input")
+
+
+def mx4_gemm(x: torch.Tensor, weight: Mx4Weight, bias: Optional[torch.Tensor] = None,
+             activation: Optional[str] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``Q(x) W^T (+ bias)`` of x [M, K] (float16 or bfloat16), Q being ``mx4_quantize``, on x's current stream.
+
+    Exact products, fp32 sums, the bias (taken in x's type) added to them, one rounding.  With ``activation`` ("silu"
+    or "gelu") W's columns are gate and up halves and the result is ``act(gate) * up``, [M, N / 2], of the unrounded
+    sums.  A row that holds an infinity or NaN gives NaN."""
+    _check_mx4_product(x, weight, activation, 1)
+    w, s, N, K = weight
+    _require_cuda(x, w, s, bias)
+    if bias is not None:
+        if bias.numel() != N:
+            raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
+        if bias.device != x.device:
+            raise ValueError("the activations and the bias must be on one device")
+        bias = _aligned(bias.to(x.dtype).reshape(-1))
+    x = _aligned(x)
+    if out is not None:
+        _check_mx4_out(out, (x.shape[0], N if activation is None else N // 2), x, w, s, bias)
+    if _undispatched(x, w, s, bias, out):
+        if out is None:
+            out = torch.empty((x.shape[0], N if activation is None else N // 2), dtype=x.dtype, device=x.device)
+        _mx4_gemm_launch(x, w, s, bias, out, N, K, _ACT_CODE[activation])
+        return out
+    name = "none" if activation is None else activation
+    if out is None:
+        return torch.ops.sglite_awq.awq_mx4_gemm(x, w, s, bias, N, K, name)
+    torch.ops.sglite_awq.awq_mx4_gemm_out(x, w, s, bias, out, N, K, name)
+    return out
+
+
+def _mx4_moe_launch(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_ids: torch.Tensor,
+                    expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, N: int,
+                    K: int, num_routed: int, top_k: int, act: int, mul_routed_weight: bool) -> None:
+    dev = a.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _mx4_moe_launch(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k, act,
+                                   mul_routed_weight)
+    lib, E = _lib.load(), w.shape[0]
+    wsb = _lib.check(lib.awq_mx4_moe_workspace_bytes(num_routed, top_k, E, N, K, act), "awq_mx4_moe_workspace_bytes")
+    ws = _workspace(wsb, dev)
+    _lib.check(lib.awq_mx4_moe_gemm(
+        a.data_ptr(), a.shape[0], w.data_ptr(), s.data_ptr(), E, N, K, dtype_code(a.dtype), sorted_ids.data_ptr(),
+        sorted_ids.numel(), expert_offsets.data_ptr(), _ptr(topk_weights), num_routed, top_k, act,
+        1 if mul_routed_weight else 0, out.data_ptr(), _ptr(ws), wsb, _stream(dev)), "awq_mx4_moe_gemm")
+
+
+@torch.library.custom_op(f"{NAMESPACE}::awq_mx4_moe_gemm", mutates_args=("out",), device_types="cuda")
+def _mx4_moe_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_ids: torch.Tensor,
+                expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, N: int, K: int,
+                num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> None:
+    _mx4_moe_launch(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k,
+                    _ACT_CODE[_ACT_NAME[activation]], mul_routed_weight)
+
+
+@_mx4_moe_op.register_fake
+def _(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k, activation, mul_routed_weight):
+    return None
+
+
+def mx4_moe_gemm(a: torch.Tensor, experts: Mx4Weight, align: MoeAlignment, topk_weights: Optional[torch.Tensor],
+                 num_routed: int, top_k: int, activation: Optional[str] = None, mul_routed_weight: bool = False,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``mx4_gemm`` over the expert buckets with a stack of MXFP4 experts (``mx4_repack`` of [E, N, K]).
+
+    Routed row r reads ``a[r // top_k]``; the output has ``num_routed`` rows of ``N`` columns, or ``N / 2`` of
+    ``act(gate) * up``; with ``mul_routed_weight`` each sum is multiplied by the row's routed weight first.  Rows that
+    ``align`` (16-row blocks) does not hold (ids outside the experts) are not written."""
+    _check_mx4_product(a, experts, activation, 2)
+    w, s, N, K = experts
+    E = w.shape[0]
+    if mul_routed_weight and topk_weights is None:
+        raise ValueError("mul_routed_weight needs topk_weights")
+    if num_routed < 0 or top_k < 1:
+        raise ValueError(f"num_routed must be at least 0 and top_k at least 1, got {num_routed} and {top_k}")
+    if align.expert_offsets.numel() != E + 1:
+        raise ValueError(f"the rows were aligned for {align.expert_offsets.numel() - 1} experts, the stack holds {E}")
+    if align.sorted_ids.dtype != torch.int32 or align.expert_offsets.dtype != torch.int32 \
+            or not align.sorted_ids.is_contiguous() or not align.expert_offsets.is_contiguous():
+        raise ValueError("the alignment must be moe_align_block_size's: contiguous int32")
+    if topk_weights is not None and topk_weights.numel() < num_routed:
+        raise ValueError(f"topk_weights must hold {num_routed} routed weights, got {topk_weights.numel()}")
+    _require_cuda(a, w, topk_weights, align.sorted_ids, align.expert_offsets)
+    for t in (topk_weights, align.sorted_ids, align.expert_offsets):
+        if t is not None and t.device != a.device:
+            raise ValueError("a, the experts, the weights and the alignment must be on one device")
+    a = _aligned(a)
+    shape = (num_routed, N // 2 if activation is not None else N)
+    if out is None:
+        out = torch.empty(shape, dtype=a.dtype, device=a.device)
+    else:
+        _check_mx4_out(out, shape, a, w, s, topk_weights, align.sorted_ids, align.expert_offsets)
+    if topk_weights is not None:
+        topk_weights = _aligned(topk_weights.float().reshape(-1), 4)
+    if _undispatched(a, w, s, topk_weights, out, align.sorted_ids, align.expert_offsets):
+        _mx4_moe_launch(a, w, s, align.sorted_ids, align.expert_offsets, topk_weights, out, N, K, num_routed, top_k,
+                        _ACT_CODE[activation], mul_routed_weight)
+        return out
+    torch.ops.sglite_awq.awq_mx4_moe_gemm(a, w, s, align.sorted_ids, align.expert_offsets, topk_weights, out, N, K,
+                                          num_routed, top_k, "none" if activation is None else activation,
+                                          bool(mul_routed_weight))
+    return out
+
+
+# ---------------------------------------------------------------------------
 # Low-rank adapters of many requests beside a projection (awq_lora_add).
 # ---------------------------------------------------------------------------
 
@@ -1370,5 +1740,6 @@ REGISTERED_OPS: List[str] = [
     "awq_repack_cdna4", "awq_unrepack_cdna4", "awq_dequant", "awq_dequant_repacked", "awq_w4a16_gemm",
     "awq_w4a16_gemm_out", "awq_w4a16_gemm_act", "awq_w4a16_gemm_act_out", "awq_repack_experts",
     "awq_moe_topk_softmax", "awq_moe_align_block_size", "awq_moe_route", "awq_moe_w4a16_gemm", "awq_moe_sum_reduce",
-    "awq_moe_dense_gemm", "awq_lora_route", "awq_lora_add", "awq_lora_add_",
+    "awq_moe_dense_gemm", "awq_mx4_quantize", "awq_mx4_dequantize", "awq_mx4_repack", "awq_mx4_unrepack",
+    "awq_mx4_gemm", "awq_mx4_gemm_out", "awq_mx4_moe_gemm", "awq_lora_route", "awq_lora_add", "awq_lora_add_",
 ]
