@@ -185,6 +185,7 @@ hipError_t launch_mx4_repack(void* codes, void* scales, void* w, void* ws, int64
 constexpr int64_t kMx4MaxGrid = 1 << 22;  // workgroups of up to 1024 threads
 struct Mx4Plan {
   bool pre;            // the rows are quantised by a launch of their own
+  bool tile;           // by tiles of many rows
   int mt, ntw, waves;  // m-tiles and column tiles of a workgroup, its waves
   int64_t groups;      // column groups
   int64_t slots;       // row blocks, for experts those the grid covers at a time

@@ -8,6 +8,7 @@
 // weight.  The products of two codes and their scales are exact; a lane's 32 k
 // are one block of each operand (awq_mx4.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "awq_buffer.h"
 #include "awq_epilogue.h"
@@ -38,7 +39,7 @@ struct MxArgs {
 // a gate tile and its up tile); its waves take k-tiles in turn, load weights
 // straight into MFMA operands and meet in LDS at the end.  PRE: the rows come
 // quantised; else a lane's 32 values are one block, which it quantises itself.
-template <typename DT, bool PRE, int MT, int NTW, int ACT, int EPL>
+template <typename DT, bool PRE, int MT, int NTW, int ACT>
 struct RowsBody {
   using E = typename DT::elem;
   using V4 = typename DT::vec4;
@@ -177,7 +178,7 @@ struct RowsBody {
 template <typename DT, bool PRE, int MT, int NTW, int ACT>
 __global__ __launch_bounds__(1024) void mx4_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
-  RowsBody<DT, PRE, MT, NTW, ACT, 0> b(a);
+  RowsBody<DT, PRE, MT, NTW, ACT> b(a);
   // Workgroup b runs on XCD b % 8: all row blocks of a column group share an L2.
   const int local = blockIdx.x >> 3, group = (blockIdx.x & 7) + 8 * (local / a.slots);
   if (group >= a.groups) return;
@@ -200,17 +201,15 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(MxArgs a) {
 }
 
 // The same for 16 sorted rows of one expert at a time.
-template <typename DT, bool PRE, int NTW, int ACT, int EPL>
+template <typename DT, int NTW, int ACT, int EPL>
 __global__ __launch_bounds__(1024) void mx4_expert_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
-  RowsBody<DT, PRE, 1, NTW, ACT, EPL> b(a);
+  RowsBody<DT, false, 1, NTW, ACT> b(a);
   const int slot = blockIdx.x / a.groups, group = blockIdx.x - slot * a.groups, c = b.lane & 15;
   RowTiles<EPL> tiles;
   tiles.load(a.offsets, a.E, a.sorted_cap, b.lane);
   tiles.scan(16, b.lane);
-  const uint32_t pitch = PRE ? a.K / 2 : a.K * 2;
-  b.xr = make_rsrc(a.x, (uint32_t)a.M * pitch);
-  if constexpr (PRE) b.xsr = make_rsrc(a.xs, (uint32_t)a.M * a.KS * 16u);
+  b.xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u);
   for (int t = slot;; t += a.slots) {
     int e, rb, rows;
     tiles.find(t, 16, b.lane, e, rb, rows);
@@ -225,6 +224,269 @@ __global__ __launch_bounds__(1024) void mx4_expert_rows_kernel(MxArgs a) {
     if (b.wave == 0 && sid >= 0) b.store(red, 0, sid, group, a.topk_w != nullptr ? a.topk_w[sid] : 1.f);
     __syncthreads();  // before the next tile's partial sums
   }
+}
+
+// Many rows: a workgroup of four waves is up to 128 quantised rows and 256 rows of
+// W (with an activation 128 gate and their 128 up rows), two workgroups a CU.
+// The rows go through two LDS stages of 512 k by LDS-DMA, in the order of the
+// MFMA operands; a wave's weights are its own (64 columns) and go straight to
+// registers, two k-tiles ahead.
+constexpr int kMxTileM = 128;
+constexpr int kMxTileGrain = 32;  // a tile's rows come in multiples of two m-tiles
+constexpr int kMxCodes = 4 * (kMxTileM / 16) * 64;      // 16-byte vectors of a stage's codes
+constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 bytes a row
+constexpr int kMxTileLds = (2 * kMxStage + kMxTileM / 4) * 16;  // and the row ids
+
+struct MxUnit {
+  __amdgpu_buffer_rsrc_t xr, xsr;
+  int64_t e;    // expert
+  int64_t row0; // first row of the ranges (linear)
+  int group;    // column group
+};
+
+template <int MT, int ACT, typename DT>
+__device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
+                                         const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
+  using E = typename DT::elem;
+  using V8 = typename DT::vec8;
+  const int c = lane & 15, g = lane >> 4;
+  // The wave's two pairs of column tiles; one past the last is the last again and not stored.
+  const int pairs = ACT == kActNone ? a.NT / 2 : a.half / 2;
+  int pair[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    pair[h] = ACT == kActNone ? min(u.group * 8 + wave * 2 + h, pairs - 1) : min(u.group * 4 + wave, pairs - 1) + h * pairs;
+  __amdgpu_buffer_rsrc_t wr[2], sr[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t t = u.e * a.NT + 2 * pair[h];
+    wr[h] = make_rsrc(a.w + t * a.KT * 1024, (uint32_t)a.KT * 2048u);
+    sr[h] = make_rsrc(a.s + t * a.KS * 256, (uint32_t)a.KS * 512u);
+  }
+  struct Weights {
+    u32x4 q[4];
+  };
+  auto load_w = [&](Weights& w, int kt) {
+    kt = min(kt, a.KT - 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w.q[j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j >> 1], lane * 16, ((j & 1) * a.KT + kt) * 1024, 0);
+  };
+  auto load_s = [&](uint32_t (&sw)[4], int s) {
+    s = min(s, a.KS - 1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      sw[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j >> 1], lane * 4, ((j & 1) * a.KS + s) * 256, 0);
+  };
+  // Stage s's codes of m-tiles m0 .. m1 - 1: wave w brings k-tile w.
+  auto dma = [&](int s, int m0, int m1) {
+    u32x4* buf = lds + (s & 1) * kMxStage;
+    const uint32_t dead = s < a.KS && s * 512 + 128 * wave + 32 * g < a.K ? 0u : kPastEnd;
+#pragma unroll
+    for (int m = m0; m < m1; ++m) load_lds16(u.xr, buf + (wave * MT + m) * 64, (xrow[m] + 64u * wave) | dead, s * 256);
+  };
+  auto dma_scales = [&](int s) {
+    if (wave * 64 < MT * 16)
+      load_lds16(u.xsr, lds + (s & 1) * kMxStage + kMxCodes + wave * 64, xsrow | (s < a.KS ? 0u : kPastEnd), s * 16);
+  };
+
+  f32x4 acc[MT][4];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Weights w[4];
+  uint32_t sw[2][4];
+  load_s(sw[0], 0);
+  dma(0, 0, MT);
+  dma_scales(0);
+  __builtin_amdgcn_sched_barrier(0);  // the wait counts the weights' loads behind these
+  load_w(w[0], 0);
+  load_w(w[1], 1);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(8));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+
+  auto step = [&](auto bb, int s, uint32_t (&now)[4], uint32_t (&next)[4], const uint32_t (&sx)[MT]) {
+    constexpr int b = decltype(bb)::value;
+    if constexpr (b == 0) {
+      load_s(next, s + 1);
+      dma(s + 1, 0, MT / 2);
+    }
+    if constexpr (b == 1) {
+      dma(s + 1, MT / 2, MT);
+      dma_scales(s + 1);
+    }
+    load_w(w[(b + 2) & 3], 4 * s + b + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    const u32x4* xs = lds + (s & 1) * kMxStage + b * MT * 64 + lane;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const u32x4 x = xs[m * 64];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[m][j] = mfma_mx4<b, b>(w[b].q[j], x, now[j], sx[m], acc[m][j]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto super = [&](int s, uint32_t (&now)[4], uint32_t (&next)[4]) {
+    uint32_t sx[MT];
+    const uint32_t* at = (const uint32_t*)(lds + (s & 1) * kMxStage + kMxCodes) + c * 4 + g;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) sx[m] = at[m * 64];
+    step(std::integral_constant<int, 0>{}, s, now, next, sx);
+    step(std::integral_constant<int, 1>{}, s, now, next, sx);
+    step(std::integral_constant<int, 2>{}, s, now, next, sx);
+    step(std::integral_constant<int, 3>{}, s, now, next, sx);
+    // Stage s + 1 has landed when at most the weights of the last two steps are
+    // outstanding; every wave is done with stage s.
+    __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(8));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  for (int s = 0; s < a.KS; s += 2) {
+    super(s, sw[0], sw[1]);
+    if (s + 1 < a.KS) super(s + 1, sw[1], sw[0]);
+  }
+
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int sid = sids[m * 16 + c];
+    if (sid < 0) continue;
+    const float rw = a.topk_w != nullptr ? a.topk_w[sid] : 1.f;
+    E* out = (E*)a.out + (u.row0 + sid) * a.cols;
+#pragma unroll
+    for (int h = 0; h < (ACT == kActNone ? 2 : 1); ++h) {
+      const int p = ACT == kActNone ? u.group * 8 + wave * 2 + h : u.group * 4 + wave;
+      const int n = 32 * p + 8 * g;
+      if (n >= a.cols) continue;  // columns come in multiples of 8
+      float v[2][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[0][i] = acc[m][2 * h + (i >> 2)][i & 3] * rw;
+        if constexpr (ACT != kActNone) v[1][i] = acc[m][2 + (i >> 2)][i & 3] * rw;
+      }
+      if (a.bias != nullptr) {
+#pragma unroll
+        for (int k = 0; k < (ACT == kActNone ? 1 : 2); ++k) {
+          const V8 bias = *(const V8*)((const E*)a.bias + k * a.cols + n);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[k][i] += (float)bias[i];
+        }
+      }
+      V8 r;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (ACT == kActNone)
+          r[i] = (E)v[0][i];
+        else
+          r[i] = (E)(gated_act_fast(ACT, v[0][i]) * v[1][i]);
+      }
+      *(V8*)(out + n) = r;
+    }
+  }
+}
+
+template <int ACT, typename DT>
+__device__ __forceinline__ void mx4_tile_of(int rows, const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
+                                            const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
+  switch ((rows + kMxTileGrain - 1) / kMxTileGrain) {
+    case 1: mx4_tile<2, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 2: mx4_tile<4, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 3: mx4_tile<6, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    default: mx4_tile<8, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane);
+  }
+}
+
+// The offsets of the lane's rows (row ids in sids, -1 for none) in the codes and scales.
+__device__ __forceinline__ void tile_rows(const MxArgs& a, const int32_t* sids, int div, int wave, int lane,
+                                          uint32_t (&xrow)[kMxTileM / 16], uint32_t& xsrow) {
+  const int c = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int m = 0; m < kMxTileM / 16; ++m) {
+    const int sid = sids[16 * m + c];
+    xrow[m] = sid < 0 ? kPastEnd : (uint32_t)(sid / div) * (uint32_t)(a.K / 2) + 16u * g;
+  }
+  const int sid = wave < 2 ? sids[64 * wave + lane] : -1;
+  xsrow = sid < 0 ? kPastEnd : (uint32_t)(sid / div) * (uint32_t)(a.KS * 16);
+}
+
+// Linear layers: unit after unit of (row tile, column group), 8 row tiles by 8
+// groups in turn, so that the workgroups of an XCD (b % 8) share rows and weights
+// in its L2.
+template <int ACT, typename DT>
+__global__ __launch_bounds__(256, 2) void mx4_tile_kernel(MxArgs a) {
+  extern __shared__ u32x4 lds[];
+  int32_t* sids = (int32_t*)(lds + 2 * kMxStage);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int units = a.slots * a.groups, per_xcd = (units + 7) >> 3;
+  // Row tiles of nearly equal height.
+  const int height = ((a.M + a.slots - 1) / a.slots + kMxTileGrain - 1) / kMxTileGrain * kMxTileGrain;
+  for (int at = blockIdx.x >> 3; at < per_xcd; at += gridDim.x >> 3) {
+    const int unit = (blockIdx.x & 7) * per_xcd + at;
+    if (unit >= units) break;
+    const int band = unit / (8 * a.groups), in = unit - band * 8 * a.groups, high = min(8, a.slots - 8 * band);
+    MxUnit u;
+    u.e = 0;
+    u.group = in / high;
+    u.row0 = (int64_t)(8 * band + in - u.group * high) * height;
+    const int rows = (int)min((int64_t)height, a.M - u.row0);
+    if (rows <= 0) continue;
+    u.xr = make_rsrc((const char*)a.x + u.row0 * (a.K / 2), (uint32_t)rows * (uint32_t)(a.K / 2));
+    u.xsr = make_rsrc(a.xs + u.row0 * a.KS * 16, (uint32_t)rows * (uint32_t)a.KS * 16u);
+    __syncthreads();  // the unit before is done with LDS
+    if (threadIdx.x < kMxTileM) sids[threadIdx.x] = threadIdx.x < rows ? threadIdx.x : -1;
+    __syncthreads();
+    uint32_t xrow[kMxTileM / 16], xsrow;
+    tile_rows(a, sids, 1, wave, lane, xrow, xsrow);
+    mx4_tile_of<ACT, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+  }
+}
+
+// Experts: unit after unit of (tile of one expert's sorted rows, column group).
+template <int EPL, int ACT, typename DT>
+__global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
+  extern __shared__ u32x4 lds[];
+  int32_t* sids = (int32_t*)(lds + 2 * kMxStage);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  RowTiles<EPL> tiles;
+  tiles.load(a.offsets, a.E, a.sorted_cap, lane);
+  tiles.scan(kMxTileM, lane);
+  MxUnit u;
+  u.row0 = 0;
+  u.xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)(a.K / 2));
+  u.xsr = make_rsrc(a.xs, (uint32_t)a.M * (uint32_t)a.KS * 16u);
+  const int per_xcd = (tiles.total() * a.groups + 7) >> 3;
+  for (int at = blockIdx.x >> 3; at < per_xcd; at += gridDim.x >> 3) {
+    int e, rb, rows;
+    tiles.find_unit((blockIdx.x & 7) * per_xcd + at, a.groups, kMxTileM, kMxTileGrain, lane, e, rb, rows, u.group);
+    if (e < 0) break;  // the same in every wave
+    u.e = e;
+    int sid = -1;
+    if (threadIdx.x < kMxTileM && (int)threadIdx.x < rows) sid = a.sorted[rb + threadIdx.x];
+    if (sid >= a.num_routed) sid = -1;
+    __syncthreads();  // the unit before is done with LDS
+    if (threadIdx.x < kMxTileM) sids[threadIdx.x] = sid;
+    if (!__syncthreads_or(sid >= 0)) continue;  // padding alone
+    uint32_t xrow[kMxTileM / 16], xsrow;
+    tile_rows(a, sids, a.a_div, wave, lane, xrow, xsrow);
+    mx4_tile_of<ACT, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+  }
+}
+
+template <typename DT, int ACT>
+hipError_t launch_tile(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.grid), block(256);
+  if (a.sorted == nullptr) hipLaunchKernelGGL((mx4_tile_kernel<ACT, DT>), grid, block, kMxTileLds, s, a);
+  else if (a.E <= 128) hipLaunchKernelGGL((mx4_expert_tile_kernel<2, ACT, DT>), grid, block, kMxTileLds, s, a);
+  else hipLaunchKernelGGL((mx4_expert_tile_kernel<8, ACT, DT>), grid, block, kMxTileLds, s, a);
+  return hipGetLastError();
+}
+
+template <typename DT>
+hipError_t launch_tiles(const MxArgs& a, const Mx4Plan& p, int act, hipStream_t s) {
+  if (act == kActSilu) return launch_tile<DT, kActSilu>(a, p, s);
+  if (act == kActGelu) return launch_tile<DT, kActGelu>(a, p, s);
+  return launch_tile<DT, kActNone>(a, p, s);
 }
 
 template <typename DT, bool PRE, int MT, int NTW, int ACT>
@@ -250,17 +512,16 @@ hipError_t launch_linear(const MxArgs& a, const Mx4Plan& p, int act, hipStream_t
   return p.ntw == 1 ? launch_rows<DT, 1, kActNone>(a, p, s) : launch_rows<DT, 2, kActNone>(a, p, s);
 }
 
-template <typename DT, bool PRE, int ACT, int EPL>
+template <typename DT, int ACT, int EPL>
 hipError_t launch_expert_form(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_expert_rows_kernel<DT, PRE, 2, ACT, EPL>), dim3((unsigned)p.grid), dim3(64 * p.waves),
+  hipLaunchKernelGGL((mx4_expert_rows_kernel<DT, 2, ACT, EPL>), dim3((unsigned)p.grid), dim3(64 * p.waves),
                      p.waves * 2 * 1024, s, a);
   return hipGetLastError();
 }
 
 template <typename DT, int ACT>
 hipError_t launch_expert_rows(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
-  if (p.pre) return a.E <= 128 ? launch_expert_form<DT, true, ACT, 2>(a, p, s) : launch_expert_form<DT, true, ACT, 8>(a, p, s);
-  return a.E <= 128 ? launch_expert_form<DT, false, ACT, 2>(a, p, s) : launch_expert_form<DT, false, ACT, 8>(a, p, s);
+  return a.E <= 128 ? launch_expert_form<DT, ACT, 2>(a, p, s) : launch_expert_form<DT, ACT, 8>(a, p, s);
 }
 
 template <typename DT>
@@ -281,6 +542,15 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   p.pre = M > 16;
+  const int64_t col_groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256), row_tiles = (M + kMxTileM - 1) / kMxTileM;
+  if (M > 64 && row_tiles * col_groups >= device_cu_count()) {
+    p.tile = true;
+    p.groups = col_groups;
+    p.slots = row_tiles;
+    p.grid = std::min<int64_t>((row_tiles * col_groups + 7) / 8 * 8, 2 * device_cu_count() / 8 * 8);
+    p.ws_bytes = quantized_bytes(M, K);
+    return p;
+  }
   p.mt = (int)std::min<int64_t>(4, (M + 15) / 16);
   p.slots = (M + 16 * p.mt - 1) / (16 * p.mt);
   p.ntw = act || tiles / 2 * p.slots >= 256 ? 2 : 1;
@@ -295,6 +565,13 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   p.pre = num_routed > 4 * E;
+  p.ws_bytes = p.pre ? quantized_bytes((num_routed + top_k - 1) / top_k, K) : 0;
+  if (p.pre) {
+    p.tile = true;
+    p.groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256);
+    p.grid = 2 * device_cu_count() / 8 * 8;
+    return p;
+  }
   p.mt = 1;
   p.ntw = 2;
   p.groups = tiles / 2;
@@ -302,7 +579,6 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   // Every tile with rows at once, as far as a launch of kMx4MaxGrid workgroups goes.
   p.slots = std::max<int64_t>(1, std::min<int64_t>({num_routed, num_routed / 16 + E, kMx4MaxGrid / p.groups}));
   p.grid = p.slots * p.groups;
-  p.ws_bytes = p.pre ? quantized_bytes((num_routed + top_k - 1) / top_k, K) : 0;
   return p;
 }
 
@@ -336,6 +612,7 @@ hipError_t launch_mx4_gemm(const Mx4Params& p, const Mx4Plan& plan, hipStream_t 
   a.a_div = (int)p.a_div;
   a.num_routed = (int)p.num_routed;
   a.sorted_cap = (int)p.sorted_cap;
+  if (plan.tile) return p.dtype == 0 ? launch_tiles<F16>(a, plan, p.act, s) : launch_tiles<BF16>(a, plan, p.act, s);
   if (p.sorted == nullptr) return p.dtype == 0 ? launch_linear<F16>(a, plan, p.act, s) : launch_linear<BF16>(a, plan, p.act, s);
   return p.dtype == 0 ? launch_experts<F16>(a, plan, p.act, s) : launch_experts<BF16>(a, plan, p.act, s);
 }
