@@ -174,8 +174,11 @@ hipError_t launch_moe_dense(const MoeDenseParams& p, hipStream_t s);
 // tile layout (awq_mx4.hip), products (awq_mx4_gemm.hip).
 hipError_t launch_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
                                hipStream_t s);
-// Scales in the rows' order of the products.
+// A product's activations: row by row with the scales in the rows' order, or in
+// the weights' layout, 16 rows a tile.
 hipError_t launch_mx4_rows_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                                    hipStream_t s);
+hipError_t launch_mx4_tile_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
                                     hipStream_t s);
 hipError_t launch_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,
                                  hipStream_t s);

@@ -16,8 +16,9 @@
 //            i % 4, so that a lane's outputs of a pair are 8 consecutive columns
 //   scales   [NT][KS][64 lanes][4]: byte b of lane (r, g) is that of block
 //            16 s + 4 b + g, the lane's block of k-tile 4 s + b
-//   rows     codes [rows][K / 2] as they are, scales [rows][KS][4 g][4 b] in the
-//            same order
+// A product's quantised activations: of a linear layer in the same layout, rows 16
+// t .. 16 t + 15 in tile t; of experts, which gather them, row by row, codes
+// [rows][K / 2] and scales [rows][KS][4 g][4 b].
 // Columns past N and k past K hold zeros, and scales of 2^-127.
 #pragma once
 

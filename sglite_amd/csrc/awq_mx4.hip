@@ -83,6 +83,33 @@ __global__ __launch_bounds__(kMxThreads) void mx4_rows_quantize_kernel(const voi
   if ((v & 3) == 0) scales[(int64_t)row * (16 * ks) + mx4_row_byte((int)(v >> 2))] = (uint8_t)byte;
 }
 
+// The same in the weights' layout: a wave takes 16 rows and 512 k, a lane its
+// block of each of the four k-tiles.  Rows past the last are read as the last.
+template <typename DT>
+__global__ __launch_bounds__(kMxThreads) void mx4_tile_quantize_kernel(const void* x, u32x4* codes, uint32_t* scales,
+                                                                       uint32_t waves, int M, int K, int KT, int KS) {
+  const uint32_t w = blockIdx.x * (kMxThreads / 64) + (threadIdx.x >> 6);
+  if (w >= waves) return;
+  const int lane = threadIdx.x & 63, tile = w / KS, s = w - tile * KS;
+  const u32x4* row = (const u32x4*)x + (int64_t)min(16 * tile + (lane & 15), M - 1) * (K / 8);
+  u32x4 v[4][4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    const int kb = 16 * s + 4 * b + (lane >> 4);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[b][q] = kb * kMxBlock < K ? row[4 * kb + q] : u32x4{0, 0, 0, 0};
+  }
+  uint32_t word = 0;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    uint32_t byte;
+    const u32x4 c = mx4_block<DT>(v[b], byte);
+    word |= byte << (8 * b);
+    if (4 * s + b < KT) codes[((int64_t)tile * KT + 4 * s + b) * 64 + lane] = c;
+  }
+  scales[(int64_t)w * 64 + lane] = word;
+}
+
 __device__ __forceinline__ float mx4_value(uint32_t code) {
   const uint32_t m = code & 7;
   const uint32_t bits = m >= 2 ? ((m >> 1) + 126) << 23 | (m & 1) << 22 : m ? 0x3F000000u : 0u;
@@ -166,6 +193,16 @@ hipError_t launch_mx4_rows_quantize(const void* x, int dtype, int64_t rows, int6
   else
     hipLaunchKernelGGL(mx4_rows_quantize_kernel<BF16>, grid, block, 0, s, x, c, b, (uint32_t)total, (uint32_t)(K / 8),
                        (uint32_t)ks);
+  return hipGetLastError();
+}
+
+hipError_t launch_mx4_tile_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
+                                    hipStream_t s) {
+  const int64_t KT = mx4_ktiles(K), KS = mx4_ksteps(K), waves = (rows + 15) / 16 * KS;
+  const dim3 grid = blocks_for(waves * 64), block(kMxThreads);
+  const auto kernel = dtype == 0 ? mx4_tile_quantize_kernel<F16> : mx4_tile_quantize_kernel<BF16>;
+  hipLaunchKernelGGL(kernel, grid, block, 0, s, x, (u32x4*)codes, (uint32_t*)scales, (uint32_t)waves, (int)rows,
+                     (int)K, (int)KT, (int)KS);
   return hipGetLastError();
 }
 

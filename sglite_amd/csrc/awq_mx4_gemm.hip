@@ -36,26 +36,31 @@ struct MxArgs {
 };
 
 // Few rows: a workgroup owns 16 MT rows and NTW column tiles (with an activation
-// a gate tile and its up tile); its waves take k-tiles in turn, load weights
-// straight into MFMA operands and meet in LDS at the end.  PRE: the rows come
-// quantised; else a lane's 32 values are one block, which it quantises itself.
+// a gate tile and its up tile); its waves take steps of 512 k in turn, load
+// weights straight into MFMA operands and meet in LDS at the end.  Loads run half
+// a step to a whole one ahead.  PRE: the rows come quantised, in the weights'
+// layout; else a lane's 32 values are one block, which it quantises itself.
+constexpr int kMxRowsWaves = 8;  // at most
+
 template <typename DT, bool PRE, int MT, int NTW, int ACT>
 struct RowsBody {
   using E = typename DT::elem;
   using V4 = typename DT::vec4;
   using V8 = typename DT::vec8;
-  static constexpr int D = !PRE && MT > 1 ? 2 : 4;  // k-tiles in flight
   static constexpr int kPolicy = MT == 4 ? 0 : kCacheStream;
 
-  struct Stage {
-    u32x4 w[NTW], x[MT][PRE ? 1 : 4];
-    uint32_t sw[NTW], sx[MT];
+  struct Half {  // two k-tiles
+    u32x4 w[2][NTW], x[2][MT][PRE ? 1 : 4];
+  };
+  struct Scales {  // of a whole step
+    uint32_t w[NTW], x[PRE ? MT : 1];
   };
 
   const MxArgs& a;
   const int wave, waves, lane;
   __amdgpu_buffer_rsrc_t wr[NTW], sr[NTW], xr, xsr;
-  uint32_t xo[MT], xso[MT];
+  uint32_t xo[MT];  // offsets of the lane's rows, for !PRE
+  int tile[MT];     // row tiles, one past the last is the last, for PRE
 
   __device__ __forceinline__ RowsBody(const MxArgs& args)
       : a(args),
@@ -71,64 +76,85 @@ struct RowsBody {
       sr[j] = make_rsrc(a.s + (e * a.NT + t) * (int64_t)a.KS * 256, (uint32_t)a.KS * 256u);
     }
   }
-  // Row of the lane in m-tile mt, relative to the ranges' first; -1 for none.
+  // The lane's row of m-tile mt, relative to xr's first; -1 for none.
   __device__ __forceinline__ void set_row(int mt, int row) {
-    const int g = lane >> 4;
-    xo[mt] = row < 0 ? kPastEnd : PRE ? (uint32_t)row * (uint32_t)(a.K / 2) + 16u * g : (uint32_t)row * (uint32_t)a.K * 2u + 64u * g;
-    xso[mt] = row < 0 ? kPastEnd : (uint32_t)row * (uint32_t)(a.KS * 16) + 4u * g;
+    xo[mt] = row < 0 ? kPastEnd : (uint32_t)row * (uint32_t)a.K * 2u + 64u * (lane >> 4);
   }
-  __device__ __forceinline__ void load(Stage& st, int kt) const {
-    const uint32_t past = kt < a.KT ? 0u : kPastEnd;
-    const uint32_t dead = kt * 128 + 32 * (lane >> 4) < a.K ? 0u : kPastEnd;  // K is a multiple of 32
+  __device__ __forceinline__ void load(Half& h, int kt0) const {
 #pragma unroll
-    for (int j = 0; j < NTW; ++j) {
-      st.w[j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j], (uint32_t)lane * 16u | past, kt * 1024, kPolicy);
-      st.sw[j] = __builtin_amdgcn_raw_buffer_load_b8(sr[j], ((uint32_t)lane * 4u + (kt & 3)) | past, (kt >> 2) * 256, 0);
-    }
+    for (int b = 0; b < 2; ++b) {
+      const int kt = kt0 + b;
+      const uint32_t past = kt < a.KT ? 0u : kPastEnd;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (PRE) {
-        st.x[mt][0] = __builtin_amdgcn_raw_buffer_load_b128(xr, xo[mt] | dead, kt * 64, 0);
-        st.sx[mt] = __builtin_amdgcn_raw_buffer_load_b8(xsr, (xso[mt] + (kt & 3)) | dead, (kt >> 2) * 16, 0);
-      } else {
+      for (int j = 0; j < NTW; ++j)
+        h.w[b][j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j], (uint32_t)lane * 16u | past, kt * 1024, kPolicy);
+      // K is a multiple of 32: a lane's block lies in its row or past its end.
+      const uint32_t dead = kt * 128 + 32 * (lane >> 4) < a.K ? 0u : kPastEnd;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          st.x[mt][q] = __builtin_amdgcn_raw_buffer_load_b128(xr, (xo[mt] + 16u * q) | dead, kt * 256, 0);
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (PRE) {
+          h.x[b][mt][0] =
+              __builtin_amdgcn_raw_buffer_load_b128(xr, (uint32_t)lane * 16u | past, (tile[mt] * a.KT + kt) * 1024, 0);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            h.x[b][mt][q] = __builtin_amdgcn_raw_buffer_load_b128(xr, (xo[mt] + 16u * q) | dead, kt * 256, 0);
+        }
       }
     }
   }
-  __device__ __forceinline__ void mul(Stage& st, f32x4 (&acc)[MT][NTW]) const {
+  __device__ __forceinline__ void load(Scales& s, int step) const {
+    const uint32_t at = (uint32_t)lane * 4u | (step < a.KS ? 0u : kPastEnd);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      u32x4 x;
-      uint32_t sx;
-      if constexpr (PRE) {
-        x = st.x[mt][0];
-        sx = st.sx[mt];
-      } else {
-        x = mx4_block<DT>(st.x[mt], sx);
-      }
+    for (int j = 0; j < NTW; ++j) s.w[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j], at, step * 256, 0);
+    if constexpr (PRE) {
 #pragma unroll
-      for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<0, 0>(st.w[j], x, st.sw[j], sx, acc[mt][j]);
+      for (int mt = 0; mt < MT; ++mt)
+        s.x[mt] = __builtin_amdgcn_raw_buffer_load_b32(xsr, at, (tile[mt] * a.KS + step) * 256, 0);
     }
   }
-  // The wave's k-tiles, and every wave's sums in red.
+  template <int B>
+  __device__ __forceinline__ void mul(const Half& h, const Scales& s, f32x4 (&acc)[MT][NTW]) const {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if constexpr (PRE) {
+#pragma unroll
+        for (int j = 0; j < NTW; ++j)
+          acc[mt][j] = mfma_mx4<B, B>(h.w[0][j], h.x[0][mt][0], s.w[j], s.x[mt], acc[mt][j]);
+#pragma unroll
+        for (int j = 0; j < NTW; ++j)
+          acc[mt][j] = mfma_mx4<B + 1, B + 1>(h.w[1][j], h.x[1][mt][0], s.w[j], s.x[mt], acc[mt][j]);
+      } else {
+        uint32_t sx;
+        u32x4 x = mx4_block<DT>(h.x[0][mt], sx);
+#pragma unroll
+        for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<B, 0>(h.w[0][j], x, s.w[j], sx, acc[mt][j]);
+        x = mx4_block<DT>(h.x[1][mt], sx);
+#pragma unroll
+        for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<B + 1, 0>(h.w[1][j], x, s.w[j], sx, acc[mt][j]);
+      }
+    }
+  }
+  // The wave's steps, and every wave's sums in red.
   __device__ __forceinline__ void run(f32x4* red) const {
     f32x4 acc[MT][NTW];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int j = 0; j < NTW; ++j) acc[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Stage st[D];
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], wave + d * waves);
-    // Whole rounds of D: a k-tile past the last one loads zeros.
-    for (int kt = wave; kt < a.KT; kt += D * waves) {
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        mul(st[d], acc);
-        load(st[d], kt + (D + d) * waves);
-      }
+    Half h[2];
+    Scales now, next;
+    load(now, wave);
+    load(h[0], 4 * wave);
+    load(h[1], 4 * wave + 2);
+    for (int s = wave; s < a.KS; s += waves) {
+      const int s1 = s + waves;
+      load(next, s1);  // a step past the last one loads zeros, and reads nothing
+      mul<0>(h[0], now, acc);
+      load(h[0], 4 * s1);
+      mul<2>(h[1], now, acc);
+      load(h[1], 4 * s1 + 2);
+      now = next;
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -176,21 +202,27 @@ struct RowsBody {
 };
 
 template <typename DT, bool PRE, int MT, int NTW, int ACT>
-__global__ __launch_bounds__(1024) void mx4_rows_kernel(MxArgs a) {
+__global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
   RowsBody<DT, PRE, MT, NTW, ACT> b(a);
   // Workgroup b runs on XCD b % 8: all row blocks of a column group share an L2.
   const int local = blockIdx.x >> 3, group = (blockIdx.x & 7) + 8 * (local / a.slots);
   if (group >= a.groups) return;
-  const int m0 = local % a.slots * 16 * MT, rows = min(16 * MT, a.M - m0);
+  const int block = local % a.slots, m0 = block * 16 * MT, rows = min(16 * MT, a.M - m0);
   b.set_tiles(0, group);
-  const uint32_t pitch = PRE ? a.K / 2 : a.K * 2;
-  b.xr = make_rsrc((const char*)a.x + (int64_t)m0 * pitch, (uint32_t)rows * pitch);
-  if constexpr (PRE) b.xsr = make_rsrc(a.xs + (int64_t)m0 * a.KS * 16, (uint32_t)rows * a.KS * 16u);
+  if constexpr (PRE) {
+    const uint32_t tiles = (rows + 15) / 16;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = 16 * mt + (b.lane & 15);
-    b.set_row(mt, r < rows ? r : -1);
+    for (int mt = 0; mt < MT; ++mt) b.tile[mt] = min(mt, (int)tiles - 1);
+    b.xr = make_rsrc((const char*)a.x + (int64_t)block * MT * a.KT * 1024, tiles * a.KT * 1024u);
+    b.xsr = make_rsrc(a.xs + (int64_t)block * MT * a.KS * 256, tiles * a.KS * 256u);
+  } else {
+    b.xr = make_rsrc((const char*)a.x + (int64_t)m0 * a.K * 2, (uint32_t)rows * (uint32_t)a.K * 2u);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = 16 * mt + (b.lane & 15);
+      b.set_row(mt, r < rows ? r : -1);
+    }
   }
   b.run(red);
   __syncthreads();
@@ -202,7 +234,7 @@ __global__ __launch_bounds__(1024) void mx4_rows_kernel(MxArgs a) {
 
 // The same for 16 sorted rows of one expert at a time.
 template <typename DT, int NTW, int ACT, int EPL>
-__global__ __launch_bounds__(1024) void mx4_expert_rows_kernel(MxArgs a) {
+__global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
   RowsBody<DT, false, 1, NTW, ACT> b(a);
   const int slot = blockIdx.x / a.groups, group = blockIdx.x - slot * a.groups, c = b.lane & 15;
@@ -242,9 +274,13 @@ struct MxUnit {
   int64_t e;    // expert
   int64_t row0; // first row of the ranges (linear)
   int group;    // column group
+  int tiles;    // m-tiles (linear)
 };
 
-template <int MT, int ACT, typename DT>
+// ROWS: the codes row by row (xrow: offsets of the lane's rows, from its block of
+// the wave's k-tile); else in the weights' layout.  xsrow: the lane's 16 bytes of
+// the wave's scales.
+template <int MT, int ACT, bool ROWS, typename DT>
 __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
                                          const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
   using E = typename DT::elem;
@@ -281,13 +317,23 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
   // Stage s's codes of m-tiles m0 .. m1 - 1: wave w brings k-tile w.
   auto dma = [&](int s, int m0, int m1) {
     u32x4* buf = lds + (s & 1) * kMxStage;
-    const uint32_t dead = s < a.KS && s * 512 + 128 * wave + 32 * g < a.K ? 0u : kPastEnd;
+    const int kt = 4 * s + wave;
+    if constexpr (ROWS) {
+      const uint32_t dead = kt * 128 + 32 * g < a.K ? 0u : kPastEnd;
 #pragma unroll
-    for (int m = m0; m < m1; ++m) load_lds16(u.xr, buf + (wave * MT + m) * 64, (xrow[m] + 64u * wave) | dead, s * 256);
+      for (int m = m0; m < m1; ++m) load_lds16(u.xr, buf + (wave * MT + m) * 64, xrow[m] | dead, kt * 64);
+    } else {
+      const uint32_t at = lane * 16u | (kt < a.KT ? 0u : kPastEnd);
+#pragma unroll
+      for (int m = m0; m < m1; ++m)
+        load_lds16(u.xr, buf + (wave * MT + m) * 64, at, (min(m, u.tiles - 1) * a.KT + kt) * 1024);
+    }
   };
+  // Their scales: rows 64 w .. 64 w + 63 by wave w.
   auto dma_scales = [&](int s) {
     if (wave * 64 < MT * 16)
-      load_lds16(u.xsr, lds + (s & 1) * kMxStage + kMxCodes + wave * 64, xsrow | (s < a.KS ? 0u : kPastEnd), s * 16);
+      load_lds16(u.xsr, lds + (s & 1) * kMxStage + kMxCodes + wave * 64, xsrow | (s < a.KS ? 0u : kPastEnd),
+                 s * (ROWS ? 16 : 256));
   };
 
   f32x4 acc[MT][4];
@@ -330,7 +376,7 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
   };
   auto super = [&](int s, uint32_t (&now)[4], uint32_t (&next)[4]) {
     uint32_t sx[MT];
-    const uint32_t* at = (const uint32_t*)(lds + (s & 1) * kMxStage + kMxCodes) + c * 4 + g;
+    const uint32_t* at = (const uint32_t*)(lds + (s & 1) * kMxStage + kMxCodes) + (ROWS ? c * 4 + g : lane);
 #pragma unroll
     for (int m = 0; m < MT; ++m) sx[m] = at[m * 64];
     step(std::integral_constant<int, 0>{}, s, now, next, sx);
@@ -386,28 +432,15 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
   }
 }
 
-template <int ACT, typename DT>
+template <int ACT, bool ROWS, typename DT>
 __device__ __forceinline__ void mx4_tile_of(int rows, const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
                                             const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
   switch ((rows + kMxTileGrain - 1) / kMxTileGrain) {
-    case 1: mx4_tile<2, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    case 2: mx4_tile<4, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    case 3: mx4_tile<6, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    default: mx4_tile<8, ACT, DT>(a, lds, sids, u, xrow, xsrow, wave, lane);
+    case 1: mx4_tile<2, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 2: mx4_tile<4, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 3: mx4_tile<6, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    default: mx4_tile<8, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane);
   }
-}
-
-// The offsets of the lane's rows (row ids in sids, -1 for none) in the codes and scales.
-__device__ __forceinline__ void tile_rows(const MxArgs& a, const int32_t* sids, int div, int wave, int lane,
-                                          uint32_t (&xrow)[kMxTileM / 16], uint32_t& xsrow) {
-  const int c = lane & 15, g = lane >> 4;
-#pragma unroll
-  for (int m = 0; m < kMxTileM / 16; ++m) {
-    const int sid = sids[16 * m + c];
-    xrow[m] = sid < 0 ? kPastEnd : (uint32_t)(sid / div) * (uint32_t)(a.K / 2) + 16u * g;
-  }
-  const int sid = wave < 2 ? sids[64 * wave + lane] : -1;
-  xsrow = sid < 0 ? kPastEnd : (uint32_t)(sid / div) * (uint32_t)(a.KS * 16);
 }
 
 // Linear layers: unit after unit of (row tile, column group), 8 row tiles by 8
@@ -431,14 +464,17 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(MxArgs a) {
     u.row0 = (int64_t)(8 * band + in - u.group * high) * height;
     const int rows = (int)min((int64_t)height, a.M - u.row0);
     if (rows <= 0) continue;
-    u.xr = make_rsrc((const char*)a.x + u.row0 * (a.K / 2), (uint32_t)rows * (uint32_t)(a.K / 2));
-    u.xsr = make_rsrc(a.xs + u.row0 * a.KS * 16, (uint32_t)rows * (uint32_t)a.KS * 16u);
+    u.tiles = (rows + 15) / 16;  // row0 is a multiple of 16
+    u.xr = make_rsrc((const char*)a.x + u.row0 / 16 * a.KT * 1024, (uint32_t)u.tiles * (uint32_t)a.KT * 1024u);
+    u.xsr = make_rsrc(a.xs + u.row0 / 16 * a.KS * 256, (uint32_t)u.tiles * (uint32_t)a.KS * 256u);
     __syncthreads();  // the unit before is done with LDS
     if (threadIdx.x < kMxTileM) sids[threadIdx.x] = threadIdx.x < rows ? threadIdx.x : -1;
     __syncthreads();
-    uint32_t xrow[kMxTileM / 16], xsrow;
-    tile_rows(a, sids, 1, wave, lane, xrow, xsrow);
-    mx4_tile_of<ACT, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+    // 16 bytes of the scales of m-tile 4 wave + lane / 16.
+    const int m = 4 * wave + (lane >> 4);
+    const uint32_t xsrow = m < u.tiles ? (uint32_t)m * a.KS * 256u + 16u * (lane & 15) : kPastEnd;
+    const uint32_t none[kMxTileM / 16] = {};
+    mx4_tile_of<ACT, false, DT>(rows, a, lds, sids, u, none, xsrow, wave, lane);
   }
 }
 
@@ -467,9 +503,15 @@ __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
     __syncthreads();  // the unit before is done with LDS
     if (threadIdx.x < kMxTileM) sids[threadIdx.x] = sid;
     if (!__syncthreads_or(sid >= 0)) continue;  // padding alone
-    uint32_t xrow[kMxTileM / 16], xsrow;
-    tile_rows(a, sids, a.a_div, wave, lane, xrow, xsrow);
-    mx4_tile_of<ACT, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+    uint32_t xrow[kMxTileM / 16];
+#pragma unroll
+    for (int m = 0; m < kMxTileM / 16; ++m) {
+      const int id = sids[16 * m + (lane & 15)];
+      xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * (lane >> 4);
+    }
+    const int id = wave < 2 ? sids[64 * wave + lane] : -1;
+    const uint32_t xsrow = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.KS * 16);
+    mx4_tile_of<ACT, true, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
   }
 }
 
@@ -531,10 +573,19 @@ hipError_t launch_experts(const MxArgs& a, const Mx4Plan& p, int act, hipStream_
   return launch_expert_rows<DT, kActNone>(a, p, s);
 }
 
-int rows_waves(int64_t KT) { return KT >= 64 ? 16 : KT > 20 ? 8 : 4; }
+// Waves of a workgroup of few rows: as many as leave none without a step, in
+// rounds of equal length.
+int rows_waves(int64_t K) {
+  const int64_t steps = mx4_ksteps(K), rounds = (steps + kMxRowsWaves - 1) / kMxRowsWaves;
+  return (int)((steps + rounds - 1) / rounds);
+}
 
-// Quantised rows ahead of the product: codes, then scales.
-int64_t quantized_bytes(int64_t rows, int64_t K) { return (rows * K / 2 + 15) / 16 * 16 + rows * mx4_ksteps(K) * 16; }
+// Quantised rows ahead of the product, codes and scales: of a linear layer in the
+// weights' layout (16 rows a tile), of experts row by row.
+int64_t linear_codes(int64_t rows, int64_t K) { return (rows + 15) / 16 * mx4_ktiles(K) * 1024; }
+int64_t linear_scales(int64_t rows, int64_t K) { return (rows + 15) / 16 * mx4_ksteps(K) * 256; }
+int64_t expert_codes(int64_t rows, int64_t K) { return rows * K / 2; }  // a multiple of 16
+int64_t expert_scales(int64_t rows, int64_t K) { return rows * mx4_ksteps(K) * 16; }
 
 }  // namespace
 
@@ -548,7 +599,7 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
     p.groups = col_groups;
     p.slots = row_tiles;
     p.grid = std::min<int64_t>((row_tiles * col_groups + 7) / 8 * 8, 2 * device_cu_count() / 8 * 8);
-    p.ws_bytes = quantized_bytes(M, K);
+    p.ws_bytes = linear_codes(M, K) + linear_scales(M, K);
     return p;
   }
   p.mt = (int)std::min<int64_t>(4, (M + 15) / 16);
@@ -556,16 +607,17 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   p.ntw = act || tiles / 2 * p.slots >= 256 ? 2 : 1;
   p.groups = act ? tiles / 2 : tiles / p.ntw;
   p.grid = (p.groups + 7) / 8 * 8 * p.slots;
-  p.waves = rows_waves(mx4_ktiles(K));
-  p.ws_bytes = p.pre ? quantized_bytes(M, K) : 0;
+  p.waves = rows_waves(K);
+  p.ws_bytes = p.pre ? linear_codes(M, K) + linear_scales(M, K) : 0;
   return p;
 }
 
 Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
+  const int64_t rows = (num_routed + top_k - 1) / top_k;
   p.pre = num_routed > 4 * E;
-  p.ws_bytes = p.pre ? quantized_bytes((num_routed + top_k - 1) / top_k, K) : 0;
+  p.ws_bytes = p.pre ? expert_codes(rows, K) + expert_scales(rows, K) : 0;
   if (p.pre) {
     p.tile = true;
     p.groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256);
@@ -575,7 +627,7 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   p.mt = 1;
   p.ntw = 2;
   p.groups = tiles / 2;
-  p.waves = rows_waves(mx4_ktiles(K));
+  p.waves = rows_waves(K);
   // Every tile with rows at once, as far as a launch of kMx4MaxGrid workgroups goes.
   p.slots = std::max<int64_t>(1, std::min<int64_t>({num_routed, num_routed / 16 + E, kMx4MaxGrid / p.groups}));
   p.grid = p.slots * p.groups;
@@ -586,8 +638,10 @@ hipError_t launch_mx4_gemm(const Mx4Params& p, const Mx4Plan& plan, hipStream_t 
   MxArgs a{};
   a.x = p.x;
   if (plan.pre) {
-    uint8_t* scales = (uint8_t*)p.ws + (p.rows * p.K / 2 + 15) / 16 * 16;
-    const hipError_t e = launch_mx4_rows_quantize(p.x, p.dtype, p.rows, p.K, p.ws, scales, s);
+    const bool experts = p.sorted != nullptr;
+    uint8_t* scales = (uint8_t*)p.ws + (experts ? expert_codes(p.rows, p.K) : linear_codes(p.rows, p.K));
+    const hipError_t e = experts ? launch_mx4_rows_quantize(p.x, p.dtype, p.rows, p.K, p.ws, scales, s)
+                                 : launch_mx4_tile_quantize(p.x, p.dtype, p.rows, p.K, p.ws, scales, s);
     if (e != hipSuccess) return e;
     a.x = p.ws;
     a.xs = scales;
