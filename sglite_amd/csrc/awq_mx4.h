@@ -114,6 +114,20 @@ __device__ __forceinline__ u32x4 mx4_block(const u32x4 (&v)[4], uint32_t& byte) 
   return r;
 }
 
+// Largest of four neighbouring lanes' values.
+__device__ __forceinline__ uint32_t max4(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));     // lanes 1 0 3 2 of four
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // 2 3 0 1
+}
+
+// One block held by four neighbouring lanes, 8 values each: the lane's codes, and the byte.
+template <typename DT>
+__device__ __forceinline__ uint32_t mx4_quarter(u32x4 v, uint32_t& byte) {
+  const uint32_t m = max_abs16(max_abs16(v[0], v[1]), max_abs16(v[2], v[3]));
+  byte = Mx4From<DT>::byte_of(max4(max(m & 0xFFFFu, m >> 16)));
+  return mx4_codes8<DT>(v, mx4_scale(byte));
+}
+
 // acc + W X^T of 16 weight rows and 16 activation rows over 128 k; SW and SX say
 // which bytes of sw and sx hold the scales.
 template <int SW, int SX>

@@ -12,20 +12,11 @@ constexpr int kMxThreads = 256;
 // What four neighbouring lanes hold of a block, 8 values each.
 struct MxF32 {};
 
-__device__ __forceinline__ uint32_t max4(uint32_t v) {
-  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));  // lanes 1 0 3 2 of four
-  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));  // 2 3 0 1
-}
-
 template <typename DT>
 struct Vec8 {
   u32x4 v;
   __device__ __forceinline__ void load(const void* x, int64_t i) { v = ((const u32x4*)x)[i]; }
-  __device__ __forceinline__ uint32_t quantize(uint32_t& byte) const {
-    uint32_t m = max_abs16(max_abs16(v[0], v[1]), max_abs16(v[2], v[3]));
-    byte = Mx4From<DT>::byte_of(max4(max(m & 0xFFFFu, m >> 16)));
-    return mx4_codes8<DT>(v, mx4_scale(byte));
-  }
+  __device__ __forceinline__ uint32_t quantize(uint32_t& byte) const { return mx4_quarter<DT>(v, byte); }
 };
 template <>
 struct Vec8<MxF32> {

@@ -37,30 +37,29 @@ struct MxArgs {
 
 // Few rows: a workgroup owns 16 MT rows and NTW column tiles (with an activation
 // a gate tile and its up tile); its waves take steps of 512 k in turn, load
-// weights straight into MFMA operands and meet in LDS at the end.  Loads run half
-// a step to a whole one ahead.  PRE: the rows come quantised, in the weights'
-// layout; else a lane's 32 values are one block, which it quantises itself.
-constexpr int kMxRowsWaves = 8;  // at most
+// weights straight into MFMA operands, a step ahead, and meet in LDS at the end.
+// RM = 0: the rows come quantised, in the weights' layout.  Else a wave quantises
+// the step's part of up to 16 rows itself, RM of them loaded ahead: four lanes a
+// block, and through LDS into the operands' order.
+constexpr int kMxRowsWaves = 8;        // at most
+constexpr int kMxRowWords = 68;        // a quantised row's step in LDS: 256 bytes of codes, and 16 against bank conflicts
+constexpr int kMxExpertRows = 4;       // of an expert's rows, loaded ahead
+constexpr int kMxRowsLds = 16 * (kMxRowWords + 4) * 4;  // a wave's, with the scales
 
-template <typename DT, bool PRE, int MT, int NTW, int ACT>
+template <typename DT, int RM, int MT, int NTW, int ACT>
 struct RowsBody {
   using E = typename DT::elem;
   using V4 = typename DT::vec4;
   using V8 = typename DT::vec8;
   static constexpr int kPolicy = MT == 4 ? 0 : kCacheStream;
-
-  struct Half {  // two k-tiles
-    u32x4 w[2][NTW], x[2][MT][PRE ? 1 : 4];
-  };
-  struct Scales {  // of a whole step
-    uint32_t w[NTW], x[PRE ? MT : 1];
-  };
+  static constexpr int XM = RM == 0 ? MT : 1;
 
   const MxArgs& a;
   const int wave, waves, lane;
   __amdgpu_buffer_rsrc_t wr[NTW], sr[NTW], xr, xsr;
-  uint32_t xo[MT];  // offsets of the lane's rows, for !PRE
-  int tile[MT];     // row tiles, one past the last is the last, for PRE
+  int tile[XM];     // RM = 0: row tiles, one past the last is the last
+  int rows;         // else: rows, and the lane's (row lane % 16) offset in xr
+  uint32_t row_at;
 
   __device__ __forceinline__ RowsBody(const MxArgs& args)
       : a(args),
@@ -76,86 +75,137 @@ struct RowsBody {
       sr[j] = make_rsrc(a.s + (e * a.NT + t) * (int64_t)a.KS * 256, (uint32_t)a.KS * 256u);
     }
   }
-  // The lane's row of m-tile mt, relative to xr's first; -1 for none.
-  __device__ __forceinline__ void set_row(int mt, int row) {
-    xo[mt] = row < 0 ? kPastEnd : (uint32_t)row * (uint32_t)a.K * 2u + 64u * (lane >> 4);
+  __device__ __forceinline__ void load_w(u32x4 (&w)[NTW], int kt) const {
+    const uint32_t past = kt < a.KT ? 0u : kPastEnd;
+#pragma unroll
+    for (int j = 0; j < NTW; ++j)
+      w[j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j], (uint32_t)lane * 16u | past, kt * 1024, kPolicy);
   }
-  __device__ __forceinline__ void load(Half& h, int kt0) const {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int kt = kt0 + b;
-      const uint32_t past = kt < a.KT ? 0u : kPastEnd;
-#pragma unroll
-      for (int j = 0; j < NTW; ++j)
-        h.w[b][j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j], (uint32_t)lane * 16u | past, kt * 1024, kPolicy);
-      // K is a multiple of 32: a lane's block lies in its row or past its end.
-      const uint32_t dead = kt * 128 + 32 * (lane >> 4) < a.K ? 0u : kPastEnd;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if constexpr (PRE) {
-          h.x[b][mt][0] =
-              __builtin_amdgcn_raw_buffer_load_b128(xr, (uint32_t)lane * 16u | past, (tile[mt] * a.KT + kt) * 1024, 0);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            h.x[b][mt][q] = __builtin_amdgcn_raw_buffer_load_b128(xr, (xo[mt] + 16u * q) | dead, kt * 256, 0);
-        }
-      }
-    }
-  }
-  __device__ __forceinline__ void load(Scales& s, int step) const {
+  __device__ __forceinline__ void load_s(uint32_t (&s)[NTW], int step) const {
     const uint32_t at = (uint32_t)lane * 4u | (step < a.KS ? 0u : kPastEnd);
 #pragma unroll
-    for (int j = 0; j < NTW; ++j) s.w[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j], at, step * 256, 0);
-    if constexpr (PRE) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        s.x[mt] = __builtin_amdgcn_raw_buffer_load_b32(xsr, at, (tile[mt] * a.KS + step) * 256, 0);
-    }
+    for (int j = 0; j < NTW; ++j) s[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j], at, step * 256, 0);
   }
   template <int B>
-  __device__ __forceinline__ void mul(const Half& h, const Scales& s, f32x4 (&acc)[MT][NTW]) const {
+  __device__ __forceinline__ void mul(const u32x4 (&w)[NTW], const uint32_t (&sw)[NTW], const u32x4 (&x)[XM],
+                                      const uint32_t (&sx)[XM], f32x4 (&acc)[MT][NTW]) const {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (PRE) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int j = 0; j < NTW; ++j)
-          acc[mt][j] = mfma_mx4<B, B>(h.w[0][j], h.x[0][mt][0], s.w[j], s.x[mt], acc[mt][j]);
+      for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<B, B>(w[j], x[mt], sw[j], sx[mt], acc[mt][j]);
+  }
+
+  // Quantised rows.
+  __device__ __forceinline__ void load_x(u32x4 (&x)[XM], int kt) const {
+    const uint32_t at = (uint32_t)lane * 16u | (kt < a.KT ? 0u : kPastEnd);
 #pragma unroll
-        for (int j = 0; j < NTW; ++j)
-          acc[mt][j] = mfma_mx4<B + 1, B + 1>(h.w[1][j], h.x[1][mt][0], s.w[j], s.x[mt], acc[mt][j]);
-      } else {
-        uint32_t sx;
-        u32x4 x = mx4_block<DT>(h.x[0][mt], sx);
+    for (int mt = 0; mt < MT; ++mt)
+      x[mt] = __builtin_amdgcn_raw_buffer_load_b128(xr, at, (tile[mt] * a.KT + kt) * 1024, 0);
+  }
+  __device__ __forceinline__ void load_sx(uint32_t (&s)[XM], int step) const {
+    const uint32_t at = (uint32_t)lane * 4u | (step < a.KS ? 0u : kPastEnd);
 #pragma unroll
-        for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<B, 0>(h.w[0][j], x, s.w[j], sx, acc[mt][j]);
-        x = mx4_block<DT>(h.x[1][mt], sx);
+    for (int mt = 0; mt < MT; ++mt)
+      s[mt] = __builtin_amdgcn_raw_buffer_load_b32(xsr, at, (tile[mt] * a.KS + step) * 256, 0);
+  }
+  __device__ __forceinline__ void steps_quantized(f32x4 (&acc)[MT][NTW]) const {
+    u32x4 w[4][NTW], x[2][XM];
+    uint32_t sw[NTW], sx[XM], sw1[NTW], sx1[XM];
+    load_s(sw, wave);
+    load_sx(sx, wave);
 #pragma unroll
-        for (int j = 0; j < NTW; ++j) acc[mt][j] = mfma_mx4<B + 1, 0>(h.w[1][j], x, s.w[j], sx, acc[mt][j]);
-      }
+    for (int b = 0; b < 4; ++b) load_w(w[b], 4 * wave + b);
+    load_x(x[0], 4 * wave);
+    load_x(x[1], 4 * wave + 1);
+    for (int s = wave; s < a.KS; s += waves) {
+      const int s1 = s + waves;  // a step past the last one loads zeros, and reads nothing
+      load_s(sw1, s1);
+      load_sx(sx1, s1);
+      mul<0>(w[0], sw, x[0], sx, acc);
+      load_w(w[0], 4 * s1);
+      load_x(x[0], 4 * s + 2);
+      mul<1>(w[1], sw, x[1], sx, acc);
+      load_w(w[1], 4 * s1 + 1);
+      load_x(x[1], 4 * s + 3);
+      mul<2>(w[2], sw, x[0], sx, acc);
+      load_w(w[2], 4 * s1 + 2);
+      load_x(x[0], 4 * s1);
+      mul<3>(w[3], sw, x[1], sx, acc);
+      load_w(w[3], 4 * s1 + 3);
+      load_x(x[1], 4 * s1 + 1);
+#pragma unroll
+      for (int j = 0; j < NTW; ++j) sw[j] = sw1[j];
+#pragma unroll
+      for (int mt = 0; mt < XM; ++mt) sx[mt] = sx1[mt];
     }
   }
-  // The wave's steps, and every wave's sums in red.
+
+  // Rows r0 .. r0 + RM - 1 of a step, 8 values a lane.
+  __device__ __forceinline__ void load_rows(u32x4 (&v)[RM ? RM : 1], int r0, int step) const {
+    // K is a multiple of 32: four lanes' block lies in its row or past its end.
+    const uint32_t dead = step * 512 + 8 * lane < a.K ? 0u : kPastEnd;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const uint32_t none = r0 + i < rows ? dead : kPastEnd;
+      const uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)row_at, min(r0 + i, 15));
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, (at + 16u * lane) | none, step * 1024, 0);
+    }
+  }
+  __device__ __forceinline__ void put_rows(const u32x4 (&v)[RM ? RM : 1], int r0, uint32_t* codes) const {
+    uint8_t* scales = (uint8_t*)(codes + 16 * kMxRowWords);
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      if (r0 + i >= rows) break;
+      uint32_t byte;
+      codes[(r0 + i) * kMxRowWords + lane] = mx4_quarter<DT>(v[i], byte);
+      if ((lane & 3) == 0) scales[16 * (r0 + i) + mx4_row_byte(lane >> 2)] = (uint8_t)byte;
+    }
+  }
+  __device__ __forceinline__ void steps_rows(f32x4 (&acc)[MT][NTW], uint32_t* codes) const {
+    u32x4 w[4][NTW], v[RM ? RM : 1];
+    uint32_t sw[NTW], sw1[NTW];
+    load_rows(v, 0, wave);  // ahead of the weights: loads come back in order
+    load_s(sw, wave);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) load_w(w[b], 4 * wave + b);
+    // Lanes of rows that are not there read the last one.
+    const int r = min(lane & 15, rows - 1), g = lane >> 4;
+    for (int s = wave; s < a.KS; s += waves) {
+      const int s1 = s + waves;
+      put_rows(v, 0, codes);
+      for (int r0 = RM; r0 < rows; r0 += RM) {
+        load_rows(v, r0, s);
+        put_rows(v, r0, codes);
+      }
+      load_rows(v, 0, s1);
+      load_s(sw1, s1);
+      const uint32_t sx[XM] = {codes[16 * kMxRowWords + 4 * r + g]};
+      const u32x4* at = (const u32x4*)(codes + r * kMxRowWords) + g;
+      const u32x4 x[4][XM] = {{at[0]}, {at[4]}, {at[8]}, {at[12]}};
+      mul<0>(w[0], sw, x[0], sx, acc);
+      load_w(w[0], 4 * s1);
+      mul<1>(w[1], sw, x[1], sx, acc);
+      load_w(w[1], 4 * s1 + 1);
+      mul<2>(w[2], sw, x[2], sx, acc);
+      load_w(w[2], 4 * s1 + 2);
+      mul<3>(w[3], sw, x[3], sx, acc);
+      load_w(w[3], 4 * s1 + 3);
+#pragma unroll
+      for (int j = 0; j < NTW; ++j) sw[j] = sw1[j];
+    }
+  }
+
+  // The wave's steps, and every wave's sums in red; what the waves quantise lies behind it.
   __device__ __forceinline__ void run(f32x4* red) const {
     f32x4 acc[MT][NTW];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int j = 0; j < NTW; ++j) acc[mt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Half h[2];
-    Scales now, next;
-    load(now, wave);
-    load(h[0], 4 * wave);
-    load(h[1], 4 * wave + 2);
-    for (int s = wave; s < a.KS; s += waves) {
-      const int s1 = s + waves;
-      load(next, s1);  // a step past the last one loads zeros, and reads nothing
-      mul<0>(h[0], now, acc);
-      load(h[0], 4 * s1);
-      mul<2>(h[1], now, acc);
-      load(h[1], 4 * s1 + 2);
-      now = next;
-    }
+    if constexpr (RM == 0)
+      steps_quantized(acc);
+    else
+      steps_rows(acc, (uint32_t*)(red + waves * MT * NTW * 64) + wave * (kMxRowsLds / 4));
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -201,34 +251,31 @@ struct RowsBody {
   }
 };
 
-template <typename DT, bool PRE, int MT, int NTW, int ACT>
+template <typename DT, int RM, int MT, int NTW, int ACT>
 __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
-  RowsBody<DT, PRE, MT, NTW, ACT> b(a);
+  RowsBody<DT, RM, MT, NTW, ACT> b(a);
   // Workgroup b runs on XCD b % 8: all row blocks of a column group share an L2.
   const int local = blockIdx.x >> 3, group = (blockIdx.x & 7) + 8 * (local / a.slots);
   if (group >= a.groups) return;
-  const int block = local % a.slots, m0 = block * 16 * MT, rows = min(16 * MT, a.M - m0);
+  const int block = local % a.slots, m0 = block * 16 * MT;
+  b.rows = min(16 * MT, a.M - m0);
   b.set_tiles(0, group);
-  if constexpr (PRE) {
-    const uint32_t tiles = (rows + 15) / 16;
+  if constexpr (RM == 0) {
+    const uint32_t tiles = (b.rows + 15) / 16;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) b.tile[mt] = min(mt, (int)tiles - 1);
     b.xr = make_rsrc((const char*)a.x + (int64_t)block * MT * a.KT * 1024, tiles * a.KT * 1024u);
     b.xsr = make_rsrc(a.xs + (int64_t)block * MT * a.KS * 256, tiles * a.KS * 256u);
   } else {
-    b.xr = make_rsrc((const char*)a.x + (int64_t)m0 * a.K * 2, (uint32_t)rows * (uint32_t)a.K * 2u);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int r = 16 * mt + (b.lane & 15);
-      b.set_row(mt, r < rows ? r : -1);
-    }
+    b.xr = make_rsrc((const char*)a.x + (int64_t)m0 * a.K * 2, (uint32_t)b.rows * (uint32_t)a.K * 2u);
+    b.row_at = (uint32_t)(b.lane & 15) * (uint32_t)a.K * 2u;
   }
   b.run(red);
   __syncthreads();
   for (int mt = b.wave; mt < MT; mt += b.waves) {
     const int r = 16 * mt + (b.lane & 15);
-    if (r < rows) b.store(red, mt, m0 + r, group, 1.f);
+    if (r < b.rows) b.store(red, mt, m0 + r, group, 1.f);
   }
 }
 
@@ -236,7 +283,7 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_rows_kernel(MxArgs a) {
 template <typename DT, int NTW, int ACT, int EPL>
 __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxArgs a) {
   extern __shared__ f32x4 red[];
-  RowsBody<DT, false, 1, NTW, ACT> b(a);
+  RowsBody<DT, kMxExpertRows, 1, NTW, ACT> b(a);
   const int slot = blockIdx.x / a.groups, group = blockIdx.x - slot * a.groups, c = b.lane & 15;
   RowTiles<EPL> tiles;
   tiles.load(a.offsets, a.E, a.sorted_cap, b.lane);
@@ -248,9 +295,12 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxAr
     if (e < 0) break;  // the same in every wave
     int sid = c < rows ? a.sorted[rb + c] : -1;
     if (sid >= a.num_routed) sid = -1;
-    if (__ballot(sid >= 0) == 0) continue;  // padding alone: the same in every wave
+    // Rows up to the last one that is no padding (the table has it behind them).
+    const uint32_t live = (uint32_t)__ballot(sid >= 0) & 0xFFFFu;
+    if (live == 0) continue;  // padding alone: the same in every wave
+    b.rows = 32 - __builtin_clz(live);
+    b.row_at = sid >= 0 ? (uint32_t)(sid / a.a_div) * (uint32_t)a.K * 2u : kPastEnd;
     b.set_tiles(e, group);
-    b.set_row(0, sid < 0 ? -1 : sid / a.a_div);
     b.run(red);
     __syncthreads();
     if (b.wave == 0 && sid >= 0) b.store(red, 0, sid, group, a.topk_w != nullptr ? a.topk_w[sid] : 1.f);
@@ -531,20 +581,24 @@ hipError_t launch_tiles(const MxArgs& a, const Mx4Plan& p, int act, hipStream_t 
   return launch_tile<DT, kActNone>(a, p, s);
 }
 
-template <typename DT, bool PRE, int MT, int NTW, int ACT>
+template <typename DT, int RM, int MT, int NTW, int ACT>
 hipError_t launch_rows_form(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
-  hipLaunchKernelGGL((mx4_rows_kernel<DT, PRE, MT, NTW, ACT>), dim3((unsigned)p.grid), dim3(64 * p.waves),
-                     p.waves * MT * NTW * 1024, s, a);
+  hipLaunchKernelGGL((mx4_rows_kernel<DT, RM, MT, NTW, ACT>), dim3((unsigned)p.grid), dim3(64 * p.waves),
+                     p.waves * (MT * NTW * 1024 + (RM ? kMxRowsLds : 0)), s, a);
   return hipGetLastError();
 }
 
 template <typename DT, int NTW, int ACT>
 hipError_t launch_rows(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
-  if (!p.pre) return launch_rows_form<DT, false, 1, NTW, ACT>(a, p, s);
-  if (p.mt == 1) return launch_rows_form<DT, true, 1, NTW, ACT>(a, p, s);
-  if (p.mt == 2) return launch_rows_form<DT, true, 2, NTW, ACT>(a, p, s);
-  if (p.mt == 3) return launch_rows_form<DT, true, 3, NTW, ACT>(a, p, s);
-  return launch_rows_form<DT, true, 4, NTW, ACT>(a, p, s);
+  if (!p.pre) {
+    if (a.M == 1) return launch_rows_form<DT, 1, 1, NTW, ACT>(a, p, s);
+    if (a.M <= 4) return launch_rows_form<DT, 4, 1, NTW, ACT>(a, p, s);
+    return launch_rows_form<DT, 8, 1, NTW, ACT>(a, p, s);
+  }
+  if (p.mt == 1) return launch_rows_form<DT, 0, 1, NTW, ACT>(a, p, s);
+  if (p.mt == 2) return launch_rows_form<DT, 0, 2, NTW, ACT>(a, p, s);
+  if (p.mt == 3) return launch_rows_form<DT, 0, 3, NTW, ACT>(a, p, s);
+  return launch_rows_form<DT, 0, 4, NTW, ACT>(a, p, s);
 }
 
 template <typename DT>
@@ -557,7 +611,7 @@ hipError_t launch_linear(const MxArgs& a, const Mx4Plan& p, int act, hipStream_t
 template <typename DT, int ACT, int EPL>
 hipError_t launch_expert_form(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
   hipLaunchKernelGGL((mx4_expert_rows_kernel<DT, 2, ACT, EPL>), dim3((unsigned)p.grid), dim3(64 * p.waves),
-                     p.waves * 2 * 1024, s, a);
+                     p.waves * (2 * 1024 + kMxRowsLds), s, a);
   return hipGetLastError();
 }
 
@@ -572,6 +626,9 @@ hipError_t launch_experts(const MxArgs& a, const Mx4Plan& p, int act, hipStream_
   if (act == kActGelu) return launch_expert_rows<DT, kActGelu>(a, p, s);
   return launch_expert_rows<DT, kActNone>(a, p, s);
 }
+
+// Rows up to which a product quantises them itself.
+constexpr int kMxInlineRows = 16;
 
 // Waves of a workgroup of few rows: as many as leave none without a step, in
 // rounds of equal length.
@@ -592,7 +649,7 @@ int64_t expert_scales(int64_t rows, int64_t K) { return rows * mx4_ksteps(K) * 1
 Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
-  p.pre = M > 16;
+  p.pre = M > kMxInlineRows;
   const int64_t col_groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256), row_tiles = (M + kMxTileM - 1) / kMxTileM;
   if (M > 64 && row_tiles * col_groups >= device_cu_count()) {
     p.tile = true;
