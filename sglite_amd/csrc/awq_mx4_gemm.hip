@@ -308,16 +308,19 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxAr
   }
 }
 
-// Many rows: a workgroup of four waves is up to 128 quantised rows and 256 rows of
-// W (with an activation 128 gate and their 128 up rows), two workgroups a CU.
-// The rows go through two LDS stages of 512 k by LDS-DMA, in the order of the
-// MFMA operands; a wave's weights are its own (64 columns) and go straight to
-// registers, two k-tiles ahead.
+// Many rows: a workgroup of four waves is up to 128 quantised rows and 64 NTW rows
+// of W (with an activation half of them gate rows, the others their up rows).  The
+// rows go through LDS stages of 512 k by LDS-DMA, in the order of the MFMA
+// operands; a wave's weights are its own (NTW column tiles) and go straight to
+// registers.
 constexpr int kMxTileM = 128;
 constexpr int kMxTileGrain = 32;  // a tile's rows come in multiples of two m-tiles
 constexpr int kMxCodes = 4 * (kMxTileM / 16) * 64;      // 16-byte vectors of a stage's codes
 constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 bytes a row
-constexpr int kMxTileLds = (2 * kMxStage + kMxTileM / 4) * 16;  // and the row ids
+// NTW = 4: two stages, weights two k-tiles ahead, two workgroups a CU.  NTW = 2,
+// for grids that leave CUs idle: three stages and weights six k-tiles ahead.
+constexpr int mx4_stages(int ntw) { return ntw == 4 ? 2 : 3; }
+constexpr int mx4_tile_lds(int ntw) { return (mx4_stages(ntw) * kMxStage + kMxTileM / 4) * 16; }  // and the row ids
 
 struct MxUnit {
   __amdgpu_buffer_rsrc_t xr, xsr;
@@ -330,43 +333,43 @@ struct MxUnit {
 // ROWS: the codes row by row (xrow: offsets of the lane's rows, from its block of
 // the wave's k-tile); else in the weights' layout.  xsrow: the lane's 16 bytes of
 // the wave's scales.
-template <int MT, int ACT, bool ROWS, typename DT>
+template <int MT, int NTW, int ACT, bool ROWS, typename DT>
 __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
                                          const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
   using E = typename DT::elem;
-  using V8 = typename DT::vec8;
+  constexpr int NS = mx4_stages(NTW);
+  constexpr int R = NTW == 4 ? 4 : 8, D = NTW == 4 ? 2 : 6;  // k-tiles of weights in registers, and ahead
   const int c = lane & 15, g = lane >> 4;
-  // The wave's two pairs of column tiles; one past the last is the last again and not stored.
-  const int pairs = ACT == kActNone ? a.NT / 2 : a.half / 2;
-  int pair[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-    pair[h] = ACT == kActNone ? min(u.group * 8 + wave * 2 + h, pairs - 1) : min(u.group * 4 + wave, pairs - 1) + h * pairs;
+  // The wave's tiles are two runs of H: of its columns, or gate and up.  A run
+  // past the last one is the last one again and not stored.
+  constexpr int H = NTW / 2;
+  const int runs = (ACT == kActNone ? a.NT : a.half) / H;
   __amdgpu_buffer_rsrc_t wr[2], sr[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t t = u.e * a.NT + 2 * pair[h];
-    wr[h] = make_rsrc(a.w + t * a.KT * 1024, (uint32_t)a.KT * 2048u);
-    sr[h] = make_rsrc(a.s + t * a.KS * 256, (uint32_t)a.KS * 512u);
+    const int r = ACT == kActNone ? min((u.group * 4 + wave) * 2 + h, runs - 1) : min(u.group * 4 + wave, runs - 1) + h * runs;
+    const int64_t t = u.e * a.NT + (int64_t)r * H;
+    wr[h] = make_rsrc(a.w + t * a.KT * 1024, (uint32_t)(a.KT * H) * 1024u);
+    sr[h] = make_rsrc(a.s + t * a.KS * 256, (uint32_t)(a.KS * H) * 256u);
   }
   struct Weights {
-    u32x4 q[4];
+    u32x4 q[NTW];
   };
   auto load_w = [&](Weights& w, int kt) {
     kt = min(kt, a.KT - 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w.q[j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j >> 1], lane * 16, ((j & 1) * a.KT + kt) * 1024, 0);
+    for (int j = 0; j < NTW; ++j)
+      w.q[j] = __builtin_amdgcn_raw_buffer_load_b128(wr[j / H], lane * 16, (j % H * a.KT + kt) * 1024, 0);
   };
-  auto load_s = [&](uint32_t (&sw)[4], int s) {
+  auto load_s = [&](uint32_t (&sw)[NTW], int s) {
     s = min(s, a.KS - 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sw[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j >> 1], lane * 4, ((j & 1) * a.KS + s) * 256, 0);
+    for (int j = 0; j < NTW; ++j)
+      sw[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j / H], lane * 4, (j % H * a.KS + s) * 256, 0);
   };
   // Stage s's codes of m-tiles m0 .. m1 - 1: wave w brings k-tile w.
   auto dma = [&](int s, int m0, int m1) {
-    u32x4* buf = lds + (s & 1) * kMxStage;
+    u32x4* buf = lds + s % NS * kMxStage;
     const int kt = 4 * s + wave;
     if constexpr (ROWS) {
       const uint32_t dead = kt * 128 + 32 * g < a.K ? 0u : kPastEnd;
@@ -379,71 +382,90 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
         load_lds16(u.xr, buf + (wave * MT + m) * 64, at, (min(m, u.tiles - 1) * a.KT + kt) * 1024);
     }
   };
-  // Their scales: rows 64 w .. 64 w + 63 by wave w.
+  // Their scales: rows 64 w .. 64 w + 63 by waves w and w + 2, both the same.
   auto dma_scales = [&](int s) {
-    if (wave * 64 < MT * 16)
-      load_lds16(u.xsr, lds + (s & 1) * kMxStage + kMxCodes + wave * 64, xsrow | (s < a.KS ? 0u : kPastEnd),
-                 s * (ROWS ? 16 : 256));
+    load_lds16(u.xsr, lds + s % NS * kMxStage + kMxCodes + (wave & 1) * 64, xsrow | (s < a.KS ? 0u : kPastEnd),
+               s * (ROWS ? 16 : 256));
   };
 
-  f32x4 acc[MT][4];
+  f32x4 acc[MT][NTW];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Weights w[4];
-  uint32_t sw[2][4];
+    for (int j = 0; j < NTW; ++j) acc[m][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Weights w[R];
+  uint32_t sw[2][NTW];
   load_s(sw[0], 0);
   dma(0, 0, MT);
   dma_scales(0);
-  __builtin_amdgcn_sched_barrier(0);  // the wait counts the weights' loads behind these
-  load_w(w[0], 0);
-  load_w(w[1], 1);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(8));
+  __builtin_amdgcn_sched_barrier(0);  // the waits count the loads behind a stage's own
+  if constexpr (NS == 3) {
+    dma(1, 0, MT);
+    dma_scales(1);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int k = 0; k < D; ++k) load_w(w[k], k);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(D * NTW + (NS == 3 ? MT : 0)));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 
-  auto step = [&](auto bb, int s, uint32_t (&now)[4], uint32_t (&next)[4], const uint32_t (&sx)[MT]) {
-    constexpr int b = decltype(bb)::value;
+  constexpr int XMAX = NTW == 4 ? 3 : 7, XD = MT < XMAX ? MT : XMAX;  // row operands in registers: all but one ahead
+  u32x4 x[XD];
+  auto step = [&](auto pp, auto bb, int s, uint32_t (&now)[NTW], uint32_t (&next)[NTW], const uint32_t (&sx)[MT]) {
+    constexpr int P = decltype(pp)::value, b = decltype(bb)::value;
     if constexpr (b == 0) {
       load_s(next, s + 1);
-      dma(s + 1, 0, MT / 2);
+      dma(s + NS - 1, 0, MT / 2);
     }
     if constexpr (b == 1) {
-      dma(s + 1, MT / 2, MT);
-      dma_scales(s + 1);
+      dma(s + NS - 1, MT / 2, MT);
+      dma_scales(s + NS - 1);
     }
-    load_w(w[(b + 2) & 3], 4 * s + b + 2);
+    load_w(w[(4 * P + b + D) % R], 4 * s + b + D);
     __builtin_amdgcn_sched_barrier(0);
-    const u32x4* xs = lds + (s & 1) * kMxStage + b * MT * 64 + lane;
+    const u32x4* xs = lds + s % NS * kMxStage + b * MT * 64 + lane;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const u32x4 x = xs[m * 64];
+      // Operand b MT + m of the stage's 4 MT; the first ones are read ahead of the stage's first step.
+      constexpr int ahead = XD - 1;
+      if (b * MT + m + ahead < 4 * MT) x[(b * MT + m + ahead) % XD] = xs[(m + ahead) * 64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[m][j] = mfma_mx4<b, b>(w[b].q[j], x, now[j], sx[m], acc[m][j]);
+      for (int j = 0; j < NTW; ++j)
+        acc[m][j] = mfma_mx4<b, b>(w[(4 * P + b) % R].q[j], x[(b * MT + m) % XD], now[j], sx[m], acc[m][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_barrier(0);
   };
-  auto super = [&](int s, uint32_t (&now)[4], uint32_t (&next)[4]) {
+  auto super = [&](auto pp, int s, uint32_t (&now)[NTW], uint32_t (&next)[NTW]) {
     uint32_t sx[MT];
-    const uint32_t* at = (const uint32_t*)(lds + (s & 1) * kMxStage + kMxCodes) + (ROWS ? c * 4 + g : lane);
+    const u32x4* stage = lds + s % NS * kMxStage;
+    const uint32_t* at = (const uint32_t*)(stage + kMxCodes) + (ROWS ? c * 4 + g : lane);
+#pragma unroll
+    for (int m = 0; m < XD - 1; ++m) x[m] = stage[m * 64 + lane];
 #pragma unroll
     for (int m = 0; m < MT; ++m) sx[m] = at[m * 64];
-    step(std::integral_constant<int, 0>{}, s, now, next, sx);
-    step(std::integral_constant<int, 1>{}, s, now, next, sx);
-    step(std::integral_constant<int, 2>{}, s, now, next, sx);
-    step(std::integral_constant<int, 3>{}, s, now, next, sx);
-    // Stage s + 1 has landed when at most the weights of the last two steps are
-    // outstanding; every wave is done with stage s.
-    __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(8));
+    step(pp, std::integral_constant<int, 0>{}, s, now, next, sx);
+    step(pp, std::integral_constant<int, 1>{}, s, now, next, sx);
+    step(pp, std::integral_constant<int, 2>{}, s, now, next, sx);
+    step(pp, std::integral_constant<int, 3>{}, s, now, next, sx);
+    // Stage s + 1 has landed when at most the loads behind its own are
+    // outstanding: two k-tiles' weights, and with three stages all of this step's
+    // (but for the row scales').  Every wave is done with stage s.
+    __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(2 * NTW + (NS == 3 ? MT + 5 * NTW : 0)));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
   for (int s = 0; s < a.KS; s += 2) {
-    super(s, sw[0], sw[1]);
-    if (s + 1 < a.KS) super(s + 1, sw[1], sw[0]);
+    super(std::integral_constant<int, 0>{}, s, sw[0], sw[1]);
+    if (s + 1 < a.KS) super(std::integral_constant<int, 1>{}, s + 1, sw[1], sw[0]);
   }
 
+  // What was issued past the last stage has landed before LDS is another unit's.
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+
+  // A lane holds 4 H consecutive columns of each run.
+  constexpr int C = 4 * H;
+  typedef E VC __attribute__((ext_vector_type(C)));
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int sid = sids[m * 16 + c];
@@ -452,54 +474,54 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
     E* out = (E*)a.out + (u.row0 + sid) * a.cols;
 #pragma unroll
     for (int h = 0; h < (ACT == kActNone ? 2 : 1); ++h) {
-      const int p = ACT == kActNone ? u.group * 8 + wave * 2 + h : u.group * 4 + wave;
-      const int n = 32 * p + 8 * g;
+      const int t = (ACT == kActNone ? (u.group * 4 + wave) * 2 + h : u.group * 4 + wave) * H;
+      const int n = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
       if (n >= a.cols) continue;  // columns come in multiples of 8
-      float v[2][8];
+      float v[2][C];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[0][i] = acc[m][2 * h + (i >> 2)][i & 3] * rw;
-        if constexpr (ACT != kActNone) v[1][i] = acc[m][2 + (i >> 2)][i & 3] * rw;
+      for (int i = 0; i < C; ++i) {
+        v[0][i] = acc[m][H * h + (i >> 2)][i & 3] * rw;
+        if constexpr (ACT != kActNone) v[1][i] = acc[m][H + (i >> 2)][i & 3] * rw;
       }
       if (a.bias != nullptr) {
 #pragma unroll
         for (int k = 0; k < (ACT == kActNone ? 1 : 2); ++k) {
-          const V8 bias = *(const V8*)((const E*)a.bias + k * a.cols + n);
+          const VC bias = *(const VC*)((const E*)a.bias + k * a.cols + n);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[k][i] += (float)bias[i];
+          for (int i = 0; i < C; ++i) v[k][i] += (float)bias[i];
         }
       }
-      V8 r;
+      VC r;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < C; ++i) {
         if constexpr (ACT == kActNone)
           r[i] = (E)v[0][i];
         else
           r[i] = (E)(gated_act_fast(ACT, v[0][i]) * v[1][i]);
       }
-      *(V8*)(out + n) = r;
+      *(VC*)(out + n) = r;
     }
   }
 }
 
-template <int ACT, bool ROWS, typename DT>
+template <int NTW, int ACT, bool ROWS, typename DT>
 __device__ __forceinline__ void mx4_tile_of(int rows, const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
                                             const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
   switch ((rows + kMxTileGrain - 1) / kMxTileGrain) {
-    case 1: mx4_tile<2, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    case 2: mx4_tile<4, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    case 3: mx4_tile<6, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
-    default: mx4_tile<8, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane);
+    case 1: mx4_tile<2, NTW, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 2: mx4_tile<4, NTW, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    case 3: mx4_tile<6, NTW, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane); break;
+    default: mx4_tile<8, NTW, ACT, ROWS, DT>(a, lds, sids, u, xrow, xsrow, wave, lane);
   }
 }
 
 // Linear layers: unit after unit of (row tile, column group), 8 row tiles by 8
 // groups in turn, so that the workgroups of an XCD (b % 8) share rows and weights
 // in its L2.
-template <int ACT, typename DT>
+template <int NTW, int ACT, typename DT>
 __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(MxArgs a) {
   extern __shared__ u32x4 lds[];
-  int32_t* sids = (int32_t*)(lds + 2 * kMxStage);
+  int32_t* sids = (int32_t*)(lds + mx4_stages(NTW) * kMxStage);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int units = a.slots * a.groups, per_xcd = (units + 7) >> 3;
   // Row tiles of nearly equal height.
@@ -520,19 +542,19 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(MxArgs a) {
     __syncthreads();  // the unit before is done with LDS
     if (threadIdx.x < kMxTileM) sids[threadIdx.x] = threadIdx.x < rows ? threadIdx.x : -1;
     __syncthreads();
-    // 16 bytes of the scales of m-tile 4 wave + lane / 16.
-    const int m = 4 * wave + (lane >> 4);
+    // 16 bytes of the scales of one of four m-tiles.
+    const int m = 4 * (wave & 1) + (lane >> 4);
     const uint32_t xsrow = m < u.tiles ? (uint32_t)m * a.KS * 256u + 16u * (lane & 15) : kPastEnd;
     const uint32_t none[kMxTileM / 16] = {};
-    mx4_tile_of<ACT, false, DT>(rows, a, lds, sids, u, none, xsrow, wave, lane);
+    mx4_tile_of<NTW, ACT, false, DT>(rows, a, lds, sids, u, none, xsrow, wave, lane);
   }
 }
 
 // Experts: unit after unit of (tile of one expert's sorted rows, column group).
-template <int EPL, int ACT, typename DT>
+template <int EPL, int NTW, int ACT, typename DT>
 __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
   extern __shared__ u32x4 lds[];
-  int32_t* sids = (int32_t*)(lds + 2 * kMxStage);
+  int32_t* sids = (int32_t*)(lds + mx4_stages(NTW) * kMxStage);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   RowTiles<EPL> tiles;
   tiles.load(a.offsets, a.E, a.sorted_cap, lane);
@@ -559,18 +581,23 @@ __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
       const int id = sids[16 * m + (lane & 15)];
       xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * (lane >> 4);
     }
-    const int id = wave < 2 ? sids[64 * wave + lane] : -1;
+    const int id = sids[64 * (wave & 1) + lane];
     const uint32_t xsrow = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.KS * 16);
-    mx4_tile_of<ACT, true, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+    mx4_tile_of<NTW, ACT, true, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
   }
 }
 
 template <typename DT, int ACT>
 hipError_t launch_tile(const MxArgs& a, const Mx4Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.grid), block(256);
-  if (a.sorted == nullptr) hipLaunchKernelGGL((mx4_tile_kernel<ACT, DT>), grid, block, kMxTileLds, s, a);
-  else if (a.E <= 128) hipLaunchKernelGGL((mx4_expert_tile_kernel<2, ACT, DT>), grid, block, kMxTileLds, s, a);
-  else hipLaunchKernelGGL((mx4_expert_tile_kernel<8, ACT, DT>), grid, block, kMxTileLds, s, a);
+  if (a.sorted == nullptr && p.ntw == 2)
+    hipLaunchKernelGGL((mx4_tile_kernel<2, ACT, DT>), grid, block, mx4_tile_lds(2), s, a);
+  else if (a.sorted == nullptr)
+    hipLaunchKernelGGL((mx4_tile_kernel<4, ACT, DT>), grid, block, mx4_tile_lds(4), s, a);
+  else if (a.E <= 128)
+    hipLaunchKernelGGL((mx4_expert_tile_kernel<2, 4, ACT, DT>), grid, block, mx4_tile_lds(4), s, a);
+  else
+    hipLaunchKernelGGL((mx4_expert_tile_kernel<8, 4, ACT, DT>), grid, block, mx4_tile_lds(4), s, a);
   return hipGetLastError();
 }
 
@@ -628,7 +655,7 @@ hipError_t launch_experts(const MxArgs& a, const Mx4Plan& p, int act, hipStream_
 }
 
 // Rows up to which a product quantises them itself.
-constexpr int kMxInlineRows = 16;
+constexpr int kMxInlineRows = 8;
 
 // Waves of a workgroup of few rows: as many as leave none without a step, in
 // rounds of equal length.
@@ -644,15 +671,28 @@ int64_t linear_scales(int64_t rows, int64_t K) { return (rows + 15) / 16 * mx4_k
 int64_t expert_codes(int64_t rows, int64_t K) { return rows * K / 2; }  // a multiple of 16
 int64_t expert_scales(int64_t rows, int64_t K) { return rows * mx4_ksteps(K) * 16; }
 
+// Column groups of tiles whose waves hold ntw column tiles.
+int64_t tile_groups(int64_t N, int act, int ntw) {
+  const int64_t cols = act ? N / 2 : N, per = act ? 32 * ntw : 64 * ntw;
+  return (cols + per - 1) / per;
+}
+#ifndef TILE2
+#define TILE2 1
+#endif
+
 }  // namespace
 
 Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   p.pre = M > kMxInlineRows;
-  const int64_t col_groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256), row_tiles = (M + kMxTileM - 1) / kMxTileM;
-  if (M > 64 && row_tiles * col_groups >= device_cu_count()) {
+  const int64_t row_tiles = (M + kMxTileM - 1) / kMxTileM;
+  int64_t col_groups = tile_groups(N, act, 4);
+  const bool wide = row_tiles * col_groups >= device_cu_count();
+  if (M > 64 && (wide || TILE2)) {
     p.tile = true;
+    p.ntw = wide ? 4 : 2;
+    col_groups = tile_groups(N, act, p.ntw);
     p.groups = col_groups;
     p.slots = row_tiles;
     p.grid = std::min<int64_t>((row_tiles * col_groups + 7) / 8 * 8, 2 * device_cu_count() / 8 * 8);
@@ -677,7 +717,8 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   p.ws_bytes = p.pre ? expert_codes(rows, K) + expert_scales(rows, K) : 0;
   if (p.pre) {
     p.tile = true;
-    p.groups = ((act ? N / 2 : N) + (act ? 127 : 255)) / (act ? 128 : 256);
+    p.ntw = 4;
+    p.groups = tile_groups(N, act, 4);
     p.grid = 2 * device_cu_count() / 8 * 8;
     return p;
   }
