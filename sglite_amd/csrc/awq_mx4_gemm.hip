@@ -676,9 +676,6 @@ int64_t tile_groups(int64_t N, int act, int ntw) {
   const int64_t cols = act ? N / 2 : N, per = act ? 32 * ntw : 64 * ntw;
   return (cols + per - 1) / per;
 }
-#ifndef TILE2
-#define TILE2 1
-#endif
 
 }  // namespace
 
@@ -686,12 +683,17 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   p.pre = M > kMxInlineRows;
+  // By tiles where they give half the CUs a workgroup: of 128 columns while all of
+  // them run at once, else of 256 (us, 128-column tiles / 256 / few rows at a time,
+  // with the quantising launch: 128 rows of 2560 x 6144 17.4 / 22.7 / 13.0, of 4096 x
+  // 28672 gated 25 / 31 / 40; 333 rows of 2560 x 19456 gated 27.9 / 23.7 / 49, of
+  // 2560 x 6144 17.6 / 22.6 / 21.3, of 9728 x 2560 31 / 49 / 21.8; 1024 rows of
+  // 4096 x 2560 22 / 30 / 25).
   const int64_t row_tiles = (M + kMxTileM - 1) / kMxTileM;
-  int64_t col_groups = tile_groups(N, act, 4);
-  const bool wide = row_tiles * col_groups >= device_cu_count();
-  if (M > 64 && (wide || TILE2)) {
+  int64_t col_groups = tile_groups(N, act, 2);
+  if (M > 64 && row_tiles * col_groups >= device_cu_count() / 2) {
     p.tile = true;
-    p.ntw = wide ? 4 : 2;
+    p.ntw = row_tiles * col_groups > device_cu_count() ? 4 : 2;
     col_groups = tile_groups(N, act, p.ntw);
     p.groups = col_groups;
     p.slots = row_tiles;

@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from typing import Dict, Iterator, List, NamedTuple, Optional, Sequence, Tuple
 
@@ -1174,14 +1175,15 @@ def _check_mx4(q: Mx4) -> Tuple[int, ...]:
 
 
 def _mx4_quantize_launch(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    x = _aligned(x)
     K, dev = x.shape[-1], x.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _mx4_quantize_launch(x)
+    x = _aligned(x)
     codes = torch.empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8, device=dev)
     scales = torch.empty(x.shape[:-1] + (K // MX4_BLOCK,), dtype=torch.uint8, device=dev)
-    with _on_device(dev):
-        _lib.check(_lib.load().awq_mx4_quantize(x.data_ptr(), _LOGITS_CODE[x.dtype], x.numel() // K, K,
-                                                codes.data_ptr(), scales.data_ptr(), _stream(dev)),
-                   "awq_mx4_quantize")
+    _lib.check(_lib.load().awq_mx4_quantize(x.data_ptr(), _LOGITS_CODE[x.dtype], x.numel() // K, K, codes.data_ptr(),
+                                            scales.data_ptr(), _stream(dev)), "awq_mx4_quantize")
     return codes, scales
 
 
@@ -1215,13 +1217,14 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
 
 
 def _mx4_dequantize_launch(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    codes, scales = _aligned(codes, 4), scales.contiguous()
     K, dev = codes.shape[-1] * 2, codes.device
+    if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _mx4_dequantize_launch(codes, scales, dtype)
+    codes, scales = _aligned(codes, 4), scales.contiguous()
     out = torch.empty(codes.shape[:-1] + (K,), dtype=dtype, device=dev)
-    with _on_device(dev):
-        _lib.check(_lib.load().awq_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), out.numel() // K, K,
-                                                  _LOGITS_CODE[dtype], out.data_ptr(), _stream(dev)),
-                   "awq_mx4_dequantize")
+    _lib.check(_lib.load().awq_mx4_dequantize(codes.data_ptr(), scales.data_ptr(), out.numel() // K, K,
+                                              _LOGITS_CODE[dtype], out.data_ptr(), _stream(dev)), "awq_mx4_dequantize")
     return out
 
 
@@ -1246,6 +1249,7 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return torch.ops.sglite_awq.awq_mx4_dequantize(q.codes, q.scales, dtype)
 
 
+@functools.lru_cache(maxsize=4096)
 def mx4_weight_bytes(N: int, K: int) -> Tuple[int, int]:
     """Bytes of one weight [N, K] and of its scales in the products' layout."""
     w, s = ctypes.c_int64(), ctypes.c_int64()
@@ -1320,6 +1324,11 @@ def mx4_unrepack(weight: Mx4Weight) -> Mx4:
     return Mx4(*torch.ops.sglite_awq.awq_mx4_unrepack(weight.w, weight.s, weight.N, weight.K))
 
 
+@functools.lru_cache(maxsize=4096)
+def _mx4_workspace_bytes(M: int, N: int, K: int, act: int) -> int:
+    return _lib.check(_lib.load().awq_mx4_workspace_bytes(M, N, K, act), "awq_mx4_workspace_bytes")
+
+
 def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
                      out: torch.Tensor, N: int, K: int, act: int) -> None:
     M = x.shape[0]
@@ -1330,7 +1339,7 @@ def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Op
         with torch.cuda.device(dev):
             return _mx4_gemm_launch(x, w, s, bias, out, N, K, act)
     lib = _lib.load()
-    wsb = _lib.check(lib.awq_mx4_workspace_bytes(M, N, K, act), "awq_mx4_workspace_bytes")
+    wsb = _mx4_workspace_bytes(M, N, K, act)
     ws = _workspace(wsb, dev)
     _lib.check(lib.awq_mx4_gemm(x.data_ptr(), w.data_ptr(), s.data_ptr(), _ptr(bias), out.data_ptr(), M, N, K,
                                 dtype_code(x.dtype), act, _ptr(ws), wsb, _stream(dev)), "awq_mx4_gemm")

@@ -62,6 +62,14 @@ def test_bias(M, act):
     check(M, 1280, 1056, torch.float16, act, biased=True)
 
 
+@pytest.mark.parametrize("M,N,K,act", [
+    (2048, 8192, 160, None), (2305, 7432, 672, None), (9000, 2056, 96, None), (2600, 6144, 1024, None),
+    (2500, 8256, 352, "silu"), (4097, 5184, 128, "gelu"), (2048, 8192, 1152, "silu")])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_large(M, N, K, act, dtype):
+    check(M, N, K, dtype, act, biased=True)
+
+
 @pytest.mark.parametrize("M", [1, 16, 17, 64, 200, 1500])
 def test_rows_that_are_not_finite(M):
     x, codes, scales, w = make(M, 96, 352, torch.bfloat16)
