@@ -8,7 +8,8 @@ AWQ is recognised by ``quant_method == "awq"`` or, with no method given, by a
 ``w_bit``/``bits`` key.  The reference then prefers the Marlin method and
 falls back to Triton; here both methods run the same gfx950 kernels, and the
 same preference decides only which config class (and so which shape rules and
-metadata) the model gets.  Remote hub lookups are not performed.
+metadata) the model gets.  Remote hub lookups are not performed.  Beyond the
+reference, ``quant_method == "mxfp4"`` gives the MXFP4 config.
 """
 
 from __future__ import annotations
@@ -48,6 +49,10 @@ def load_quantization_config(model_path: str, hf_config: Optional[Any] = None,
     is_awq = quant_method == "awq" or (not quant_method and ("w_bit" in config_dict or "bits" in config_dict))
     if is_awq:
         return _create_awq_config(config_dict, force_awq_triton)
+    if quant_method == "mxfp4":
+        from .quantization.mxfp4 import MXFP4Config
+
+        return MXFP4Config.from_config(config_dict)
     return None
 
 

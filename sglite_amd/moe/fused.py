@@ -1,4 +1,4 @@
-"""Fused MoE forward with AWQ W4A16 or dense (fp16 / bf16) experts.
+"""Fused MoE forward with AWQ W4A16, MXFP4 or dense (fp16 / bf16) experts.
 
 Follows python/sglite/srt/model_executor/layers/fused_moe/fused.py:
   fused_topk            fused.py:11-31   (topk_softmax + renormalise)
@@ -37,8 +37,8 @@ class AWQMoeWeights(NamedTuple):
         return self.experts.w.shape[0]
 
 
-# An expert stack: repacked AWQ, or dense [E, N, K] as a checkpoint holds it.
-MoeWeights = Union[AWQMoeWeights, torch.Tensor]
+# An expert stack: repacked AWQ, MXFP4 laid out for the products, or dense [E, N, K] as a checkpoint holds it.
+MoeWeights = Union[AWQMoeWeights, ops.Mx4Weight, torch.Tensor]
 
 
 def _expert_dims(w: MoeWeights) -> Tuple[int, int, int]:
@@ -46,6 +46,8 @@ def _expert_dims(w: MoeWeights) -> Tuple[int, int, int]:
     if isinstance(w, torch.Tensor):
         assert w.dim() == 3, "dense expert weights must be [E, N, K]"
         return w.shape[0], w.shape[2], w.shape[1]
+    if isinstance(w, ops.Mx4Weight):
+        return w.num_experts, w.K, w.N
     return w.num_experts, w.input_size, w.output_size
 
 
@@ -56,6 +58,12 @@ def process_awq_moe_weights(qweight: torch.Tensor, qzeros: torch.Tensor, scales:
     E, K, N8 = qweight.shape
     G = K // qzeros.shape[1]
     return AWQMoeWeights(ops.repack_experts(qweight, qzeros, scales), K, N8 * 8, G)
+
+
+def process_mxfp4_moe_weights(weight: torch.Tensor, weight_scale: Optional[torch.Tensor] = None) -> ops.Mx4Weight:
+    """Expert-stacked MXFP4 tensors ``[E, N, K/2]`` and ``[E, N, K/32]`` (uint8), or without scales a 16- or 32-bit
+    stack ``[E, N, K]`` to be quantised, laid out for the products on the device."""
+    return ops.mx4_repack(ops.mx4_quantize(weight) if weight_scale is None else ops.Mx4(weight, weight_scale))
 
 
 def fused_topk(hidden_states: torch.Tensor, gating_output: torch.Tensor, topk: int, renormalize: bool,
@@ -103,8 +111,9 @@ def fused_experts_impl(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeigh
 def _check_experts(hidden_states: torch.Tensor, w1: MoeWeights, w2: MoeWeights, activation: str) -> None:
     if activation not in ("silu", "gelu"):
         raise ValueError(f"unsupported activation {activation!r}")
-    if isinstance(w1, torch.Tensor) != isinstance(w2, torch.Tensor):
-        raise ValueError("w1 and w2 must both be dense or both repacked AWQ experts")
+    for kind in (torch.Tensor, ops.Mx4Weight):
+        if isinstance(w1, kind) != isinstance(w2, kind):
+            raise ValueError("w1 and w2 must both be dense, both MXFP4 or both repacked AWQ experts")
     (E1, K1, N1), (E2, K2, N2) = _expert_dims(w1), _expert_dims(w2)
     assert hidden_states.shape[1] == K1, "Hidden size mismatch"
     assert hidden_states.is_contiguous(), "Hidden_states must be contiguous"
@@ -119,6 +128,9 @@ def _expert_gemm(a: torch.Tensor, w: MoeWeights, align: ops.MoeAlignment, topk_w
     if isinstance(w, torch.Tensor):
         return ops.moe_dense_gemm(a, w, align, topk_weights, num_routed, top_k, activation=activation,
                                   mul_routed_weight=mul_routed_weight)
+    if isinstance(w, ops.Mx4Weight):
+        return ops.mx4_moe_gemm(a, w, align, topk_weights, num_routed, top_k, activation=activation,
+                                mul_routed_weight=mul_routed_weight)
     return ops.moe_gemm(a, w.experts, w.input_size, w.output_size, w.group_size, align, topk_weights, num_routed,
                         top_k, activation=activation, mul_routed_weight=mul_routed_weight)
 
@@ -171,8 +183,9 @@ class AWQFusedMoe(BaseMoeBackend):
     def forward(self, hidden_states: torch.Tensor, w1: AWQMoeWeights, w2: AWQMoeWeights, gating_output: torch.Tensor,
                 topk: int, renormalize: bool, activation: str = "silu",
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
-        if isinstance(w1, torch.Tensor) or isinstance(w2, torch.Tensor):
-            raise ValueError("the awq_fused backend takes repacked AWQ experts; dense ones go to fused")
+        if any(isinstance(w, (torch.Tensor, ops.Mx4Weight)) for w in (w1, w2)):
+            raise ValueError("the awq_fused backend takes repacked AWQ experts; dense ones go to fused, MXFP4 ones to "
+                             "mxfp4_fused")
         return _route_and_run(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
                               apply_router_weight_on_input)
 
@@ -184,6 +197,20 @@ class FusedMoe(BaseMoeBackend):
                 topk: int, renormalize: bool, activation: str = "silu",
                 apply_router_weight_on_input: bool = False) -> torch.Tensor:
         if not (isinstance(w1, torch.Tensor) and isinstance(w2, torch.Tensor)):
-            raise ValueError("the fused backend takes dense expert weights; repacked AWQ ones go to awq_fused")
+            raise ValueError("the fused backend takes dense expert weights; repacked AWQ ones go to awq_fused, MXFP4 "
+                             "ones to mxfp4_fused")
+        return _route_and_run(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
+                              apply_router_weight_on_input)
+
+
+class MXFP4FusedMoe(BaseMoeBackend):
+    """The same backend over MXFP4 experts (``process_mxfp4_moe_weights``); both products quantise their rows."""
+
+    def forward(self, hidden_states: torch.Tensor, w1: ops.Mx4Weight, w2: ops.Mx4Weight, gating_output: torch.Tensor,
+                topk: int, renormalize: bool, activation: str = "silu",
+                apply_router_weight_on_input: bool = False) -> torch.Tensor:
+        if not (isinstance(w1, ops.Mx4Weight) and isinstance(w2, ops.Mx4Weight)):
+            raise ValueError("the mxfp4_fused backend takes MXFP4 experts; dense ones go to fused, repacked AWQ ones to "
+                             "awq_fused")
         return _route_and_run(hidden_states, w1, w2, gating_output, topk, renormalize, activation,
                               apply_router_weight_on_input)

@@ -1,4 +1,4 @@
-"""Mixture-of-experts layers over AWQ expert stacks and over dense experts.
+"""Mixture-of-experts layers over AWQ expert stacks, dense and MXFP4 experts.
 
 ``AWQMoELayer`` is a mirror of ``MoELayer`` (python/sglite/srt/model_executor/layers/moe_layer.py:11-64)
 for AWQ checkpoints:
@@ -27,7 +27,8 @@ for AWQ checkpoints:
 
 ``MoELayer`` is the same block for experts that a checkpoint leaves unquantised:
 its state dict holds gate_up_proj [E, 2I, H] and down_proj [E, H, I], which the
-products read as they are.
+products read as they are.  ``MXFP4MoELayer`` is it for MXFP4 experts, as a
+checkpoint holds them (uint8 codes and scales) or quantised when they are loaded.
 """
 
 from __future__ import annotations
@@ -38,7 +39,8 @@ import torch
 
 from .. import ops
 from ..linear import div_even
-from .fused import AWQFusedMoe, AWQMoeWeights, BaseMoeBackend, FusedMoe, MoeWeights, process_awq_moe_weights
+from .fused import (AWQFusedMoe, AWQMoeWeights, BaseMoeBackend, FusedMoe, MoeWeights, MXFP4FusedMoe,
+                    process_awq_moe_weights, process_mxfp4_moe_weights)
 
 _AWQ_NAMES = ("qweight", "qzeros", "scales")
 
@@ -103,8 +105,8 @@ class _MoEBlock:
 
     # Columns of the gate (and up) projection come in multiples of this.
     _COLUMNS = 16
-    # Of the backends here, the one for the other kind of experts.
-    _NOT_FOR: Type[BaseMoeBackend] = FusedMoe
+    # Of the backends here, those for other kinds of experts.
+    _NOT_FOR: Tuple[Type[BaseMoeBackend], ...] = (FusedMoe, MXFP4FusedMoe)
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int, renormalize: bool,
                  activation: str, apply_router_weight_on_input: bool, tp_size: int, process_group, backend: str):
@@ -194,7 +196,7 @@ class MoELayer(_MoEBlock):
     """Experts of one MoE block with dense weights (MoELayer, moe_layer.py:11-64)."""
 
     _COLUMNS = 8  # rows of the weights are whole 16-byte vectors
-    _NOT_FOR = AWQFusedMoe
+    _NOT_FOR = (AWQFusedMoe, MXFP4FusedMoe)
 
     def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
                  renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,
@@ -239,3 +241,71 @@ class MoELayer(_MoEBlock):
         if self.gate_up_proj.is_meta:
             raise RuntimeError("expert weights are not loaded (call load_state_dict first)")
         return self.gate_up_proj, self.down_proj
+
+
+class MXFP4MoELayer(_MoEBlock):
+    """Experts of one MoE block in MXFP4.
+
+    The state dict holds ``gate_up_proj`` uint8 [E, 2I, H/2], ``gate_up_proj.weight_scale`` uint8 [E, 2I, H/32],
+    ``down_proj`` [E, H, I/2] and ``down_proj.weight_scale`` [E, H, I/32], which is what ingestion yields for a
+    checkpoint's ``experts.<i>.<proj>.weight`` and ``.weight_scale``; with ``serialized`` false a MoELayer's dense
+    stacks in ``params_dtype``, quantised after loading.  Loaded tensors are not kept."""
+
+    _COLUMNS = ops.MX4_BLOCK  # the down projection's blocks
+    _NOT_FOR = (AWQFusedMoe, FusedMoe)
+
+    def __init__(self, num_experts: int, top_k: int, hidden_size: int, intermediate_size: int,
+                 renormalize: bool = True, activation: str = "silu", apply_router_weight_on_input: bool = False,
+                 serialized: bool = True, params_dtype: torch.dtype = torch.float16, tp_size: int = 1,
+                 process_group=None, backend: str = "mxfp4_fused"):
+        super().__init__(num_experts, top_k, hidden_size, intermediate_size, renormalize, activation,
+                         apply_router_weight_on_input, tp_size, process_group, backend)
+        if hidden_size % ops.MX4_BLOCK:
+            raise ValueError(f"the hidden size {hidden_size} must be a multiple of {ops.MX4_BLOCK}")
+        if params_dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            raise ValueError(f"experts are quantised from float16, bfloat16 or float32, got {params_dtype}")
+        self.serialized = serialized
+        local = self.intermediate_size_per_partition
+        # What the state dict must hold.
+        self._params: Dict[str, torch.Tensor] = {}
+        for name, N, K in (("gate_up_proj", 2 * local, hidden_size), ("down_proj", hidden_size, local)):
+            if serialized:
+                self._params[name] = torch.empty((num_experts, N, K // 2), dtype=torch.uint8, device="meta")
+                self._params[name + ".weight_scale"] = torch.empty((num_experts, N, K // ops.MX4_BLOCK),
+                                                                   dtype=torch.uint8, device="meta")
+            else:
+                self._params[name] = torch.empty((num_experts, N, K), dtype=params_dtype, device="meta")
+        self._experts: Optional[Tuple[ops.Mx4Weight, ops.Mx4Weight]] = None
+
+    def state_dict(self, *, prefix: str = "", result: Optional[Dict[str, torch.Tensor]] = None):
+        result = result if result is not None else {}
+        for name, param in self._params.items():
+            result[_concat_prefix(prefix, name)] = param
+        return result
+
+    def state_dict_keys(self, prefix: str = "") -> List[str]:
+        return list(self.state_dict(prefix=prefix).keys())
+
+    def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
+                        _internal: bool = False) -> None:
+        items = {}
+        for name, param in self._params.items():  # check everything before any change
+            key = _concat_prefix(prefix, name)
+            if key not in state_dict:
+                raise KeyError(key)
+            item = state_dict[key]
+            assert isinstance(item, torch.Tensor)
+            assert param.shape == item.shape and param.dtype == item.dtype, (
+                f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
+            items[name] = item
+        for name in self._params:
+            state_dict.pop(_concat_prefix(prefix, name))
+        self._experts = (process_mxfp4_moe_weights(items["gate_up_proj"], items.get("gate_up_proj.weight_scale")),
+                         process_mxfp4_moe_weights(items["down_proj"], items.get("down_proj.weight_scale")))
+        if not _internal and state_dict:
+            raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
+
+    def _expert_weights(self) -> Tuple[MoeWeights, MoeWeights]:
+        if self._experts is None:
+            raise RuntimeError("expert weights are not loaded (call load_state_dict first)")
+        return self._experts

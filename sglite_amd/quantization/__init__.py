@@ -2,8 +2,9 @@
 
 Same exports and lazy-import behaviour as
 python/sglite/srt/model_executor/layers/quantization/__init__.py:10-55: the
-base types import eagerly; the AWQ methods, which load the HIP library, import
-on first use.  Both method names ("awq", "awq_marlin") run the same kernels.
+base types import eagerly; the methods that load the HIP library import on
+first use.  Both AWQ method names ("awq", "awq_marlin") run the same kernels;
+"mxfp4" has no counterpart in the reference.
 """
 
 from .base_config import LinearMethodBase, QuantizationConfig, set_weight_attrs
@@ -21,7 +22,11 @@ def get_quantization_config(method_name: str) -> type:
         from .awq_marlin import AWQMarlinConfig
 
         return AWQMarlinConfig
-    raise ValueError(f"Unknown quantization method: {method_name!r}. Supported methods: ['awq', 'awq_marlin']")
+    if method_name == "mxfp4":
+        from .mxfp4 import MXFP4Config
+
+        return MXFP4Config
+    raise ValueError(f"Unknown quantization method: {method_name!r}. Supported methods: ['awq', 'awq_marlin', 'mxfp4']")
 
 
 def __getattr__(name: str):
@@ -33,6 +38,10 @@ def __getattr__(name: str):
         from . import awq_marlin
 
         return getattr(awq_marlin, name)
+    if name in ("MXFP4Config", "MXFP4LinearMethod"):
+        from . import mxfp4
+
+        return getattr(mxfp4, name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
@@ -42,6 +51,8 @@ __all__ = [
     "AWQMarlinConfig",
     "AWQMarlinLinearMethod",
     "LinearMethodBase",
+    "MXFP4Config",
+    "MXFP4LinearMethod",
     "QuantizationConfig",
     "UnquantizedLinearMethod",
     "set_weight_attrs",
