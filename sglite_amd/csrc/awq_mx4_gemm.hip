@@ -550,41 +550,44 @@ __global__ __launch_bounds__(256, 2) void mx4_tile_kernel(MxArgs a) {
   }
 }
 
-// Experts: unit after unit of (tile of one expert's sorted rows, column group).
+// Experts: a workgroup is one (tile of one expert's sorted rows, column group) of
+// those that there are; the grid covers as many as there can be.  Each XCD (b % 8)
+// takes a run of consecutive ones, so that the tiles that read one expert's
+// weights share an L2.
 template <int EPL, int NTW, int ACT, typename DT>
 __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
   extern __shared__ u32x4 lds[];
   int32_t* sids = (int32_t*)(lds + mx4_stages(NTW) * kMxStage);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  RowTiles<EPL> tiles;
-  tiles.load(a.offsets, a.E, a.sorted_cap, lane);
-  tiles.scan(kMxTileM, lane);
   MxUnit u;
+  int e, rb, rows;
+  {
+    RowTiles<EPL> tiles;
+    tiles.load(a.offsets, a.E, a.sorted_cap, lane);
+    tiles.scan(kMxTileM, lane);
+    const int per_xcd = (tiles.total() * a.groups + 7) >> 3, at = blockIdx.x >> 3;
+    if (at >= per_xcd) return;
+    tiles.find_unit((blockIdx.x & 7) * per_xcd + at, a.groups, kMxTileM, kMxTileGrain, lane, e, rb, rows, u.group);
+    if (e < 0) return;  // the same in every wave
+  }
+  int sid = -1;
+  if (threadIdx.x < kMxTileM && (int)threadIdx.x < rows) sid = a.sorted[rb + threadIdx.x];
+  if (sid >= a.num_routed) sid = -1;
+  if (threadIdx.x < kMxTileM) sids[threadIdx.x] = sid;
+  if (!__syncthreads_or(sid >= 0)) return;  // padding alone
+  u.e = e;
   u.row0 = 0;
   u.xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)(a.K / 2));
   u.xsr = make_rsrc(a.xs, (uint32_t)a.M * (uint32_t)a.KS * 16u);
-  const int per_xcd = (tiles.total() * a.groups + 7) >> 3;
-  for (int at = blockIdx.x >> 3; at < per_xcd; at += gridDim.x >> 3) {
-    int e, rb, rows;
-    tiles.find_unit((blockIdx.x & 7) * per_xcd + at, a.groups, kMxTileM, kMxTileGrain, lane, e, rb, rows, u.group);
-    if (e < 0) break;  // the same in every wave
-    u.e = e;
-    int sid = -1;
-    if (threadIdx.x < kMxTileM && (int)threadIdx.x < rows) sid = a.sorted[rb + threadIdx.x];
-    if (sid >= a.num_routed) sid = -1;
-    __syncthreads();  // the unit before is done with LDS
-    if (threadIdx.x < kMxTileM) sids[threadIdx.x] = sid;
-    if (!__syncthreads_or(sid >= 0)) continue;  // padding alone
-    uint32_t xrow[kMxTileM / 16];
+  uint32_t xrow[kMxTileM / 16];
 #pragma unroll
-    for (int m = 0; m < kMxTileM / 16; ++m) {
-      const int id = sids[16 * m + (lane & 15)];
-      xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * (lane >> 4);
-    }
-    const int id = sids[64 * (wave & 1) + lane];
-    const uint32_t xsrow = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.KS * 16);
-    mx4_tile_of<NTW, ACT, true, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
+  for (int m = 0; m < kMxTileM / 16; ++m) {
+    const int id = sids[16 * m + (lane & 15)];
+    xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * (lane >> 4);
   }
+  const int id = sids[64 * (wave & 1) + lane];
+  const uint32_t xsrow = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.KS * 16);
+  mx4_tile_of<NTW, ACT, true, DT>(rows, a, lds, sids, u, xrow, xsrow, wave, lane);
 }
 
 template <typename DT, int ACT>
@@ -721,7 +724,8 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
     p.tile = true;
     p.ntw = 4;
     p.groups = tile_groups(N, act, 4);
-    p.grid = 2 * device_cu_count() / 8 * 8;
+    // Of the sorted rows, padding included, each expert has one tile more than its full ones at most.
+    p.grid = ((num_routed + 15 * std::min(num_routed, E)) / kMxTileM + std::min(num_routed, E)) * p.groups / 8 * 8 + 8;
     return p;
   }
   p.mt = 1;
