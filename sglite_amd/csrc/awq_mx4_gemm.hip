@@ -330,9 +330,11 @@ struct MxUnit {
   int tiles;    // m-tiles (linear)
 };
 
-// ROWS: the codes row by row (xrow: offsets of the lane's rows, from its block of
-// the wave's k-tile); else in the weights' layout.  xsrow: the lane's 16 bytes of
-// the wave's scales.
+// ROWS: the codes row by row; a DMA brings 256 bytes of each of four rows (xrow:
+// offsets of the lane's rows, with its 16 bytes), block j of row r lands in place
+// j ^ (r % 16) of the row's 256 bytes of LDS, and the operand reads of 16 rows meet
+// all banks.  Else in the weights' layout.  xsrow: the lane's 16 bytes of the
+// wave's scales.
 template <int MT, int NTW, int ACT, bool ROWS, typename DT>
 __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int32_t* sids, const MxUnit& u,
                                          const uint32_t (&xrow)[kMxTileM / 16], uint32_t xsrow, int wave, int lane) {
@@ -367,14 +369,15 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
     for (int j = 0; j < NTW; ++j)
       sw[j] = __builtin_amdgcn_raw_buffer_load_b32(sr[j / H], lane * 4, (j % H * a.KS + s) * 256, 0);
   };
-  // Stage s's codes of m-tiles m0 .. m1 - 1: wave w brings k-tile w.
+  // Stage s's codes of m-tiles m0 .. m1 - 1: of each, wave w brings rows 4 w .. 4 w + 3,
+  // or k-tile w.
   auto dma = [&](int s, int m0, int m1) {
     u32x4* buf = lds + s % NS * kMxStage;
     const int kt = 4 * s + wave;
     if constexpr (ROWS) {
-      const uint32_t dead = kt * 128 + 32 * g < a.K ? 0u : kPastEnd;
+      const uint32_t dead = s * 512 + 32 * (c ^ (4 * wave + g)) < a.K ? 0u : kPastEnd;
 #pragma unroll
-      for (int m = m0; m < m1; ++m) load_lds16(u.xr, buf + (wave * MT + m) * 64, xrow[m] | dead, kt * 64);
+      for (int m = m0; m < m1; ++m) load_lds16(u.xr, buf + (4 * m + wave) * 64, xrow[m] | dead, s * 256);
     } else {
       const uint32_t at = lane * 16u | (kt < a.KT ? 0u : kPastEnd);
 #pragma unroll
@@ -412,10 +415,15 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
 
   constexpr int XMAX = NTW == 4 ? 3 : 7, XD = MT < XMAX ? MT : XMAX;  // row operands in registers: all but one ahead
   u32x4 x[XD];
-  auto step = [&](auto pp, auto bb, int s, uint32_t (&now)[NTW], uint32_t (&next)[NTW], const uint32_t (&sx)[MT]) {
+  // Where the lane's operand of k-tile b and m-tile m lies in a stage.
+  int xat[4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) xat[b] = ROWS ? c * 16 + ((4 * b + g) ^ c) : b * MT * 64 + lane;
+  constexpr int kRowTile = ROWS ? 256 : 64;
+  auto step = [&](auto pp, auto bb, int s, uint32_t (&now)[NTW], uint32_t (&later)[NTW], const uint32_t (&sx)[MT]) {
     constexpr int P = decltype(pp)::value, b = decltype(bb)::value;
     if constexpr (b == 0) {
-      load_s(next, s + 1);
+      load_s(later, s + 1);
       dma(s + NS - 1, 0, MT / 2);
     }
     if constexpr (b == 1) {
@@ -424,30 +432,30 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
     }
     load_w(w[(4 * P + b + D) % R], 4 * s + b + D);
     __builtin_amdgcn_sched_barrier(0);
-    const u32x4* xs = lds + s % NS * kMxStage + b * MT * 64 + lane;
+    const u32x4* xs = lds + s % NS * kMxStage;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       // Operand b MT + m of the stage's 4 MT; the first ones are read ahead of the stage's first step.
-      constexpr int ahead = XD - 1;
-      if (b * MT + m + ahead < 4 * MT) x[(b * MT + m + ahead) % XD] = xs[(m + ahead) * 64];
+      const int next = b * MT + m + XD - 1;
+      if (next < 4 * MT) x[next % XD] = xs[xat[next / MT] + next % MT * kRowTile];
 #pragma unroll
       for (int j = 0; j < NTW; ++j)
         acc[m][j] = mfma_mx4<b, b>(w[(4 * P + b) % R].q[j], x[(b * MT + m) % XD], now[j], sx[m], acc[m][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto super = [&](auto pp, int s, uint32_t (&now)[NTW], uint32_t (&next)[NTW]) {
+  auto super = [&](auto pp, int s, uint32_t (&now)[NTW], uint32_t (&later)[NTW]) {
     uint32_t sx[MT];
     const u32x4* stage = lds + s % NS * kMxStage;
     const uint32_t* at = (const uint32_t*)(stage + kMxCodes) + (ROWS ? c * 4 + g : lane);
 #pragma unroll
-    for (int m = 0; m < XD - 1; ++m) x[m] = stage[m * 64 + lane];
+    for (int m = 0; m < XD - 1; ++m) x[m] = stage[xat[0] + m * kRowTile];
 #pragma unroll
     for (int m = 0; m < MT; ++m) sx[m] = at[m * 64];
-    step(pp, std::integral_constant<int, 0>{}, s, now, next, sx);
-    step(pp, std::integral_constant<int, 1>{}, s, now, next, sx);
-    step(pp, std::integral_constant<int, 2>{}, s, now, next, sx);
-    step(pp, std::integral_constant<int, 3>{}, s, now, next, sx);
+    step(pp, std::integral_constant<int, 0>{}, s, now, later, sx);
+    step(pp, std::integral_constant<int, 1>{}, s, now, later, sx);
+    step(pp, std::integral_constant<int, 2>{}, s, now, later, sx);
+    step(pp, std::integral_constant<int, 3>{}, s, now, later, sx);
     // Stage s + 1 has landed when at most the loads behind its own are
     // outstanding: two k-tiles' weights, and with three stages all of this step's
     // (but for the row scales').  Every wave is done with stage s.
@@ -582,8 +590,8 @@ __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
   uint32_t xrow[kMxTileM / 16];
 #pragma unroll
   for (int m = 0; m < kMxTileM / 16; ++m) {
-    const int id = sids[16 * m + (lane & 15)];
-    xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * (lane >> 4);
+    const int r = 4 * wave + (lane >> 4), id = sids[16 * m + r];
+    xrow[m] = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.K / 2) + 16u * ((lane & 15) ^ r);
   }
   const int id = sids[64 * (wave & 1) + lane];
   const uint32_t xsrow = id < 0 ? kPastEnd : (uint32_t)(id / a.a_div) * (uint32_t)(a.KS * 16);
