@@ -225,29 +225,22 @@ struct RowsBody {
     }
     return v;
   }
-  // m-tile mt's outputs of row `row` of out: the lane's 4 columns of each tile.
-  __device__ __forceinline__ void store(const f32x4* red, int mt, int64_t row, int group, float rw) const {
-    const int g = lane >> 4;
-    E* out = (E*)a.out + row * a.cols;
+  // The lane's 4 columns of m-tile mt and output tile j, row `row` of out.
+  static constexpr int kOutTiles = ACT != kActNone ? NTW / 2 : NTW;
+  __device__ __forceinline__ void store(const f32x4* red, int mt, int j, int64_t row, int group, float rw) const {
+    const int t = group * kOutTiles + j, n = 32 * (t >> 1) + 8 * (lane >> 4) + 4 * (t & 1);
+    if (n >= a.cols) return;  // N is a multiple of 8
+    const f32x4 v = biased(sum(red, mt, j), n, rw);
+    V4 r;
     if constexpr (ACT != kActNone) {
-      const int n = 32 * (group >> 1) + 8 * g + 4 * (group & 1);
-      const f32x4 gate = biased(sum(red, mt, 0), n, rw), up = biased(sum(red, mt, 1), a.cols + n, rw);
-      V4 r;
+      const f32x4 up = biased(sum(red, mt, j + kOutTiles), a.cols + n, rw);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = (E)(gated_act(ACT, gate[i]) * up[i]);
-      *(V4*)(out + n) = r;
+      for (int i = 0; i < 4; ++i) r[i] = (E)(gated_act(ACT, v[i]) * up[i]);
     } else {
-      const int t = group * NTW, n = 32 * (t >> 1) + 8 * g + 4 * (t & 1);
-      if (n >= a.cols) return;  // N is a multiple of 8
 #pragma unroll
-      for (int j = 0; j < NTW; ++j) {
-        const f32x4 v = biased(sum(red, mt, j), n + 4 * j, rw);
-        V4 r;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (E)v[i];
-        *(V4*)(out + n + 4 * j) = r;
-      }
+      for (int i = 0; i < 4; ++i) r[i] = (E)v[i];
     }
+    *(V4*)((E*)a.out + row * a.cols + n) = r;
   }
 };
 
@@ -273,9 +266,9 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_rows_kernel(MxArgs a) {
   }
   b.run(red);
   __syncthreads();
-  for (int mt = b.wave; mt < MT; mt += b.waves) {
-    const int r = 16 * mt + (b.lane & 15);
-    if (r < b.rows) b.store(red, mt, m0 + r, group, 1.f);
+  for (int i = b.wave; i < MT * b.kOutTiles; i += b.waves) {
+    const int mt = i / b.kOutTiles, r = 16 * mt + (b.lane & 15);
+    if (r < b.rows) b.store(red, mt, i - mt * b.kOutTiles, m0 + r, group, 1.f);
   }
 }
 
@@ -303,7 +296,9 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxAr
     b.set_tiles(e, group);
     b.run(red);
     __syncthreads();
-    if (b.wave == 0 && sid >= 0) b.store(red, 0, sid, group, a.topk_w != nullptr ? a.topk_w[sid] : 1.f);
+    if (sid >= 0)
+      for (int j = b.wave; j < b.kOutTiles; j += b.waves)
+        b.store(red, 0, j, sid, group, a.topk_w != nullptr ? a.topk_w[sid] : 1.f);
     __syncthreads();  // before the next tile's partial sums
   }
 }
@@ -726,7 +721,11 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   const int64_t rows = (num_routed + top_k - 1) / top_k;
-  p.pre = num_routed > 4 * E;
+  // From three rows an expert the tiles are ahead, although they quantise in a
+  // launch of their own (us of both products, row by row / by tiles: E = 128, H =
+  // 2048, I = 768 top-8 at 24 tokens 64 / 66, 32 70 / 75, 48 78 / 77, 96 87 / 82; E =
+  // 16, H = 4096, I = 1408 top-2 at 8 tokens 31 / 37, at 24 45 / 42).
+  p.pre = num_routed > 2 * E;
   p.ws_bytes = p.pre ? expert_codes(rows, K) + expert_scales(rows, K) : 0;
   if (p.pre) {
     p.tile = true;
