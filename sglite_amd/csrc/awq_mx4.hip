@@ -127,8 +127,8 @@ __global__ __launch_bounds__(kMxThreads) void mx4_dequantize_kernel(const uint32
   V4 r[2];
 #pragma unroll
   for (int j = 0; j < 8; ++j) r[j >> 2][j & 3] = (E)(mx4_value(c >> (4 * j)) * s);
-  ((V4*)out)[2 * i] = r[0];
-  ((V4*)out)[2 * i + 1] = r[1];
+  __builtin_nontemporal_store(r[0], (V4*)out + 2 * i);
+  __builtin_nontemporal_store(r[1], (V4*)out + 2 * i + 1);
 }
 
 // Column of MFMA row i of tile t.

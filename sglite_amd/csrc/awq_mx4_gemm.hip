@@ -315,7 +315,7 @@ constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 by
 // NTW = 4: two stages, weights two k-tiles ahead, two workgroups a CU.  NTW = 2,
 // for grids that leave CUs idle: three stages and weights six k-tiles ahead.
 constexpr int mx4_stages(int ntw) { return ntw == 4 ? 2 : 3; }
-constexpr int mx4_tile_lds(int ntw) { return (mx4_stages(ntw) * kMxStage + kMxTileM / 4) * 16; }  // and the row ids
+constexpr int mx4_tile_lds(int ntw) { return (mx4_stages(ntw) * kMxStage + kMxTileM / 2) * 16; }  // row ids, routed weights
 
 struct MxUnit {
   __amdgpu_buffer_rsrc_t xr, xsr;
@@ -469,11 +469,12 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
   // A lane holds 4 H consecutive columns of each run.
   constexpr int C = 4 * H;
   typedef E VC __attribute__((ext_vector_type(C)));
+  const float* rws = (const float*)(sids + kMxTileM);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const int sid = sids[m * 16 + c];
     if (sid < 0) continue;
-    const float rw = a.topk_w != nullptr ? a.topk_w[sid] : 1.f;
+    const float rw = a.topk_w != nullptr ? rws[m * 16 + c] : 1.f;
     E* out = (E*)a.out + (u.row0 + sid) * a.cols;
 #pragma unroll
     for (int h = 0; h < (ACT == kActNone ? 2 : 1); ++h) {
@@ -576,7 +577,10 @@ __global__ __launch_bounds__(256, 2) void mx4_expert_tile_kernel(MxArgs a) {
   int sid = -1;
   if (threadIdx.x < kMxTileM && (int)threadIdx.x < rows) sid = a.sorted[rb + threadIdx.x];
   if (sid >= a.num_routed) sid = -1;
-  if (threadIdx.x < kMxTileM) sids[threadIdx.x] = sid;
+  if (threadIdx.x < kMxTileM) {
+    sids[threadIdx.x] = sid;
+    if (a.topk_w != nullptr && sid >= 0) ((float*)sids)[kMxTileM + threadIdx.x] = a.topk_w[sid];
+  }
   if (!__syncthreads_or(sid >= 0)) return;  // padding alone
   u.e = e;
   u.row0 = 0;
