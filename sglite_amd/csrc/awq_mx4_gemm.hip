@@ -427,6 +427,7 @@ __device__ __forceinline__ void mx4_tile(const MxArgs& a, u32x4* lds, const int3
     }
     load_w(w[(4 * P + b + D) % R], 4 * s + b + D);
     __builtin_amdgcn_sched_barrier(0);
+    if (b > 0 && ROWS && 4 * s + b >= a.KT) return;  // past K
     const u32x4* xs = lds + s % NS * kMxStage;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
