@@ -869,7 +869,9 @@ int check_mx4_weight(int64_t N, int64_t K, int activation, const char* who) {
 }
 
 int check_mx4_workspace(const Mx4Plan& p, const void* ws, int64_t ws_bytes, const char* who) {
-  if (p.grid > kMx4MaxGrid) return fail(AWQ_STATUS_UNSUPPORTED, "%s: too many rows and columns for one launch", who);
+  // Linear tiles are counted in 32 bits and taken in turn by fewer workgroups.
+  if (p.grid > kMx4MaxGrid || p.slots * p.groups >= (int64_t(1) << 30))
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: too many rows and columns for one launch", who);
   if (p.ws_bytes == 0) return AWQ_STATUS_OK;
   if (!ws || ws_bytes < p.ws_bytes)
     return fail(AWQ_STATUS_WORKSPACE, "%s: workspace of %lld bytes needed, %lld given", who, (long long)p.ws_bytes,
@@ -1026,7 +1028,7 @@ int64_t awq_mx4_moe_workspace_bytes(int64_t num_routed, int64_t top_k, int64_t E
   const int st = check_mx4_moe(num_routed, top_k, E, N, K, activation, "awq_mx4_moe_workspace_bytes");
   if (st != 0) return st;
   ok();
-  return num_routed == 0 ? 0 : plan_mx4_moe(num_routed, top_k, E, N, K, activation).ws_bytes;
+  return num_routed == 0 ? 0 : plan_mx4_moe(num_routed, top_k, E, N, K, activation, 0).ws_bytes;
 }
 
 int awq_mx4_moe_gemm(const void* a, int64_t a_rows, const void* w, const void* s, int64_t E, int64_t N, int64_t K,
@@ -1050,7 +1052,7 @@ int awq_mx4_moe_gemm(const void* a, int64_t a_rows, const void* w, const void* s
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_moe_gemm: null pointer argument");
   if (!aligned(a, 16) || !aligned(w, 16) || !aligned(s, 4) || !aligned(out, 16))
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_moe_gemm: a, w and out must be 16-byte and s 4-byte aligned");
-  const Mx4Plan plan = plan_mx4_moe(num_routed, top_k, E, N, K, activation);
+  const Mx4Plan plan = plan_mx4_moe(num_routed, top_k, E, N, K, activation, sorted_cap);
   st = check_mx4_workspace(plan, ws, ws_bytes, "awq_mx4_moe_gemm");
   if (st != 0) return st;
   Mx4Params p{};

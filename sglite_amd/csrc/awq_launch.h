@@ -195,7 +195,8 @@ struct Mx4Plan {
   int64_t grid, ws_bytes;
 };
 Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act);
-Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act);
+// sorted_cap: rows of the sorted table, for the grid.
+Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act, int64_t sorted_cap);
 struct Mx4Params {
   const void* x;
   const void* w;

@@ -722,7 +722,7 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   return p;
 }
 
-Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act) {
+Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K, int act, int64_t sorted_cap) {
   Mx4Plan p{};
   const int64_t tiles = mx4_tiles(N);
   const int64_t rows = (num_routed + top_k - 1) / top_k;
@@ -737,7 +737,7 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
     p.ntw = 4;
     p.groups = tile_groups(N, act, 4);
     // Of the sorted rows, padding included, each expert has one tile more than its full ones at most.
-    p.grid = ((num_routed + 15 * std::min(num_routed, E)) / kMxTileM + std::min(num_routed, E)) * p.groups / 8 * 8 + 8;
+    p.grid = (sorted_cap / kMxTileM + std::min(num_routed, E)) * p.groups / 8 * 8 + 8;
     return p;
   }
   p.mt = 1;

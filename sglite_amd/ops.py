@@ -1249,9 +1249,14 @@ def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     return torch.ops.sglite_awq.awq_mx4_dequantize(q.codes, q.scales, dtype)
 
 
-@functools.lru_cache(maxsize=4096)
+def _mx4_layout_bytes(N: int, K: int) -> Tuple[int, int]:
+    """awq_mx4_weight_bytes, of sizes that it takes."""
+    tiles = (N + 31) // 32 * 2
+    return tiles * ((K + 127) // 128) * 1024, tiles * ((K + 511) // 512) * 256
+
+
 def mx4_weight_bytes(N: int, K: int) -> Tuple[int, int]:
-    """Bytes of one weight [N, K] and of its scales in the products' layout."""
+    """Bytes of one weight [N, K] and of its scales in the products' layout; sizes that they cannot take are refused."""
     w, s = ctypes.c_int64(), ctypes.c_int64()
     _lib.check(_lib.load().awq_mx4_weight_bytes(N, K, ctypes.byref(w), ctypes.byref(s)), "awq_mx4_weight_bytes")
     return w.value, s.value
@@ -1272,7 +1277,7 @@ def _mx4_repack_op(codes: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Ten
 
 @_mx4_repack_op.register_fake
 def _(codes, scales):
-    wb, sb = mx4_weight_bytes(codes.shape[-2], codes.shape[-1] * 2)
+    wb, sb = _mx4_layout_bytes(codes.shape[-2], codes.shape[-1] * 2)
     return codes.new_empty(codes.shape[:-2] + (wb,)), codes.new_empty(codes.shape[:-2] + (sb,))
 
 
@@ -1308,7 +1313,7 @@ def _check_mx4_weight(weight: Mx4Weight, dims: int) -> None:
     if weight.w.dim() != dims or weight.s.dim() != dims or weight.w.shape[:-1] != weight.s.shape[:-1]:
         raise ValueError("the weight must be " + ("one linear's [N, K]" if dims == 1 else "a stack of experts' [E, N, K]")
                          + " from mx4_repack")
-    if (weight.w.shape[-1], weight.s.shape[-1]) != mx4_weight_bytes(weight.N, weight.K):
+    if (weight.w.shape[-1], weight.s.shape[-1]) != _mx4_layout_bytes(weight.N, weight.K):
         raise ValueError(f"the weight does not hold [{weight.N}, {weight.K}]")
     for t in weight[:2]:
         if t.dtype != torch.uint8 or not t.is_contiguous() or t.data_ptr() % 16:
@@ -1349,8 +1354,9 @@ def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Op
 def _mx4_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor], N: int, K: int,
                  activation: str) -> torch.Tensor:
     act = _ACT_CODE[_ACT_NAME[activation]]
+    _check_mx4_product(x, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 1)
     out = torch.empty((x.shape[0], N // 2 if act else N), dtype=x.dtype, device=x.device)
-    _mx4_gemm_launch(x, w, s, bias, out, N, K, act)
+    _mx4_gemm_launch(_aligned(x), w, s, bias, out, N, K, act)
     return out
 
 
@@ -1362,7 +1368,8 @@ def _(x, w, s, bias, N, K, activation):
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_gemm_out", mutates_args=("out",), device_types="cuda")
 def _mx4_gemm_out_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
                      out: torch.Tensor, N: int, K: int, activation: str) -> None:
-    _mx4_gemm_launch(x, w, s, bias, out, N, K, _ACT_CODE[_ACT_NAME[activation]])
+    _check_mx4_product(x, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 1)
+    _mx4_gemm_launch(_aligned(x), w, s, bias, out, N, K, _ACT_CODE[_ACT_NAME[activation]])
 
 
 @_mx4_gemm_out_op.register_fake
@@ -1444,7 +1451,8 @@ def _mx4_moe_launch(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_id
 def _mx4_moe_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_ids: torch.Tensor,
                 expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, N: int, K: int,
                 num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> None:
-    _mx4_moe_launch(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k,
+    _check_mx4_product(a, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 2)
+    _mx4_moe_launch(_aligned(a), w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k,
                     _ACT_CODE[_ACT_NAME[activation]], mul_routed_weight)
 
 

@@ -156,6 +156,72 @@ def test_two_streams_at_once():
         assert all(torch.equal(w, y) for y in ys)
 
 
+def test_threads_on_one_stream():
+    """The quantised rows of a call lie in its thread's own workspace."""
+    import threading
+
+    pairs = [make(300, 640, 1024, torch.float16, seed) for seed in range(4)]
+    want, bad = [ops.mx4_gemm(p[0], p[3]) for p in pairs], []
+
+    def work(i):
+        for _ in range(30):
+            y = ops.mx4_gemm(pairs[i][0], pairs[i][3])
+        torch.cuda.synchronize()
+        if not torch.equal(y, want[i]):
+            bad.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_offsets_past_31_bits():
+    """A weight of more than 2 GiB, and an output of more than 2^32 bytes."""
+    N, K = 65536, 69632
+    g = torch.Generator(device=DEV).manual_seed(0)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.randint(118, 122, (N, K // 32), generator=g, device=DEV, dtype=torch.uint8)
+    w = ops.mx4_repack(ops.Mx4(codes, scales))
+    cols = torch.tensor([0, 77, 40000, N - 1], device=DEV)
+    values = oracle.values(codes[cols], scales[cols])
+    back = ops.mx4_unrepack(w)
+    assert torch.equal(back.codes[cols], codes[cols]) and torch.equal(back.scales[cols], scales[cols])
+    del back, codes
+    for M in (2, 70, 300):
+        x = torch.randn((M, K), generator=g, device=DEV).bfloat16()
+        close(ops.mx4_gemm(x, w)[:, cols], *oracle.product(oracle.quantized(x), values))
+    del w
+    M, N, K = 70000, 32768, 64
+    x = torch.randn((M, K), generator=g, device=DEV).half()
+    q = ops.mx4_quantize(torch.randn((N, K), generator=g, device=DEV))
+    y = ops.mx4_gemm(x, ops.mx4_repack(q))
+    rows = torch.tensor([0, 1, 40001, 65535, 65536, M - 1], device=DEV)
+    close(y[rows], *oracle.product(oracle.quantized(x[rows]), oracle.values(*q)))
+
+
+def test_compiled():
+    x, codes, scales, w = make(20, 128, 96, torch.bfloat16)
+
+    def op(v):
+        return torch.ops.sglite_awq.awq_mx4_gemm(v, w.w, w.s, None, 128, 96, "none") * 2.0
+    assert torch.equal(torch.compile(op, backend="aot_eager", fullgraph=True)(x), ops.mx4_gemm(x, w) * 2.0)
+    assert torch.equal(torch.compile(lambda v: ops.mx4_gemm(v, w) * 2.0, backend="aot_eager")(x), ops.mx4_gemm(x, w) * 2.0)
+
+
+def test_ops_called_by_themselves_check_too():
+    x, codes, scales, w = make(20, 128, 96, torch.bfloat16)
+    op = torch.ops.sglite_awq.awq_mx4_gemm
+    wide = torch.zeros((20, 200), dtype=torch.bfloat16, device=DEV)
+    wide[:, 8:104] = x
+    assert torch.equal(op(wide[:, 8:104], w.w, w.s, None, 128, 96, "none"), ops.mx4_gemm(x, w))
+    for bad in ((x[:, :64], w.w, w.s, None, 128, 96, "none"), (x, w.w[:-16], w.s, None, 128, 96, "none"),
+                (x, w.w, w.s, None, 160, 96, "none"), (x.float(), w.w, w.s, None, 128, 96, "none")):
+        with pytest.raises(ValueError):
+            op(*bad)
+
+
 def test_registered_ops_meet_the_direct_calls():
     x, codes, scales, w = make(20, 128, 96, torch.bfloat16)
     y = torch.ops.sglite_awq.awq_mx4_gemm(x, w.w, w.s, None, 128, 96, "silu")

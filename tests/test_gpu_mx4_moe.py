@@ -77,6 +77,41 @@ def test_ids_outside_the_experts_leave_their_rows(T):
     assert (out == 7).all()
 
 
+@pytest.mark.parametrize("T", [3, 250])
+@pytest.mark.parametrize("block", [16, 64, 128])
+def test_rows_aligned_to_larger_blocks(T, block):
+    E, k = 9, 2
+    a, codes, scales, w = make(T, 96, 160, torch.bfloat16, E=E)
+    ids, tw = route(T, E, k, "skewed")
+    got = ops.mx4_moe_gemm(a, w, ops.moe_align_block_size(ids, block, E), tw, T * k, k, mul_routed_weight=True)
+    close(got, *formula(a, codes, scales, ids, k, tw, None))
+
+
+@pytest.mark.parametrize("T", [2, 90])
+def test_a_token_that_names_an_expert_twice(T):
+    a, codes, scales, w = make(T, 64, 96, torch.float16, E=5)
+    ids, tw = route(T, 5, 3)
+    ids[:, 2] = ids[:, 0]
+    got = ops.mx4_moe_gemm(a, w, ops.moe_align_block_size(ids, 16, 5), tw, 3 * T, 3, "silu")
+    close(got, *formula(a, codes, scales, ids, 3, None, "silu"))
+
+
+def test_stacks_past_31_bits():
+    E, N, K = 9, 16384, 30720
+    g = torch.Generator(device=DEV).manual_seed(0)
+    codes = torch.randint(0, 256, (E, N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
+    scales = torch.randint(118, 122, (E, N, K // 32), generator=g, device=DEV, dtype=torch.uint8)
+    w = ops.mx4_repack(ops.Mx4(codes, scales))
+    assert w.w.numel() > 1 << 31
+    cols = torch.tensor([0, 9000, N - 1], device=DEV)
+    for T in (2, 100):
+        a = torch.randn((T, K), generator=g, device=DEV).half()
+        ids, tw = route(T, E, 2)
+        ids[0, 0] = E - 1
+        got = ops.mx4_moe_gemm(a, w, ops.moe_align_block_size(ids, 16, E), tw, 2 * T, 2)
+        close(got[:, cols], *formula(a, codes[:, cols], scales[:, cols], ids, 2, None, None))
+
+
 def test_no_tokens():
     _, _, _, w = make(1, 64, 96, torch.float16, E=6)
     ids = torch.empty((0, 2), dtype=torch.int32, device=DEV)
