@@ -43,7 +43,8 @@ struct Vec8<MxF32> {
 };
 
 // Codes and scales in the order that they are kept in: a tensor of rows of whole
-// blocks is one run of blocks.  Bound by memory.
+// blocks is one run of blocks.  Bound by memory: 28672 x 4096 bf16 in 46 to 57 us,
+// 5.2 to 6.4 TB/s.
 template <typename DT>
 __global__ __launch_bounds__(kMxThreads) void mx4_quantize_kernel(const void* x, uint32_t* codes, uint8_t* scales,
                                                                   int64_t vecs) {
@@ -77,8 +78,8 @@ __global__ __launch_bounds__(kMxThreads) void mx4_rows_quantize_kernel(const voi
 // The same in the weights' layout: a wave takes 16 rows and NB k-tiles, a lane its
 // block of each.  Rows past the last are read as the last.  With few rows a wave
 // is one k-tile, with many a whole step whose scales leave as words: 128 rows of
-// 14336 take 5.6 us by steps and 4.4 by tiles under the profiler, 8192 rows 66 by
-// steps (4.5 TB/s).
+// 14336 take 5.6 us by steps and 4.7 by k-tiles under the profiler, 8192 rows 66 to
+// 70 by steps (4.3 to 4.5 TB/s).
 template <typename DT, int NB>
 __global__ __launch_bounds__(kMxThreads) void mx4_tile_quantize_kernel(const void* x, u32x4* codes, uint8_t* scales,
                                                                        uint32_t waves, int M, int K, int KT, int KS) {
@@ -115,7 +116,8 @@ __device__ __forceinline__ float mx4_value(uint32_t code) {
   return __builtin_bit_cast(float, bits | (code & 8) << 28);
 }
 
-// Values, each rounded once to the type asked for.
+// Values, each rounded once to the type asked for and stored past the caches: 28672
+// x 4096 bf16 in 44 us, 6.7 TB/s (69 us through them).
 template <typename E>
 __global__ __launch_bounds__(kMxThreads) void mx4_dequantize_kernel(const uint32_t* codes, const uint8_t* scales,
                                                                     E* out, int64_t vecs) {

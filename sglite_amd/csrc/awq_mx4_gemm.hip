@@ -22,7 +22,7 @@ namespace {
 
 struct MxArgs {
   const void* x;       // activations, or their codes
-  const uint8_t* xs;   // the codes' scales, in the rows' order
+  const uint8_t* xs;   // the codes' scales
   const char* w;
   const char* s;
   const void* bias;
@@ -41,6 +41,16 @@ struct MxArgs {
 // RM = 0: the rows come quantised, in the weights' layout.  Else a wave quantises
 // the step's part of up to 16 rows itself, RM of them loaded ahead: four lanes a
 // block, and through LDS into the operands' order.
+//
+// Bound by the weights' stream and the launch's own length: one row through
+// Qwen3-4B's qkv, o, gate/up with silu and down (8.4, 5.6, 26.5 and 13.2 MB) takes
+// 4.5, 4.0, 8.7 and 6.1 us in a graph.  From 64 rows on what counts is the rows'
+// way from the L2 (10 TB/s at 128 rows of 14336 x 4096, 18 us).  Quantising a block
+// a lane, with 16 loads a k-tile, took 35 us in place of 23 for those four layers.
+// Tried without gain: 16 rows loaded ahead (9 to 16 rows: 8.8 against 7.7 us for
+// qkv), rows a whole step ahead (128 rows of qkv 14.9 against 13.0: registers),
+// four column tiles a workgroup (128 rows of 14336 x 4096 26 against 21; experts
+// at one token 10.9 -> 12.3, at 32 43 -> 41.5).
 constexpr int kMxRowsWaves = 8;        // at most
 constexpr int kMxRowWords = 68;        // a quantised row's step in LDS: 256 bytes of codes, and 16 against bank conflicts
 constexpr int kMxExpertRows = 4;       // of an expert's rows, loaded ahead
@@ -314,6 +324,16 @@ constexpr int kMxCodes = 4 * (kMxTileM / 16) * 64;      // 16-byte vectors of a 
 constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 bytes a row
 // NTW = 4: two stages, weights two k-tiles ahead, two workgroups a CU.  NTW = 2,
 // for grids that leave CUs idle: three stages and weights six k-tiles ahead.
+//
+// 8192 rows of Llama-3-8B's gate/up with silu take 450 to 480 us without the
+// quantising launch, 4.0 to 4.3 PFLOP/s; the MFMA alone, its operands in registers,
+// reaches 6.2 on random data (9.0 on zeros: power).  MFMAs are busy 53 % of the
+// time there, the L2 gives 12 TB/s.  Tiles of 256 x 256 by eight waves, both
+// operands through a ring of LDS stages, take a third less from the L2 and were no
+// faster (526 against 509 us); neither were row operands further ahead, or
+// workgroups of one CU on one column group.  E = 128, H = 2048, I = 768 top-8 at
+// 4096 tokens: 93 and 86 us, MFMAs busy 20 %: four and two stages a tile, between
+// its start and its scattered rows' stores.
 constexpr int mx4_stages(int ntw) { return ntw == 4 ? 2 : 3; }
 constexpr int mx4_tile_lds(int ntw) { return (mx4_stages(ntw) * kMxStage + kMxTileM / 2) * 16; }  // row ids, routed weights
 
@@ -665,7 +685,9 @@ hipError_t launch_experts(const MxArgs& a, const Mx4Plan& p, int act, hipStream_
   return launch_expert_rows<DT, kActNone>(a, p, s);
 }
 
-// Rows up to which a product quantises them itself.
+// Rows up to which a product quantises them itself (us, itself / by a launch ahead:
+// Qwen3-4B's qkv, gate/up with silu and down at 8 rows 6.2 / 8.4, 12.7 / 12.3, 8.6 /
+// 10.2; at 16 rows 7.7 / 9.0, 15.0 / 12.9, 12.6 / 10.7).
 constexpr int kMxInlineRows = 8;
 
 // Waves of a workgroup of few rows: as many as leave none without a step, in
@@ -714,6 +736,7 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   }
   p.mt = (int)std::min<int64_t>(4, (M + 15) / 16);
   p.slots = (M + 16 * p.mt - 1) / (16 * p.mt);
+  // Two column tiles where the grid still fills the CUs: a row operand then serves both.
   p.ntw = act || tiles / 2 * p.slots >= 256 ? 2 : 1;
   p.groups = act ? tiles / 2 : tiles / p.ntw;
   p.grid = (p.groups + 7) / 8 * 8 * p.slots;

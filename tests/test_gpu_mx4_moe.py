@@ -97,7 +97,7 @@ def test_a_token_that_names_an_expert_twice(T):
 
 
 def test_stacks_past_31_bits():
-    E, N, K = 9, 16384, 30720
+    E, N, K = 9, 16384, 31744
     g = torch.Generator(device=DEV).manual_seed(0)
     codes = torch.randint(0, 256, (E, N, K // 2), generator=g, device=DEV, dtype=torch.uint8)
     scales = torch.randint(118, 122, (E, N, K // 32), generator=g, device=DEV, dtype=torch.uint8)
