@@ -452,8 +452,9 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  *   mul_routed_weight each sum times topk_weights[r] first.  Rows that the
  *   sorted table does not hold are not written
  * K % 32 == 0, N % 8 == 0, with an activation I % 32 == 0; x, a, w, bias, out and
- * ws 16-byte aligned.  Limits: K, N and M below 2^24, E <= 512, x of a product
- * below 2^34 elements, the routed activation rows below 2 GiB. */
+ * ws 16-byte aligned.  Limits: K, N and M below 2^24, E <= 512, x below 2^34
+ * elements, the routed activation rows below 2 GiB; a call repacks at most 2^24
+ * tiles of 16 rows by 512 k. */
 int awq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
                      awq_stream_t stream);
 int awq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,

@@ -896,8 +896,8 @@ int awq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* co
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_quantize: dtype must be 0, 1 or 2, got %d", dtype);
   const int st = check_mx4(rows, K, "awq_mx4_quantize");
   if (st != 0) return st;
-  if (rows >= (int64_t(1) << 31) || rows * K >= (int64_t(1) << 35))
-    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_quantize: x must have below 2^35 elements");
+  if (rows >= (int64_t(1) << 30) || rows * K >= (int64_t(1) << 34))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_quantize: x must have below 2^34 elements");
   if (rows == 0) return ok();
   if (!x || !codes || !scales) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_quantize: null pointer argument");
   if (!aligned(x, 16) || !aligned(codes, 4))
@@ -913,8 +913,8 @@ int awq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int6
     return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_dequantize: dtype must be 0, 1 or 2, got %d", dtype);
   const int st = check_mx4(rows, K, "awq_mx4_dequantize");
   if (st != 0) return st;
-  if (rows >= (int64_t(1) << 31) || rows * K >= (int64_t(1) << 35))
-    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_dequantize: the tensor must have below 2^35 elements");
+  if (rows >= (int64_t(1) << 30) || rows * K >= (int64_t(1) << 34))
+    return fail(AWQ_STATUS_UNSUPPORTED, "awq_mx4_dequantize: the tensor must have below 2^34 elements");
   if (rows == 0) return ok();
   if (!codes || !scales || !out) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_dequantize: null pointer argument");
   if (!aligned(codes, 4) || !aligned(out, 16))
