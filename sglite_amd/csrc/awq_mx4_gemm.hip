@@ -60,7 +60,7 @@ template <typename DT, int RM, int MT, int NTW, int ACT>
 struct RowsBody {
   using E = typename DT::elem;
   using V4 = typename DT::vec4;
-  using V8 = typename DT::vec8;
+  // Weights that one row block reads pass the caches as a stream.
   static constexpr int kPolicy = MT == 4 ? 0 : kCacheStream;
   static constexpr int XM = RM == 0 ? MT : 1;
 
@@ -737,7 +737,7 @@ Mx4Plan plan_mx4(int64_t M, int64_t N, int64_t K, int act) {
   p.mt = (int)std::min<int64_t>(4, (M + 15) / 16);
   p.slots = (M + 16 * p.mt - 1) / (16 * p.mt);
   // Two column tiles where the grid still fills the CUs: a row operand then serves both.
-  p.ntw = act || tiles / 2 * p.slots >= 256 ? 2 : 1;
+  p.ntw = act || tiles / 2 * p.slots >= device_cu_count() ? 2 : 1;
   p.groups = act ? tiles / 2 : tiles / p.ntw;
   p.grid = (p.groups + 7) / 8 * 8 * p.slots;
   p.waves = rows_waves(K);
