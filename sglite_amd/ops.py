@@ -79,6 +79,16 @@ def _on_device(device: torch.device) -> Iterator[None]:
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
+def _traced(t: torch.Tensor) -> bool:
+    """Whether t is a tensor of a trace, which has no address."""
+    return torch.compiler.is_compiling() or (type(t) not in _PLAIN and is_fake(t))
+
+
+def _at(t: torch.Tensor, a: int) -> bool:
+    """Whether t lies at a multiple of ``a`` bytes, as far as it has an address."""
+    return _traced(t) or t.data_ptr() % a == 0
+
+
 def _undispatched(*tensors: Optional[torch.Tensor]) -> bool:
     """True where the dispatcher would only hand these tensors on to the device implementation: plain tensors
     and Parameters outside every mode, trace, transform, profiler and gradient.  A call may then run that
@@ -488,18 +498,18 @@ def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, de
         raise ValueError(f"{what} must be {dtype}, got {out.dtype}")
     if out.device != device:
         raise ValueError(f"{what} must be on {device}, got {out.device}")
-    if not out.is_contiguous() or out.data_ptr() % 8:
+    if not out.is_contiguous() or not _at(out, 8):
         raise ValueError(f"{what} must be contiguous and 8-byte aligned")
 
 
 def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
     """Whether the address ranges that two tensors' elements span meet (the tensors of a trace have none)."""
-    if torch.compiler.is_compiling() or s.numel() == 0 or t.numel() == 0:
+    if _traced(s) or _traced(t) or s.numel() == 0 or t.numel() == 0:
         return False
 
     def end(v: torch.Tensor) -> int:
         return v.data_ptr() + (sum((n - 1) * st for n, st in zip(v.shape, v.stride())) + 1) * v.element_size()
-    return s.data_ptr() < end(t) and t.data_ptr() < end(s) and not (is_fake(s) or is_fake(t))
+    return s.data_ptr() < end(t) and t.data_ptr() < end(s)
 
 
 def _check_counters(counters: torch.Tensor, N: int, device: torch.device) -> None:
@@ -1174,6 +1184,27 @@ def _check_mx4(q: Mx4) -> Tuple[int, ...]:
     return tuple(codes.shape[:-1]) + (K,)
 
 
+def _check_mx4_source(x: torch.Tensor) -> None:
+    if x.dtype not in _MX4_DTYPES:
+        raise ValueError(f"MXFP4 is made from float16, bfloat16 or float32, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one axis")
+    _mx4_rows(x.shape[-1])
+
+
+def _check_mx4_values(q: Mx4, dtype: torch.dtype) -> None:
+    _check_mx4(q)
+    if dtype not in _MX4_DTYPES:
+        raise ValueError(f"values are float16, bfloat16 or float32, got {dtype}")
+
+
+def _check_mx4_pack(q: Mx4) -> Tuple[int, ...]:
+    shape = _check_mx4(q)
+    if len(shape) not in (2, 3):
+        raise ValueError(f"the weight must be [N, K] or [E, N, K], got {shape}")
+    return shape
+
+
 def _mx4_quantize_launch(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     K, dev = x.shape[-1], x.device
     if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
@@ -1189,11 +1220,13 @@ def _mx4_quantize_launch(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_quantize", mutates_args=(), device_types="cuda")
 def _mx4_quantize_op(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    _check_mx4_source(x)
     return _mx4_quantize_launch(x)
 
 
 @_mx4_quantize_op.register_fake
 def _(x):
+    _check_mx4_source(x)
     K = x.shape[-1]
     return (x.new_empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8),
             x.new_empty(x.shape[:-1] + (K // MX4_BLOCK,), dtype=torch.uint8))
@@ -1205,11 +1238,7 @@ def mx4_quantize(x: torch.Tensor) -> Mx4:
     A block's byte is that of 2^e, e the exponent of its largest magnitude less 2 (at least -127); each value goes to
     the nearest one, ties to the even code, and beyond 6 * 2^e to that.  A block that holds an infinity or NaN becomes
     NaN whole."""
-    if x.dtype not in _MX4_DTYPES:
-        raise ValueError(f"MXFP4 is made from float16, bfloat16 or float32, got {x.dtype}")
-    if x.dim() < 1:
-        raise ValueError("x must have at least one axis")
-    _mx4_rows(x.shape[-1])
+    _check_mx4_source(x)
     _require_cuda(x)
     if _undispatched(x):
         return Mx4(*_mx4_quantize_launch(x))
@@ -1230,19 +1259,19 @@ def _mx4_dequantize_launch(codes: torch.Tensor, scales: torch.Tensor, dtype: tor
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_dequantize", mutates_args=(), device_types="cuda")
 def _mx4_dequantize_op(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    _check_mx4_values(Mx4(codes, scales), dtype)
     return _mx4_dequantize_launch(codes, scales, dtype)
 
 
 @_mx4_dequantize_op.register_fake
 def _(codes, scales, dtype):
+    _check_mx4_values(Mx4(codes, scales), dtype)
     return codes.new_empty(codes.shape[:-1] + (codes.shape[-1] * 2,), dtype=dtype)
 
 
 def mx4_dequantize(q: Mx4, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values of q, [..., K], each rounded once to ``dtype`` (float16, bfloat16 or float32)."""
-    _check_mx4(q)
-    if dtype not in _MX4_DTYPES:
-        raise ValueError(f"values are float16, bfloat16 or float32, got {dtype}")
+    _check_mx4_values(q, dtype)
     _require_cuda(*q)
     if _undispatched(*q):
         return _mx4_dequantize_launch(q.codes, q.scales, dtype)
@@ -1264,6 +1293,7 @@ def mx4_weight_bytes(N: int, K: int) -> Tuple[int, int]:
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_repack", mutates_args=(), device_types="cuda")
 def _mx4_repack_op(codes: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    _check_mx4_pack(Mx4(codes, scales))
     lead, N, K, dev = tuple(codes.shape[:-2]), codes.shape[-2], codes.shape[-1] * 2, codes.device
     wb, sb = mx4_weight_bytes(N, K)
     codes, scales = _aligned(codes), scales.contiguous()
@@ -1277,15 +1307,14 @@ def _mx4_repack_op(codes: torch.Tensor, scales: torch.Tensor) -> Tuple[torch.Ten
 
 @_mx4_repack_op.register_fake
 def _(codes, scales):
+    _check_mx4_pack(Mx4(codes, scales))
     wb, sb = _mx4_layout_bytes(codes.shape[-2], codes.shape[-1] * 2)
     return codes.new_empty(codes.shape[:-2] + (wb,)), codes.new_empty(codes.shape[:-2] + (sb,))
 
 
 def mx4_repack(q: Mx4) -> Mx4Weight:
     """A weight [N, K], or a stack of experts' [E, N, K], laid out for ``mx4_gemm`` and ``mx4_moe_gemm``, once."""
-    shape = _check_mx4(q)
-    if len(shape) not in (2, 3):
-        raise ValueError(f"the weight must be [N, K] or [E, N, K], got {shape}")
+    shape = _check_mx4_pack(q)
     mx4_weight_bytes(shape[-2], shape[-1])  # refuses sizes that the products cannot take
     _require_cuda(*q)
     return Mx4Weight(*torch.ops.sglite_awq.awq_mx4_repack(q.codes, q.scales), shape[-2], shape[-1])
@@ -1293,6 +1322,7 @@ def mx4_repack(q: Mx4) -> Mx4Weight:
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_unrepack", mutates_args=(), device_types="cuda")
 def _mx4_unrepack_op(w: torch.Tensor, s: torch.Tensor, N: int, K: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    _check_mx4_weight(Mx4Weight(w, s, N, K), 2 if w.dim() == 2 else 1)
     lead, dev = tuple(w.shape[:-1]), w.device
     codes = torch.empty(lead + (N, K // 2), dtype=torch.uint8, device=dev)
     scales = torch.empty(lead + (N, K // MX4_BLOCK), dtype=torch.uint8, device=dev)
@@ -1305,20 +1335,22 @@ def _mx4_unrepack_op(w: torch.Tensor, s: torch.Tensor, N: int, K: int) -> Tuple[
 
 @_mx4_unrepack_op.register_fake
 def _(w, s, N, K):
+    _check_mx4_weight(Mx4Weight(w, s, N, K), 2 if w.dim() == 2 else 1)
     return w.new_empty(w.shape[:-1] + (N, K // 2)), w.new_empty(w.shape[:-1] + (N, K // MX4_BLOCK))
 
 
 def _check_mx4_weight(weight: Mx4Weight, dims: int) -> None:
     """A weight that mx4_repack made, of one linear (dims 1) or a stack of experts (2)."""
-    if weight.w.dim() != dims or weight.s.dim() != dims or weight.w.shape[:-1] != weight.s.shape[:-1]:
+    w, s, N, K = weight
+    if w.dim() != dims or s.dim() != dims or w.shape[:-1] != s.shape[:-1]:
         raise ValueError("the weight must be " + ("one linear's [N, K]" if dims == 1 else "a stack of experts' [E, N, K]")
                          + " from mx4_repack")
-    if (weight.w.shape[-1], weight.s.shape[-1]) != _mx4_layout_bytes(weight.N, weight.K):
-        raise ValueError(f"the weight does not hold [{weight.N}, {weight.K}]")
-    for t in weight[:2]:
-        if t.dtype != torch.uint8 or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError("the weight must be mx4_repack's: contiguous, 16-byte aligned uint8")
-    if weight.w.device != weight.s.device:
+    if (w.shape[-1], s.shape[-1]) != _mx4_layout_bytes(N, K):
+        raise ValueError(f"the weight does not hold [{N}, {K}]")
+    if not (w.dtype == s.dtype == torch.uint8) or not w.is_contiguous() or not s.is_contiguous() \
+            or not (_traced(w) or (w.data_ptr() | s.data_ptr()) % 16 == 0):
+        raise ValueError("the weight must be mx4_repack's: contiguous, 16-byte aligned uint8")
+    if w.device != s.device:
         raise ValueError("the weight must be on one device")
 
 
@@ -1353,28 +1385,28 @@ def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Op
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_gemm", mutates_args=(), device_types="cuda")
 def _mx4_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor], N: int, K: int,
                  activation: str) -> torch.Tensor:
-    act = _ACT_CODE[_ACT_NAME[activation]]
-    _check_mx4_product(x, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 1)
+    act = _check_mx4_gemm_op(x, w, s, bias, N, K, activation)
     out = torch.empty((x.shape[0], N // 2 if act else N), dtype=x.dtype, device=x.device)
-    _mx4_gemm_launch(_aligned(x), w, s, bias, out, N, K, act)
+    _mx4_gemm_launch(_aligned(x), w, s, None if bias is None else _aligned(bias), out, N, K, act)
     return out
 
 
 @_mx4_gemm_op.register_fake
 def _(x, w, s, bias, N, K, activation):
+    _check_mx4_gemm_op(x, w, s, bias, N, K, activation)
     return x.new_empty((x.shape[0], N if activation == "none" else N // 2))
 
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_mx4_gemm_out", mutates_args=("out",), device_types="cuda")
 def _mx4_gemm_out_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
                      out: torch.Tensor, N: int, K: int, activation: str) -> None:
-    _check_mx4_product(x, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 1)
-    _mx4_gemm_launch(_aligned(x), w, s, bias, out, N, K, _ACT_CODE[_ACT_NAME[activation]])
+    act = _check_mx4_gemm_op(x, w, s, bias, N, K, activation, out)
+    _mx4_gemm_launch(_aligned(x), w, s, None if bias is None else _aligned(bias), out, N, K, act)
 
 
 @_mx4_gemm_out_op.register_fake
 def _(x, w, s, bias, out, N, K, activation):
-    return None
+    _check_mx4_gemm_op(x, w, s, bias, N, K, activation, out)
 
 
 def _check_mx4_product(x: torch.Tensor, weight: Mx4Weight, activation: Optional[str], dims: int) -> None:
@@ -1391,9 +1423,37 @@ def _check_mx4_product(x: torch.Tensor, weight: Mx4Weight, activation: Optional[
         raise ValueError("the activations and the weight must be on one device")
 
 
+def _check_mx4_bias(bias: torch.Tensor, x: torch.Tensor, N: int) -> None:
+    if bias.numel() != N:
+        raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
+    if bias.device != x.device:
+        raise ValueError("the activations and the bias must be on one device")
+
+
+def _mx4_op_activation(activation: str) -> Optional[str]:
+    """The activation that a registered op names."""
+    if activation not in _ACT_NAME:
+        raise ValueError(f"unsupported activation {activation!r}")
+    return _ACT_NAME[activation]
+
+
+def _check_mx4_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor], N: int, K: int,
+                       activation: str, out: Optional[torch.Tensor] = None) -> int:
+    """What the registered products read and write; the activation's code."""
+    act = _mx4_op_activation(activation)
+    _check_mx4_product(x, Mx4Weight(w, s, N, K), act, 1)
+    if bias is not None:
+        _check_mx4_bias(bias, x, N)
+        if bias.dtype != x.dtype:
+            raise ValueError(f"bias must be {x.dtype} as the activations, got {bias.dtype}")
+    if out is not None:
+        _check_mx4_out(out, (x.shape[0], N if act is None else N // 2), x, w, s, bias)
+    return _ACT_CODE[act]
+
+
 def _check_mx4_out(out: torch.Tensor, shape: Tuple[int, ...], x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     _check_out(out, shape, x.dtype, x.device)
-    if out.data_ptr() % 16:
+    if not _at(out, 16):
         raise ValueError("out must be 16-byte aligned")
     if any(t is not None and _overlap(out, t) for t in (x,) + others):
         raise ValueError("out must not share memory with an input")
@@ -1410,10 +1470,7 @@ def mx4_gemm(x: torch.Tensor, weight: Mx4Weight, bias: Optional[torch.Tensor] = 
     w, s, N, K = weight
     _require_cuda(x, w, s, bias)
     if bias is not None:
-        if bias.numel() != N:
-            raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
-        if bias.device != x.device:
-            raise ValueError("the activations and the bias must be on one device")
+        _check_mx4_bias(bias, x, N)
         bias = _aligned(bias.to(x.dtype).reshape(-1))
     x = _aligned(x)
     if out is not None:
@@ -1451,14 +1508,52 @@ def _mx4_moe_launch(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_id
 def _mx4_moe_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_ids: torch.Tensor,
                 expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, N: int, K: int,
                 num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> None:
-    _check_mx4_product(a, Mx4Weight(w, s, N, K), _ACT_NAME[activation], 2)
-    _mx4_moe_launch(_aligned(a), w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k,
-                    _ACT_CODE[_ACT_NAME[activation]], mul_routed_weight)
+    act = _check_mx4_moe_op(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k,
+                            activation, mul_routed_weight)
+    topk_weights = None if topk_weights is None else _aligned(topk_weights, 4)
+    _mx4_moe_launch(_aligned(a), w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k, act,
+                    mul_routed_weight)
 
 
 @_mx4_moe_op.register_fake
 def _(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k, activation, mul_routed_weight):
-    return None
+    _check_mx4_moe_op(a, w, s, sorted_ids, expert_offsets, topk_weights, out, N, K, num_routed, top_k, activation,
+                      mul_routed_weight)
+
+
+def _check_mx4_moe(a: torch.Tensor, experts: Mx4Weight, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
+                   topk_weights: Optional[torch.Tensor], num_routed: int, top_k: int, activation: Optional[str],
+                   mul_routed_weight: bool) -> None:
+    _check_mx4_product(a, experts, activation, 2)
+    E = experts.w.shape[0]
+    if mul_routed_weight and topk_weights is None:
+        raise ValueError("mul_routed_weight needs topk_weights")
+    if num_routed < 0 or top_k < 1:
+        raise ValueError(f"num_routed must be at least 0 and top_k at least 1, got {num_routed} and {top_k}")
+    if expert_offsets.numel() != E + 1:
+        raise ValueError(f"the rows were aligned for {expert_offsets.numel() - 1} experts, the stack holds {E}")
+    if sorted_ids.dtype != torch.int32 or expert_offsets.dtype != torch.int32 \
+            or not sorted_ids.is_contiguous() or not expert_offsets.is_contiguous():
+        raise ValueError("the alignment must be moe_align_block_size's: contiguous int32")
+    if topk_weights is not None and topk_weights.numel() < num_routed:
+        raise ValueError(f"topk_weights must hold {num_routed} routed weights, got {topk_weights.numel()}")
+    _require_cuda(a, experts.w, topk_weights, sorted_ids, expert_offsets)
+    for t in (topk_weights, sorted_ids, expert_offsets):
+        if t is not None and t.device != a.device:
+            raise ValueError("a, the experts, the weights and the alignment must be on one device")
+
+
+def _check_mx4_moe_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, sorted_ids: torch.Tensor,
+                      expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, N: int,
+                      K: int, num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> int:
+    """What the registered product reads and writes; the activation's code."""
+    act = _mx4_op_activation(activation)
+    _check_mx4_moe(a, Mx4Weight(w, s, N, K), sorted_ids, expert_offsets, topk_weights, num_routed, top_k, act,
+                   mul_routed_weight)
+    if topk_weights is not None and topk_weights.dtype != torch.float32:
+        raise ValueError(f"topk_weights must be float32, got {topk_weights.dtype}")
+    _check_mx4_out(out, (num_routed, N if act is None else N // 2), a, w, s, topk_weights, sorted_ids, expert_offsets)
+    return _ACT_CODE[act]
 
 
 def mx4_moe_gemm(a: torch.Tensor, experts: Mx4Weight, align: MoeAlignment, topk_weights: Optional[torch.Tensor],
@@ -1469,24 +1564,9 @@ def mx4_moe_gemm(a: torch.Tensor, experts: Mx4Weight, align: MoeAlignment, topk_
     Routed row r reads ``a[r // top_k]``; the output has ``num_routed`` rows of ``N`` columns, or ``N / 2`` of
     ``act(gate) * up``; with ``mul_routed_weight`` each sum is multiplied by the row's routed weight first.  Rows that
     ``align`` (16-row blocks) does not hold (ids outside the experts) are not written."""
-    _check_mx4_product(a, experts, activation, 2)
+    _check_mx4_moe(a, experts, align.sorted_ids, align.expert_offsets, topk_weights, num_routed, top_k, activation,
+                   mul_routed_weight)
     w, s, N, K = experts
-    E = w.shape[0]
-    if mul_routed_weight and topk_weights is None:
-        raise ValueError("mul_routed_weight needs topk_weights")
-    if num_routed < 0 or top_k < 1:
-        raise ValueError(f"num_routed must be at least 0 and top_k at least 1, got {num_routed} and {top_k}")
-    if align.expert_offsets.numel() != E + 1:
-        raise ValueError(f"the rows were aligned for {align.expert_offsets.numel() - 1} experts, the stack holds {E}")
-    if align.sorted_ids.dtype != torch.int32 or align.expert_offsets.dtype != torch.int32 \
-            or not align.sorted_ids.is_contiguous() or not align.expert_offsets.is_contiguous():
-        raise ValueError("the alignment must be moe_align_block_size's: contiguous int32")
-    if topk_weights is not None and topk_weights.numel() < num_routed:
-        raise ValueError(f"topk_weights must hold {num_routed} routed weights, got {topk_weights.numel()}")
-    _require_cuda(a, w, topk_weights, align.sorted_ids, align.expert_offsets)
-    for t in (topk_weights, align.sorted_ids, align.expert_offsets):
-        if t is not None and t.device != a.device:
-            raise ValueError("a, the experts, the weights and the alignment must be on one device")
     a = _aligned(a)
     shape = (num_routed, N // 2 if activation is not None else N)
     if out is None:
