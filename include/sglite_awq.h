@@ -387,7 +387,7 @@ enum { AWQ_MOE_ACT_NONE = 0, AWQ_MOE_ACT_SILU = 1, AWQ_MOE_ACT_GELU = 2 };
  * python/sglite/kernels/moe_triton.py:8-65) for AWQ B operands.
  *   a        [a_rows, K]; routed row r reads activation row r / top_k
  *            (top_k = topk for the first GEMM, 1 for the second, as in
- *            moe_triton.py's `top_k` argument)
+ *            moe_triton.py's `top_k` argument; below 2^31)
  *   w/s/z    expert-stacked repacked weights of [K, N] per expert
  *   out      activation == AWQ_MOE_ACT_NONE: [num_routed, N], row r
  *            activation != NONE: N = 2I (gate columns first, then up), the
@@ -406,7 +406,8 @@ int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void*
 /* The same product for dense (fp16 or bf16) experts; replaces fused_moe_kernel
  * (python/sglite/kernels/triton/fused_moe.py:54-183) for the weights that the
  * reference's backend holds.
- *   a        [a_rows, K]; routed row r reads activation row r / top_k
+ *   a        [a_rows, K]; routed row r reads activation row r / top_k (top_k
+ *            below 2^31)
  *   w        [E, N, K], each expert's rows contiguous
  *   out      activation == AWQ_MOE_ACT_NONE: [num_routed, N]
  *            activation != NONE: N = 2I (gate rows first, then up) ->

@@ -723,6 +723,9 @@ int awq_moe_route(const void* gating_output, int dtype, int64_t T, int64_t E, in
   return hip_status(launch_moe_route(p, (hipStream_t)stream), "awq_moe_route launch");
 }
 
+// The kernels divide a routed row's number by top_k in 32 bits.
+static constexpr int64_t kMaxTopK = int64_t(1) << 31;
+
 int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void* s, const void* z, int64_t E,
                        int64_t N, int64_t K, int64_t G, int dtype, const int32_t* sorted_ids, int64_t sorted_cap,
                        const int32_t* expert_offsets, const float* topk_weights, int64_t num_routed, int64_t top_k,
@@ -738,7 +741,8 @@ int awq_moe_w4a16_gemm(const void* a, int64_t a_rows, const void* w, const void*
   if (activation != AWQ_MOE_ACT_NONE && N % 32 != 0)
     return fail(AWQ_STATUS_INVALID_ARGUMENT,
                 "awq_moe_w4a16_gemm: gate/up pairing needs N = 2I with I %% 16 == 0, got N=%lld", (long long)N);
-  if (top_k <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_w4a16_gemm: top_k must be positive");
+  if (top_k <= 0 || top_k >= kMaxTopK)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_w4a16_gemm: top_k must be in [1, 2^31), got %lld", (long long)top_k);
   if (num_routed < 0 || num_routed >= (int64_t(1) << 24) || sorted_cap < 0 || sorted_cap >= (int64_t(1) << 30))
     return fail(AWQ_STATUS_UNSUPPORTED, "awq_moe_w4a16_gemm: num_routed must be below 2^24 and sorted_cap below 2^30");
   if ((num_routed + top_k - 1) / top_k > a_rows)
@@ -791,7 +795,8 @@ int awq_moe_dense_gemm(const void* a, int64_t a_rows, const void* w, int64_t E, 
   if (activation != AWQ_MOE_ACT_NONE && N % 16 != 0)
     return fail(AWQ_STATUS_INVALID_ARGUMENT,
                 "awq_moe_dense_gemm: gate/up pairing needs N = 2I with I %% 8 == 0, got N=%lld", (long long)N);
-  if (top_k <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: top_k must be positive");
+  if (top_k <= 0 || top_k >= kMaxTopK)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_moe_dense_gemm: top_k must be in [1, 2^31), got %lld", (long long)top_k);
   if (num_routed < 0 || num_routed >= (int64_t(1) << 24) || sorted_cap < 0 || sorted_cap >= (int64_t(1) << 30))
     return fail(AWQ_STATUS_UNSUPPORTED, "awq_moe_dense_gemm: num_routed must be below 2^24 and sorted_cap below 2^30");
   const int64_t rows = (num_routed + top_k - 1) / top_k, lim = int64_t(1) << 31;
@@ -1011,7 +1016,8 @@ int check_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64
   const int st = check_mx4_weight(N, K, activation, who);
   if (st != 0) return st;
   if (E <= 0 || E > 512) return fail(AWQ_STATUS_UNSUPPORTED, "%s: E must be in [1, 512], got %lld", who, (long long)E);
-  if (top_k <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: top_k must be positive", who);
+  if (top_k <= 0 || top_k >= kMaxTopK)
+    return fail(AWQ_STATUS_INVALID_ARGUMENT, "%s: top_k must be in [1, 2^31), got %lld", who, (long long)top_k);
   if (num_routed < 0 || num_routed >= (int64_t(1) << 24))
     return fail(AWQ_STATUS_UNSUPPORTED, "%s: num_routed must be in [0, 2^24)", who);
   const int64_t rows = (num_routed + top_k - 1) / top_k;
