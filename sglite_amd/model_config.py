@@ -9,7 +9,8 @@ AWQ is recognised by ``quant_method == "awq"`` or, with no method given, by a
 falls back to Triton; here both methods run the same gfx950 kernels, and the
 same preference decides only which config class (and so which shape rules and
 metadata) the model gets.  Remote hub lookups are not performed.  Beyond the
-reference, ``quant_method == "mxfp4"`` gives the MXFP4 config.
+reference, ``quant_method == "mxfp4"`` gives the MXFP4 config, if it implements
+all that is asked for; else, as every method not known here, no config at all.
 """
 
 from __future__ import annotations
@@ -52,7 +53,10 @@ def load_quantization_config(model_path: str, hf_config: Optional[Any] = None,
     if quant_method == "mxfp4":
         from .quantization.mxfp4 import MXFP4Config
 
-        return MXFP4Config.from_config(config_dict)
+        try:
+            return MXFP4Config.from_config(config_dict)
+        except ValueError as e:
+            logger.warning("Not an MXFP4 config of this engine, taken as no quantization config: %s", e)
     return None
 
 

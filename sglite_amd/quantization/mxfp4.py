@@ -4,7 +4,8 @@ No counterpart in the reference; the interface is that of its methods (base_conf
 ``weight`` uint8 [N, K/2] (two codes a byte, the lower k in the low bits) and ``weight_scale`` uint8 [N, K/32]
 (exponent bytes) for every projection, which the loader shards and merges like a dense weight (weight_loader.py:40-77);
 with ``is_checkpoint_mxfp4_serialized`` false it holds 16- or 32-bit ``weight`` [N, K], quantised once after loading.
-Activations are quantised by the products (``ops.mx4_gemm``).
+Activations are quantised by the products (``ops.mx4_gemm``).  The configuration is this framework's own: published
+ones of the same method name mean weight-only experts beside 16-bit layers, which it does not implement and refuses.
 """
 
 from typing import Any, Dict, List, Optional
@@ -38,7 +39,7 @@ class MXFP4Config(QuantizationConfig):
         return [torch.half, torch.bfloat16]
 
     def get_min_capability(self) -> int:
-        return 80
+        return 95  # the products are gfx950's scaled MFMAs
 
     @staticmethod
     def get_config_filenames() -> List[str]:
@@ -46,6 +47,12 @@ class MXFP4Config(QuantizationConfig):
 
     @classmethod
     def from_config(cls, config: Dict[str, Any]) -> "MXFP4Config":
+        """Every linear layer's weights and activations in MXFP4; what else a config asks for is refused by name."""
+        known = ("quant_method", "is_checkpoint_mxfp4_serialized", "bits", "group_size")
+        others = sorted(k for k, v in config.items() if k not in known and v not in (None, False, [], {}, ""))
+        if others:
+            raise ValueError(f"the mxfp4 method quantises all linear layers, weights and activations; it does not "
+                             f"implement {others}")
         return cls(bool(config.get("is_checkpoint_mxfp4_serialized", True)), config.get("bits", 4),
                    config.get("group_size", ops.MX4_BLOCK))
 
