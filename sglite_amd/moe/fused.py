@@ -47,7 +47,7 @@ def _expert_dims(w: MoeWeights) -> Tuple[int, int, int]:
         assert w.dim() == 3, "dense expert weights must be [E, N, K]"
         return w.shape[0], w.shape[2], w.shape[1]
     if isinstance(w, ops.Mx4Weight):
-        return w.num_experts, w.K, w.N
+        return ops._mx4_num_experts(w), w.K, w.N
     return w.num_experts, w.input_size, w.output_size
 
 

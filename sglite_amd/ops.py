@@ -79,16 +79,6 @@ def _on_device(device: torch.device) -> Iterator[None]:
 _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
-def _traced(t: torch.Tensor) -> bool:
-    """Whether t is a tensor of a trace, which has no address."""
-    return torch.compiler.is_compiling() or (type(t) not in _PLAIN and is_fake(t))
-
-
-def _at(t: torch.Tensor, a: int) -> bool:
-    """Whether t lies at a multiple of ``a`` bytes, as far as it has an address."""
-    return _traced(t) or t.data_ptr() % a == 0
-
-
 def _undispatched(*tensors: Optional[torch.Tensor]) -> bool:
     """True where the dispatcher would only hand these tensors on to the device implementation: plain tensors
     and Parameters outside every mode, trace, transform, profiler and gradient.  A call may then run that
@@ -490,21 +480,31 @@ def _(x, w, s, z, bias, counters, out, K, N, G, activation):
     return None
 
 
-def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device,
-               what: str = "out") -> None:
+def _check_out_form(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device,
+                    what: str = "out") -> None:
+    """All but the address, which the tensors of a trace have not."""
     if tuple(out.shape) != tuple(shape):
         raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(out.shape)}")
     if out.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {out.dtype}")
     if out.device != device:
         raise ValueError(f"{what} must be on {device}, got {out.device}")
-    if not out.is_contiguous() or not _at(out, 8):
+    if not out.is_contiguous():
+        raise ValueError(f"{what} must be contiguous and 8-byte aligned")
+
+
+def _check_out(out: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device,
+               what: str = "out") -> None:
+    _check_out_form(out, shape, dtype, device, what)
+    if out.data_ptr() % 8:
         raise ValueError(f"{what} must be contiguous and 8-byte aligned")
 
 
 def _overlap(s: torch.Tensor, t: torch.Tensor) -> bool:
     """Whether the address ranges that two tensors' elements span meet (the tensors of a trace have none)."""
-    if _traced(s) or _traced(t) or s.numel() == 0 or t.numel() == 0:
+    if torch.compiler.is_compiling() or s.numel() == 0 or t.numel() == 0:
+        return False
+    if any(type(v) not in _PLAIN and is_fake(v) for v in (s, t)):
         return False
 
     def end(v: torch.Tensor) -> int:
@@ -1154,12 +1154,17 @@ class Mx4Weight(NamedTuple):
 
     @property
     def num_experts(self) -> int:
-        if self.w.dim() != 2:
-            raise ValueError("this weight is one linear's, not a stack of experts'")
-        return self.w.shape[0]
+        return _mx4_num_experts(self)
 
     def expert(self, e: int) -> "Mx4Weight":
         return Mx4Weight(self.w[e], self.s[e], self.N, self.K)
+
+
+def _mx4_num_experts(weight: Mx4Weight) -> int:
+    """``weight.num_experts``, where a compiler traces (it reads no property of a named tuple)."""
+    if weight.w.dim() != 2:
+        raise ValueError("this weight is one linear's, not a stack of experts'")
+    return weight.w.shape[0]
 
 
 def _mx4_rows(K: int) -> None:
@@ -1347,9 +1352,9 @@ def _check_mx4_weight(weight: Mx4Weight, dims: int) -> None:
                          + " from mx4_repack")
     if (w.shape[-1], s.shape[-1]) != _mx4_layout_bytes(N, K):
         raise ValueError(f"the weight does not hold [{N}, {K}]")
-    if not (w.dtype == s.dtype == torch.uint8) or not w.is_contiguous() or not s.is_contiguous() \
-            or not (_traced(w) or (w.data_ptr() | s.data_ptr()) % 16 == 0):
-        raise ValueError("the weight must be mx4_repack's: contiguous, 16-byte aligned uint8")
+    # Addresses are the C ABI's to check: a compiler traces none.
+    if not (w.dtype == s.dtype == torch.uint8) or not w.is_contiguous() or not s.is_contiguous():
+        raise ValueError("the weight must be mx4_repack's: contiguous uint8")
     if w.device != s.device:
         raise ValueError("the weight must be on one device")
 
@@ -1423,6 +1428,11 @@ def _check_mx4_product(x: torch.Tensor, weight: Mx4Weight, activation: Optional[
         raise ValueError("the activations and the weight must be on one device")
 
 
+def _mx4_operand(t: torch.Tensor, a: int = 16) -> torch.Tensor:
+    """t as a launch takes it; of a compiled call the registered op sees to its address."""
+    return t.contiguous() if torch.compiler.is_compiling() else _aligned(t, a)
+
+
 def _check_mx4_bias(bias: torch.Tensor, x: torch.Tensor, N: int) -> None:
     if bias.numel() != N:
         raise ValueError(f"bias must have {N} elements, got {bias.numel()}")
@@ -1452,9 +1462,7 @@ def _check_mx4_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: 
 
 
 def _check_mx4_out(out: torch.Tensor, shape: Tuple[int, ...], x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    _check_out(out, shape, x.dtype, x.device)
-    if not _at(out, 16):
-        raise ValueError("out must be 16-byte aligned")
+    _check_out_form(out, shape, x.dtype, x.device)
     if any(t is not None and _overlap(out, t) for t in (x,) + others):
         raise ValueError("out must not share memory with an input")
 
@@ -1471,8 +1479,8 @@ def mx4_gemm(x: torch.Tensor, weight: Mx4Weight, bias: Optional[torch.Tensor] = 
     _require_cuda(x, w, s, bias)
     if bias is not None:
         _check_mx4_bias(bias, x, N)
-        bias = _aligned(bias.to(x.dtype).reshape(-1))
-    x = _aligned(x)
+        bias = _mx4_operand(bias.to(x.dtype).reshape(-1))
+    x = _mx4_operand(x)
     if out is not None:
         _check_mx4_out(out, (x.shape[0], N if activation is None else N // 2), x, w, s, bias)
     if _undispatched(x, w, s, bias, out):
@@ -1567,14 +1575,14 @@ def mx4_moe_gemm(a: torch.Tensor, experts: Mx4Weight, align: MoeAlignment, topk_
     _check_mx4_moe(a, experts, align.sorted_ids, align.expert_offsets, topk_weights, num_routed, top_k, activation,
                    mul_routed_weight)
     w, s, N, K = experts
-    a = _aligned(a)
+    a = _mx4_operand(a)
     shape = (num_routed, N // 2 if activation is not None else N)
     if out is None:
         out = torch.empty(shape, dtype=a.dtype, device=a.device)
     else:
         _check_mx4_out(out, shape, a, w, s, topk_weights, align.sorted_ids, align.expert_offsets)
     if topk_weights is not None:
-        topk_weights = _aligned(topk_weights.float().reshape(-1), 4)
+        topk_weights = _mx4_operand(topk_weights.float().reshape(-1), 4)
     if _undispatched(a, w, s, topk_weights, out, align.sorted_ids, align.expert_offsets):
         _mx4_moe_launch(a, w, s, align.sorted_ids, align.expert_offsets, topk_weights, out, N, K, num_routed, top_k,
                         _ACT_CODE[activation], mul_routed_weight)
