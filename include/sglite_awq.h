@@ -466,6 +466,11 @@ int awq_mx4_repack(const void* codes, const void* scales, int64_t E, int64_t N, 
 int awq_mx4_unrepack(const void* w, const void* s, int64_t E, int64_t N, int64_t K, void* codes, void* scales,
                      awq_stream_t stream);
 int64_t awq_mx4_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation);
+/* What awq_mx4_gemm launches for this shape on the current device, written to
+ * info[0..5]: kernel (0 mx4_rows_kernel, 1 mx4_tile_kernel), rows and columns
+ * of W of a workgroup at most, workgroups, whether a launch ahead quantises the
+ * rows, and the workspace bytes. */
+int awq_mx4_plan_info(int64_t M, int64_t N, int64_t K, int activation, int64_t* info);
 int awq_mx4_gemm(const void* x, const void* w, const void* s, const void* bias, void* out, int64_t M, int64_t N,
                  int64_t K, int dtype, int activation, void* ws, int64_t ws_bytes, awq_stream_t stream);
 int64_t awq_mx4_moe_workspace_bytes(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, int64_t K,

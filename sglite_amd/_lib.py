@@ -83,6 +83,7 @@ SIGNATURES = {
     "awq_mx4_repack": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "awq_mx4_unrepack": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp]),
     "awq_mx4_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "awq_mx4_plan_info": (_int, [_i64, _i64, _i64, _int, ctypes.POINTER(_i64)]),
     "awq_mx4_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp, _i64, _vp]),
     "awq_mx4_moe_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),
     "awq_mx4_moe_gemm": (_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _int, _vp, _i64, _vp, _vp, _i64, _i64, _int,

@@ -978,6 +978,23 @@ int64_t awq_mx4_workspace_bytes(int64_t M, int64_t N, int64_t K, int activation)
   return M == 0 ? 0 : plan_mx4(M, N, K, activation).ws_bytes;
 }
 
+int awq_mx4_plan_info(int64_t M, int64_t N, int64_t K, int activation, int64_t* info) {
+  int st = check_mx4_weight(N, K, activation, "awq_mx4_plan_info");
+  if (st != 0) return st;
+  if (M <= 0) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_plan_info: M must be positive");
+  if (!info) return fail(AWQ_STATUS_INVALID_ARGUMENT, "awq_mx4_plan_info: null pointer argument");
+  st = check_mx4_rows(M, K, "awq_mx4_plan_info");
+  if (st != 0) return st;
+  const Mx4Plan p = plan_mx4(M, N, K, activation);
+  info[0] = p.tile ? 1 : 0;
+  info[1] = p.tile ? kMx4TileRows : 16 * p.mt;
+  info[2] = p.tile ? 64 * p.ntw : 16 * p.ntw;
+  info[3] = p.grid;
+  info[4] = p.pre ? 1 : 0;
+  info[5] = p.ws_bytes;
+  return ok();
+}
+
 int awq_mx4_gemm(const void* x, const void* w, const void* s, const void* bias, void* out, int64_t M, int64_t N,
                  int64_t K, int dtype, int activation, void* ws, int64_t ws_bytes, awq_stream_t stream) {
   const TraceRange range("awq_mx4_gemm");

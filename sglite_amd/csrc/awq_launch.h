@@ -186,6 +186,7 @@ hipError_t launch_mx4_dequantize(const void* codes, const void* scales, int64_t 
 hipError_t launch_mx4_repack(void* codes, void* scales, void* w, void* ws, int64_t E, int64_t N, int64_t K, bool back,
                              hipStream_t s);
 constexpr int64_t kMx4MaxGrid = 1 << 22;  // workgroups of up to 1024 threads
+constexpr int kMx4TileRows = 128;         // rows of a tile's workgroup, at most
 struct Mx4Plan {
   bool pre;            // the rows are quantised by a launch of their own
   bool tile;           // by tiles of many rows

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(64 * kMxRowsWaves) void mx4_expert_rows_kernel(MxAr
 // rows go through LDS stages of 512 k by LDS-DMA, in the order of the MFMA
 // operands; a wave's weights are its own (NTW column tiles) and go straight to
 // registers.
-constexpr int kMxTileM = 128;
+constexpr int kMxTileM = kMx4TileRows;
 constexpr int kMxTileGrain = 32;  // a tile's rows come in multiples of two m-tiles
 constexpr int kMxCodes = 4 * (kMxTileM / 16) * 64;      // 16-byte vectors of a stage's codes
 constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 bytes a row

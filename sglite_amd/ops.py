@@ -1371,6 +1371,25 @@ def _mx4_workspace_bytes(M: int, N: int, K: int, act: int) -> int:
     return _lib.check(_lib.load().awq_mx4_workspace_bytes(M, N, K, act), "awq_mx4_workspace_bytes")
 
 
+class Mx4PlanInfo(NamedTuple):
+    kernel: str             # the function of the product's launch
+    rows: int               # of a workgroup, at most
+    columns: int            # of W, of a workgroup
+    workgroups: int
+    quantised_ahead: bool   # by a launch of its own
+    workspace_bytes: int
+
+
+def mx4_plan_info(M: int, N: int, K: int, activation: Optional[str] = None) -> Mx4PlanInfo:
+    """What ``mx4_gemm`` launches for this shape on the current device."""
+    if activation not in _ACT_CODE:
+        raise ValueError(f"unsupported activation {activation!r}")
+    info = (ctypes.c_int64 * 6)()
+    _lib.check(_lib.load().awq_mx4_plan_info(M, N, K, _ACT_CODE[activation], info), "awq_mx4_plan_info")
+    return Mx4PlanInfo(("mx4_rows_kernel", "mx4_tile_kernel")[info[0]], int(info[1]), int(info[2]), int(info[3]),
+                       bool(info[4]), int(info[5]))
+
+
 def _mx4_gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, bias: Optional[torch.Tensor],
                      out: torch.Tensor, N: int, K: int, act: int) -> None:
     M = x.shape[0]
