@@ -49,6 +49,22 @@ def _concat_prefix(prefix: str, name: str) -> str:
     return f"{prefix}.{name}" if prefix else name
 
 
+def _checked(params: Dict[str, torch.Tensor], state_dict: Dict[str, torch.Tensor],
+             prefix: str) -> Dict[str, torch.Tensor]:
+    """The tensors of ``state_dict`` that ``params`` names, of their shapes and dtypes; nothing is removed from it."""
+    items = {}
+    for name, param in params.items():
+        key = _concat_prefix(prefix, name)
+        if key not in state_dict:
+            raise KeyError(key)
+        item = state_dict[key]
+        assert isinstance(item, torch.Tensor)
+        assert param.shape == item.shape and param.dtype == item.dtype, (
+            f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
+        items[name] = item
+    return items
+
+
 class AWQExpertStack:
     """One projection's expert-stacked AWQ tensors: [E, K, N/8], [E, K/G, N/8], [E, K/G, N]."""
 
@@ -83,17 +99,7 @@ class AWQExpertStack:
     def take(self, state_dict: Dict[str, torch.Tensor], prefix: str = "") -> Dict[str, torch.Tensor]:
         """This stack's three tensors from ``state_dict``, checked against the expected
         shapes and dtypes; nothing is removed from ``state_dict``."""
-        items = {}
-        for name in _AWQ_NAMES:
-            key = _concat_prefix(prefix, name)
-            if key not in state_dict:
-                raise KeyError(key)
-            param, item = getattr(self, name), state_dict[key]
-            assert isinstance(item, torch.Tensor)
-            assert param.shape == item.shape and param.dtype == item.dtype, (
-                f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
-            items[name] = item
-        return items
+        return _checked({name: getattr(self, name) for name in _AWQ_NAMES}, state_dict, prefix)
 
     def process(self, items: Dict[str, torch.Tensor]) -> None:
         """Post-load repack of checked tensors into the tile layout (on their device)."""
@@ -224,16 +230,10 @@ class MoELayer(_MoEBlock):
 
     def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
                         _internal: bool = False) -> None:
-        keys = {name: _concat_prefix(prefix, name) for name in _DENSE_NAMES}
-        for name, key in keys.items():  # check everything before any change
-            if key not in state_dict:
-                raise KeyError(key)
-            param, item = getattr(self, name), state_dict[key]
-            assert isinstance(item, torch.Tensor)
-            assert param.shape == item.shape and param.dtype == item.dtype, (
-                f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
-        for name, key in keys.items():
-            setattr(self, name, ops._aligned(state_dict.pop(key)))
+        items = _checked({name: getattr(self, name) for name in _DENSE_NAMES}, state_dict, prefix)
+        for name, item in items.items():  # everything is checked before any change
+            del state_dict[_concat_prefix(prefix, name)]
+            setattr(self, name, ops._aligned(item))
         if not _internal and state_dict:
             raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
 
@@ -288,20 +288,12 @@ class MXFP4MoELayer(_MoEBlock):
 
     def load_state_dict(self, state_dict: Dict[str, torch.Tensor], *, prefix: str = "",
                         _internal: bool = False) -> None:
-        items = {}
-        for name, param in self._params.items():  # check everything before any change
-            key = _concat_prefix(prefix, name)
-            if key not in state_dict:
-                raise KeyError(key)
-            item = state_dict[key]
-            assert isinstance(item, torch.Tensor)
-            assert param.shape == item.shape and param.dtype == item.dtype, (
-                f"{key}: expected {tuple(param.shape)} {param.dtype}, got {tuple(item.shape)} {item.dtype}")
-            items[name] = item
-        for name in self._params:
-            state_dict.pop(_concat_prefix(prefix, name))
-        self._experts = (process_mxfp4_moe_weights(items["gate_up_proj"], items.get("gate_up_proj.weight_scale")),
-                         process_mxfp4_moe_weights(items["down_proj"], items.get("down_proj.weight_scale")))
+        items = _checked(self._params, state_dict, prefix)
+        experts = (process_mxfp4_moe_weights(items["gate_up_proj"], items.get("gate_up_proj.weight_scale")),
+                   process_mxfp4_moe_weights(items["down_proj"], items.get("down_proj.weight_scale")))
+        for name in self._params:  # only now: the device's part may refuse them too
+            del state_dict[_concat_prefix(prefix, name)]
+        self._experts = experts
         if not _internal and state_dict:
             raise RuntimeError(f"Unexpected keys in state_dict: {list(state_dict.keys())}")
 
