@@ -130,7 +130,24 @@ def _check_awq_shapes(qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch
     if qzeros.shape[1] != N8 or tuple(scales.shape) != (ng, N):
         raise ValueError(f"inconsistent AWQ shapes: qweight {tuple(qweight.shape)}, qzeros {tuple(qzeros.shape)}, "
                          f"scales {tuple(scales.shape)}")
+    if qzeros.device != qweight.device or scales.device != qweight.device:
+        raise ValueError("qweight, qzeros and scales must be on one device")
     return K, N, G
+
+
+def _check_repacked(w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, K: int, N: int, G: int) -> None:
+    """That these tensors hold the tile layout of [K, N] in groups of G, which the kernels read to its end."""
+    if K < 1 or N < 1 or G < 1 or K % G:
+        raise ValueError(f"K and N must be positive and the group size a divisor of K, got {K}, {N} and {G}")
+    dtype_code(s.dtype)
+    NT, NG = (N + 15) // 16, K // G
+    for t, dtype, n in ((w, torch.int32, NT * ((K + 127) // 128) * 256), (s, s.dtype, NT * NG * 16),
+                        (z, torch.int64, NT * NG)):
+        if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"the repacked tensors of [{K}, {N}] in groups of {G} must be contiguous, here {n} of "
+                             f"{dtype}, got {t.numel()} of {t.dtype}")
+        if t.device != w.device:
+            raise ValueError("the repacked tensors must be on one device")
 
 
 # ---------------------------------------------------------------------------
@@ -169,6 +186,7 @@ def _(qweight, qzeros, scales):
 @torch.library.custom_op(f"{NAMESPACE}::awq_unrepack_cdna4", mutates_args=(), device_types="cuda")
 def _unrepack_op(w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, K: int, N: int,
                  G: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_repacked(w, s, z, K, N, G)
     dev = w.device
     qweight = torch.empty((K, N // 8), dtype=torch.int32, device=dev)
     qzeros = torch.empty((K // G, N // 8), dtype=torch.int32, device=dev)
@@ -203,6 +221,7 @@ def _(qweight, qzeros, scales):
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_dequant_repacked", mutates_args=(), device_types="cuda")
 def _dequant_repacked_op(w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, K: int, N: int, G: int) -> torch.Tensor:
+    _check_repacked(w, s, z, K, N, G)
     out = torch.empty((K, N), dtype=s.dtype, device=w.device)
     with _on_device(w.device):
         _lib.check(_lib.load().awq_dequant_repacked(w.data_ptr(), s.data_ptr(), z.data_ptr(), dtype_code(s.dtype), K,
@@ -430,12 +449,43 @@ def _gemm_launch(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Ten
                                           _ptr(counters), cb, _stream(dev)), "awq_w4a16_gemm_act")
 
 
+def _gemm_op_checked(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor,
+                     bias: Optional[torch.Tensor], counters: Optional[torch.Tensor], out: Optional[torch.Tensor],
+                     K: int, N: int, G: int, activation: Optional[str] = None) -> torch.Tensor:
+    """A registered product: all that the kernels read and write is checked, as ``gemm`` checks it."""
+    _check_gemm_op(x, w, s, z, bias, counters, out, K, N, G, activation)
+    if out is None:
+        out = torch.empty((x.shape[0], N if activation is None else N // 2), dtype=x.dtype, device=x.device)
+    _gemm_launch(_aligned(x), w, s, z, None if bias is None else _aligned(bias, 8), counters, out, K, N, G,
+                 0 if activation is None else _GATED_ACT[activation])
+    return out
+
+
+def _check_gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, bias: Optional[torch.Tensor],
+                   counters: Optional[torch.Tensor], out: Optional[torch.Tensor], K: int, N: int, G: int,
+                   activation: Optional[str]) -> None:
+    _check_repacked(w, s, z, K, N, G)
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be [M, {K}], got {tuple(x.shape)}")
+    if x.dtype != s.dtype:
+        raise ValueError(f"activation dtype {x.dtype} does not match the scale dtype {s.dtype}")
+    if w.device != x.device:
+        raise ValueError("x and the repacked weights must be on one device")
+    if activation is not None and activation not in _GATED_ACT:
+        raise ValueError(f"unsupported activation {activation!r}")
+    if bias is not None and (bias.numel() != N or bias.dtype != x.dtype or bias.device != x.device):
+        raise ValueError(f"bias must be {N} elements of x's type and device, got {bias.numel()} of {bias.dtype}")
+    if counters is not None and (counters.dtype != torch.int32 or counters.device != x.device
+                                 or not counters.is_contiguous()):  # how many the C ABI knows
+        raise ValueError(f"counters must be contiguous int32 on {x.device}")
+    if out is not None:
+        _check_out(out, (x.shape[0], N if activation is None else N // 2), x.dtype, x.device)
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_w4a16_gemm", mutates_args=("counters",), device_types="cuda")
 def _gemm_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, bias: Optional[torch.Tensor],
              counters: Optional[torch.Tensor], K: int, N: int, G: int) -> torch.Tensor:
-    out = torch.empty((x.shape[0], N), dtype=x.dtype, device=x.device)
-    _gemm_launch(x, w, s, z, bias, counters, out, K, N, G, 0)
-    return out
+    return _gemm_op_checked(x, w, s, z, bias, counters, None, K, N, G)
 
 
 @_gemm_op.register_fake
@@ -446,7 +496,7 @@ def _(x, w, s, z, bias, counters, K, N, G):
 @torch.library.custom_op(f"{NAMESPACE}::awq_w4a16_gemm_out", mutates_args=("counters", "out"), device_types="cuda")
 def _gemm_out_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, bias: Optional[torch.Tensor],
                  counters: Optional[torch.Tensor], out: torch.Tensor, K: int, N: int, G: int) -> None:
-    _gemm_launch(x, w, s, z, bias, counters, out, K, N, G, 0)
+    _gemm_op_checked(x, w, s, z, bias, counters, out, K, N, G)
 
 
 @_gemm_out_op.register_fake
@@ -457,9 +507,7 @@ def _(x, w, s, z, bias, counters, out, K, N, G):
 @torch.library.custom_op(f"{NAMESPACE}::awq_w4a16_gemm_act", mutates_args=("counters",), device_types="cuda")
 def _gemm_act_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, bias: Optional[torch.Tensor],
                  counters: Optional[torch.Tensor], K: int, N: int, G: int, activation: str) -> torch.Tensor:
-    out = torch.empty((x.shape[0], N // 2), dtype=x.dtype, device=x.device)
-    _gemm_launch(x, w, s, z, bias, counters, out, K, N, G, _GATED_ACT[activation])
-    return out
+    return _gemm_op_checked(x, w, s, z, bias, counters, None, K, N, G, activation)
 
 
 @_gemm_act_op.register_fake
@@ -472,7 +520,7 @@ def _(x, w, s, z, bias, counters, K, N, G, activation):
 def _gemm_act_out_op(x: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, bias: Optional[torch.Tensor],
                      counters: Optional[torch.Tensor], out: torch.Tensor, K: int, N: int, G: int,
                      activation: str) -> None:
-    _gemm_launch(x, w, s, z, bias, counters, out, K, N, G, _GATED_ACT[activation])
+    _gemm_op_checked(x, w, s, z, bias, counters, out, K, N, G, activation)
 
 
 @_gemm_act_out_op.register_fake
@@ -564,8 +612,9 @@ def gemm(x: torch.Tensor, r: Repacked, K: int, N: int, group_size: int, bias: Op
     ncols = N if activation is None else N // 2
     if out is not None:
         _check_out(out, (M, ncols), x.dtype, dev)
-    if out is None and _undispatched(x, r.w, r.s, r.z, bias, counters):
-        out = torch.empty((M, ncols), dtype=x.dtype, device=dev)
+    if _undispatched(x, r.w, r.s, r.z, bias, counters, out):
+        if out is None:
+            out = torch.empty((M, ncols), dtype=x.dtype, device=dev)
         _gemm_launch(x, r.w, r.s, r.z, bias, counters, out, K, N, G, 0 if activation is None else _GATED_ACT[activation])
         return out
     if activation is None:
