@@ -838,11 +838,23 @@ def expert_strides(K: int, N: int, group_size: int) -> Tuple[int, int, int]:
     return w.value, s.value, z.value
 
 
+_expert_stride_bytes = functools.lru_cache(maxsize=4096)(expert_strides)
+
+
+def _check_expert_stacks(qweight: torch.Tensor, qzeros: torch.Tensor,
+                         scales: torch.Tensor) -> Tuple[int, int, int, int]:
+    if qweight.dim() != 3 or qzeros.dim() != 3 or scales.dim() != 3:
+        raise ValueError("expert stacks must be 3-D [E, ...]")
+    E = qweight.shape[0]
+    if qzeros.shape[0] != E or scales.shape[0] != E:
+        raise ValueError("qweight, qzeros and scales must stack the same number of experts")
+    return (E, *_check_awq_shapes(qweight[0], qzeros[0], scales[0]))
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_repack_experts", mutates_args=(), device_types="cuda")
 def _repack_experts_op(qweight: torch.Tensor, qzeros: torch.Tensor,
                        scales: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    E = qweight.shape[0]
-    K, N, G = _check_awq_shapes(qweight[0], qzeros[0], scales[0])
+    E, K, N, G = _check_expert_stacks(qweight, qzeros, scales)
     code = dtype_code(scales.dtype)
     ws, ss, zs = expert_strides(K, N, G)
     dev = qweight.device
@@ -878,12 +890,7 @@ def repack_experts(qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Te
     Each expert is repacked into its own row of the stacks (the layout
     ``awq_moe_w4a16_gemm`` expects)."""
     _require_cuda(qweight, qzeros, scales)
-    if qweight.dim() != 3 or qzeros.dim() != 3 or scales.dim() != 3:
-        raise ValueError("expert stacks must be 3-D [E, ...]")
-    E = qweight.shape[0]
-    if qzeros.shape[0] != E or scales.shape[0] != E:
-        raise ValueError("qweight, qzeros and scales must stack the same number of experts")
-    K, N, G = _check_awq_shapes(qweight[0], qzeros[0], scales[0])
+    _, K, N, G = _check_expert_stacks(qweight, qzeros, scales)
     dtype_code(scales.dtype)
     w, s, z = torch.ops.sglite_awq.awq_repack_experts(qweight, qzeros, scales)
     return RepackedExperts(w, s, z, K, N, G)
@@ -934,6 +941,8 @@ def _align_caps(n: int, num_experts: int, block_size: int) -> Tuple[int, int]:
 @torch.library.custom_op(f"{NAMESPACE}::awq_moe_align_block_size", mutates_args=(), device_types="cuda")
 def _align_op(topk_ids: torch.Tensor, block_size: int,
               num_experts: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    if topk_ids.dtype != torch.int32:
+        raise ValueError("topk_ids must be int32")
     ids = topk_ids.contiguous().reshape(-1)
     n = ids.numel()
     cap, bcap = _align_caps(n, num_experts, block_size)
@@ -1015,17 +1024,69 @@ _ACT_CODE = {None: _lib.AWQ_MOE_ACT_NONE, "silu": _lib.AWQ_MOE_ACT_SILU, "gelu":
 _ACT_NAME = {"none": None, "silu": "silu", "gelu": "gelu"}
 
 
+def _check_routed_op(a: torch.Tensor, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
+                     topk_weights: Optional[torch.Tensor], out: torch.Tensor, E: int, N: int, K: int, num_routed: int,
+                     top_k: int, activation: str, mul_routed_weight: bool) -> int:
+    """What every registered grouped product reads and writes beside its weights; the activation's code."""
+    if activation not in _ACT_NAME:
+        raise ValueError(f"unsupported activation {activation!r}")
+    if a.dim() != 2 or a.shape[1] != K:
+        raise ValueError(f"a must be [rows, {K}], got {tuple(a.shape)}")
+    if mul_routed_weight and topk_weights is None:
+        raise ValueError("mul_routed_weight needs topk_weights")
+    if num_routed < 0 or top_k < 1:
+        raise ValueError(f"num_routed must be at least 0 and top_k at least 1, got {num_routed} and {top_k}")
+    if expert_offsets.numel() != E + 1:
+        raise ValueError(f"the rows were aligned for {expert_offsets.numel() - 1} experts, the stack holds {E}")
+    if sorted_ids.dtype != torch.int32 or expert_offsets.dtype != torch.int32 \
+            or not sorted_ids.is_contiguous() or not expert_offsets.is_contiguous():
+        raise ValueError("the alignment must be moe_align_block_size's: contiguous int32")
+    if topk_weights is not None and (topk_weights.dtype != torch.float32 or topk_weights.numel() < num_routed):
+        raise ValueError(f"topk_weights must hold {num_routed} routed weights in float32, got "
+                         f"{topk_weights.numel()} of {topk_weights.dtype}")
+    for t in (sorted_ids, expert_offsets, topk_weights):
+        if t is not None and t.device != a.device:
+            raise ValueError("a, the experts, the weights and the alignment must be on one device")
+    _check_out(out, (num_routed, N if activation == "none" else N // 2), a.dtype, a.device)
+    return _ACT_CODE[_ACT_NAME[activation]]
+
+
+def _check_moe_gemm_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, sorted_ids: torch.Tensor,
+                       expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, K: int,
+                       N: int, G: int, num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> int:
+    if w.dim() != 2 or w.shape[0] < 1:
+        raise ValueError(f"the repacked experts must be stacked [E, ...], got {tuple(w.shape)}")
+    E = w.shape[0]
+    for t, dtype, nbytes in zip((w, s, z), (torch.int32, a.dtype, torch.int64), _expert_stride_bytes(K, N, G)):
+        if t.dtype != dtype or tuple(t.shape) != (E, nbytes // t.element_size()) or not t.is_contiguous():
+            raise ValueError(f"the repacked experts of [{K}, {N}] in groups of {G} must be contiguous "
+                             f"[{E}, {nbytes} bytes] of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+        if t.device != a.device:
+            raise ValueError("a, the experts, the weights and the alignment must be on one device")
+    return _check_routed_op(a, sorted_ids, expert_offsets, topk_weights, out, E, N, K, num_routed, top_k, activation,
+                            mul_routed_weight)
+
+
+def _moe_gemm_launch(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, sorted_ids: torch.Tensor,
+                     expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, K: int,
+                     N: int, G: int, num_routed: int, top_k: int, act: int, mul_routed_weight: bool) -> None:
+    with _on_device(a.device):
+        _lib.check(_lib.load().awq_moe_w4a16_gemm(
+            a.data_ptr(), a.shape[0], w.data_ptr(), s.data_ptr(), z.data_ptr(), w.shape[0], N, K, G,
+            dtype_code(a.dtype), sorted_ids.data_ptr(), sorted_ids.numel(), expert_offsets.data_ptr(),
+            _ptr(topk_weights), num_routed, top_k, act, 1 if mul_routed_weight else 0, out.data_ptr(),
+            _stream(a.device)), "awq_moe_w4a16_gemm")
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_moe_w4a16_gemm", mutates_args=("out",), device_types="cuda")
 def _moe_gemm_op(a: torch.Tensor, w: torch.Tensor, s: torch.Tensor, z: torch.Tensor, sorted_ids: torch.Tensor,
                  expert_offsets: torch.Tensor, topk_weights: Optional[torch.Tensor], out: torch.Tensor, K: int, N: int,
                  G: int, num_routed: int, top_k: int, activation: str, mul_routed_weight: bool) -> None:
-    E = w.shape[0]
-    with _on_device(a.device):
-        _lib.check(_lib.load().awq_moe_w4a16_gemm(
-            a.data_ptr(), a.shape[0], w.data_ptr(), s.data_ptr(), z.data_ptr(), E, N, K, G, dtype_code(a.dtype),
-            sorted_ids.data_ptr(), sorted_ids.numel(), expert_offsets.data_ptr(), _ptr(topk_weights), num_routed,
-            top_k, _ACT_CODE[_ACT_NAME[activation]], 1 if mul_routed_weight else 0, out.data_ptr(),
-            _stream(a.device)), "awq_moe_w4a16_gemm")
+    act = _check_moe_gemm_op(a, w, s, z, sorted_ids, expert_offsets, topk_weights, out, K, N, G, num_routed, top_k,
+                             activation, mul_routed_weight)
+    topk_weights = None if topk_weights is None else _aligned(topk_weights, 4)
+    _moe_gemm_launch(_aligned(a), w, s, z, sorted_ids, expert_offsets, topk_weights, out, K, N, G, num_routed, top_k,
+                     act, mul_routed_weight)
 
 
 @_moe_gemm_op.register_fake
@@ -1061,9 +1122,13 @@ def moe_gemm(a: torch.Tensor, experts: RepackedExperts, K: int, N: int, group_si
         topk_weights = _aligned(topk_weights.float().reshape(-1), 4)
         if topk_weights.numel() < num_routed:
             raise ValueError(f"topk_weights must hold {num_routed} routed weights, got {topk_weights.numel()}")
-    torch.ops.sglite_awq.awq_moe_w4a16_gemm(a, experts.w, experts.s, experts.z, align.sorted_ids, align.expert_offsets,
-                                            topk_weights, out, K, N, G, num_routed, top_k,
-                                            "none" if activation is None else activation, bool(mul_routed_weight))
+    args = (a, experts.w, experts.s, experts.z, align.sorted_ids, align.expert_offsets, topk_weights, out, K, N, G,
+            num_routed, top_k, "none" if activation is None else activation, bool(mul_routed_weight))
+    if _undispatched(*args[:8]):
+        act = _check_moe_gemm_op(*args)
+        _moe_gemm_launch(*args[:13], act, args[14])
+    else:
+        torch.ops.sglite_awq.awq_moe_w4a16_gemm(*args)
     return out
 
 
@@ -1082,12 +1147,29 @@ def _moe_dense_launch(a: torch.Tensor, w: torch.Tensor, sorted_ids: torch.Tensor
         1 if mul_routed_weight else 0, out.data_ptr(), _stream(dev)), "awq_moe_dense_gemm")
 
 
+def _check_moe_dense_op(a: torch.Tensor, w: torch.Tensor, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
+                        topk_weights: Optional[torch.Tensor], out: torch.Tensor, num_routed: int, top_k: int,
+                        activation: str, mul_routed_weight: bool) -> int:
+    if w.dim() != 3 or not w.is_contiguous():
+        raise ValueError(f"w must be contiguous [E, N, K], got {tuple(w.shape)}")
+    if a.dtype != w.dtype or a.device != w.device:
+        raise ValueError("a and w must share a type and a device")
+    act = _check_routed_op(a, sorted_ids, expert_offsets, topk_weights, out, *w.shape, num_routed, top_k, activation,
+                           mul_routed_weight)
+    if _overlap(out, a) or _overlap(out, w):
+        raise ValueError("out must not share memory with a or w")
+    return act
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_moe_dense_gemm", mutates_args=("out",), device_types="cuda")
 def _moe_dense_op(a: torch.Tensor, w: torch.Tensor, sorted_ids: torch.Tensor, expert_offsets: torch.Tensor,
                   topk_weights: Optional[torch.Tensor], out: torch.Tensor, num_routed: int, top_k: int,
                   activation: str, mul_routed_weight: bool) -> None:
-    _moe_dense_launch(a, w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k,
-                      _ACT_CODE[_ACT_NAME[activation]], mul_routed_weight)
+    act = _check_moe_dense_op(a, w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k, activation,
+                              mul_routed_weight)
+    topk_weights = None if topk_weights is None else _aligned(topk_weights, 4)
+    _moe_dense_launch(_aligned(a), w, sorted_ids, expert_offsets, topk_weights, out, num_routed, top_k, act,
+                      mul_routed_weight)
 
 
 @_moe_dense_op.register_fake
@@ -1152,8 +1234,24 @@ def moe_dense_gemm(a: torch.Tensor, w: torch.Tensor, align: MoeAlignment, topk_w
     return out
 
 
+def _check_moe_sum(inp: torch.Tensor, out: torch.Tensor) -> None:
+    if inp.dim() != 3 or out.dim() != 2 or out.shape[0] != inp.shape[0] or out.shape[1] != inp.shape[2]:
+        raise ValueError(f"shapes do not match: in {tuple(inp.shape)}, out {tuple(out.shape)}")
+    if inp.dtype != out.dtype:
+        raise ValueError("in and out must share a dtype")
+    if not (inp.is_contiguous() and out.is_contiguous()):
+        raise ValueError("in and out must be contiguous")
+    if inp.device != out.device:
+        raise ValueError("in and out must be on one device")
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_moe_sum_reduce", mutates_args=("out",), device_types="cuda")
 def _moe_sum_op(inp: torch.Tensor, out: torch.Tensor) -> None:
+    _check_moe_sum(inp, out)
+    _moe_sum_launch(inp, out)
+
+
+def _moe_sum_launch(inp: torch.Tensor, out: torch.Tensor) -> None:
     T, k, H = inp.shape
     with _on_device(inp.device):
         _lib.check(_lib.load().awq_moe_sum_reduce(inp.data_ptr(), out.data_ptr(), T, k, H, dtype_code(inp.dtype),
@@ -1168,12 +1266,10 @@ def _(inp, out):
 def moe_sum_reduce(inp: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     """out[t] = rnd(sum_j inp[t, j]) with an fp32 sum (inp [T, k, H], out [T, H])."""
     _require_cuda(inp, out)
-    if inp.dim() != 3 or out.dim() != 2 or out.shape[0] != inp.shape[0] or out.shape[1] != inp.shape[2]:
-        raise ValueError(f"shapes do not match: in {tuple(inp.shape)}, out {tuple(out.shape)}")
-    if inp.dtype != out.dtype:
-        raise ValueError("in and out must share a dtype")
-    if not (inp.is_contiguous() and out.is_contiguous()):
-        raise ValueError("in and out must be contiguous")
+    _check_moe_sum(inp, out)
+    if _undispatched(inp, out):
+        _moe_sum_launch(inp, out)
+        return out
     torch.ops.sglite_awq.awq_moe_sum_reduce(inp, out)
     return out
 

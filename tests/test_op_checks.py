@@ -81,12 +81,112 @@ def test_checkpoint_tensors_lie_on_one_device():
             ops._check_awq_shapes(*bad)
 
 
+E, TOP_K, ROWS = 4, 2, 2 * M
+
+
+def routed(dev, cols):
+    empty = zeros(dev)
+    return dict(a=empty(M, K), sorted_ids=torch.full((ROWS + 15 * E,), ROWS, dtype=I32, device=dev),
+                expert_offsets=empty(E + 1, dtype=I32), topk_weights=empty(ROWS, dtype=torch.float32),
+                out=empty(ROWS, cols), num_routed=ROWS, top_k=TOP_K, activation="none", mul_routed_weight=True)
+
+
+def bad_routed(ok, dev, cols):
+    empty, other, ids, offsets = zeros(dev), OTHER[dev], ok["sorted_ids"], ok["expert_offsets"]
+    return [dict(a=empty(M, K - 8)), dict(a=empty(K)), dict(a=empty(M, K, dtype=torch.bfloat16)),
+            dict(sorted_ids=ids.long()), dict(sorted_ids=ids.repeat(2)[::2]), dict(sorted_ids=ids.to(other)),
+            dict(expert_offsets=offsets[:-1]), dict(expert_offsets=empty(E + 2, dtype=I32)),
+            dict(expert_offsets=offsets.long()), dict(expert_offsets=offsets.to(other)), dict(topk_weights=None),
+            dict(topk_weights=ok["topk_weights"][:-1]), dict(topk_weights=empty(ROWS)),
+            dict(topk_weights=ok["topk_weights"].to(other)), dict(out=empty(ROWS - 1, cols)), dict(out=empty(ROWS, cols + 8)),
+            dict(out=empty(ROWS, 2 * cols)[:, ::2]), dict(out=empty(ROWS, cols, dtype=torch.float32)),
+            dict(out=ok["out"].to(other)), dict(activation="silu"), dict(activation="relu"), dict(num_routed=-1),
+            dict(num_routed=ROWS + 1), dict(top_k=0)]
+
+
+def grouped(name, dev):
+    empty, other = zeros(dev), OTHER[dev]
+    ok = routed(dev, N)
+    bad = bad_routed(ok, dev, N)
+    if name == "awq_moe_dense_gemm":
+        w = empty(E, N, K)
+        ok["w"] = w
+        return ok, bad + [dict(w=w[0]), dict(w=w[:, :, :-8]), dict(w=empty(E, K, N).transpose(1, 2)), dict(w=w.bfloat16()),
+                          dict(w=empty(E + 1, N, K)), dict(w=empty(E, N + 8, K)), dict(w=w.to(other))]
+    ws, ss, zs = ops.expert_strides(K, N, G)
+    ok.update(w=empty(E, ws // 4, dtype=I32), s=empty(E, ss // 2), z=empty(E, zs // 8, dtype=I64), K=K, N=N, G=G)
+    return ok, bad + [dict(w=ok["w"][:-1]), dict(w=ok["w"].long()), dict(w=ok["w"][0]), dict(s=ok["s"][:, :-8]),
+                      dict(s=ok["s"].bfloat16()), dict(s=ok["s"][:-1]), dict(z=ok["z"][:, :-1]), dict(z=ok["z"].int()),
+                      dict(z=ok["z"].to(other)), dict(N=2 * N), dict(K=2 * K), dict(G=64), dict(G=48), dict(K=0),
+                      dict(N=0), dict(G=0)]
+
+
+GROUPED = {"awq_moe_w4a16_gemm": ops._check_moe_gemm_op, "awq_moe_dense_gemm": ops._check_moe_dense_op}
+
+
+@pytest.mark.parametrize("name", GROUPED)
+def test_grouped_checks(name):
+    ok, bad = grouped(name, "cpu")
+    GROUPED[name](**ok)
+    for change in bad:
+        with pytest.raises(ValueError):
+            GROUPED[name](**{**ok, **change})
+
+
+def test_sum_and_stack_checks():
+    one, out = torch.zeros(M, 2, 64).half(), torch.zeros(M, 64).half()
+    ops._check_moe_sum(one, out)
+    for bad in ((one[0], out), (one, out[:-1]), (one, out[:, :32]), (one, out.float()), (one[:, :, ::2], out[:, ::2]),
+                (one, out.to("meta"))):
+        with pytest.raises(ValueError):
+            ops._check_moe_sum(*bad)
+    q, z, s = torch.zeros(E, K, N // 8, dtype=I32), torch.zeros(E, K // G, N // 8, dtype=I32), torch.ones(E, K // G, N).half()
+    assert ops._check_expert_stacks(q, z, s) == (E, K, N, G)
+    for bad in ((q[0], z[0], s[0]), (q, z[1:], s), (q, z, s[1:]), (q, z.to("meta"), s), (q, z, s[:, :1])):
+        with pytest.raises(ValueError):
+            ops._check_expert_stacks(*bad)
+
+
 def refused_by_the_op(name, ok, bad):
     getattr(OPS, name)(**ok)
     for change in bad:
         with pytest.raises(ValueError):
             getattr(OPS, name)(**{**ok, **change})
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", GROUPED)
+def test_grouped_ops(name):
+    refused_by_the_op(name, *grouped(name, "cuda"))
+
+
+@pytest.mark.gpu
+def test_other_moe_ops():
+    one, out = torch.ones((M, 2, 64), device="cuda").half(), torch.zeros((M, 64), device="cuda").half()
+    OPS.awq_moe_sum_reduce(one, out)
+    assert (out == 2).all()
+    with pytest.raises(ValueError):
+        OPS.awq_moe_sum_reduce(one, out[:-1])
+    with pytest.raises(ValueError, match="int32"):
+        OPS.awq_moe_align_block_size(torch.zeros((M, 2), dtype=I64, device="cuda"), 16, E)
+
+
+@pytest.mark.gpu
+def test_moe_gemm_checks_its_alignment():
+    """The Python call too: an alignment for other experts or of another type is refused."""
+    ok, _ = grouped("awq_moe_w4a16_gemm", "cuda")
+    ex = ops.RepackedExperts(ok["w"], ok["s"], ok["z"], K, N, G)
+    al = ops.moe_align_block_size(torch.zeros((M, TOP_K), dtype=I32, device="cuda"), 16, E)
+
+    def call(align, n=N):
+        return ops.moe_gemm(ok["a"], ex, K, n, G, align, ok["topk_weights"], ROWS, TOP_K)
+    assert call(al).shape == (ROWS, N)
+    for bad in (al._replace(expert_offsets=al.expert_offsets[:-1]), al._replace(sorted_ids=al.sorted_ids.long())):
+        with pytest.raises(ValueError):
+            call(bad)
+    with pytest.raises(ValueError):
+        call(al, 2 * N)
 
 
 @pytest.mark.gpu
