@@ -740,11 +740,36 @@ def _mlp_launch(x: torch.Tensor, gw: torch.Tensor, gs: torch.Tensor, gz: torch.T
                                      counters.numel() * 4, _stream(dev)), "awq_gated_mlp")
 
 
+def _check_mlp_counters(counters: torch.Tensor, device: torch.device) -> None:
+    if counters.dtype != torch.int32 or counters.device != device or not counters.is_contiguous() \
+            or counters.numel() * 4 < _lib.AWQ_MLP_COUNTER_BYTES or counters.data_ptr() % 128:
+        raise ValueError("counters must be make_mlp_counters(device)")
+
+
+def _check_mlp_op(x: torch.Tensor, gw: torch.Tensor, gs: torch.Tensor, gz: torch.Tensor, dw: torch.Tensor,
+                  ds: torch.Tensor, dz: torch.Tensor, counters: torch.Tensor, out: torch.Tensor, H: int, I: int, G: int,
+                  activation: str) -> None:
+    """All that the registered op reads and writes."""
+    _check_repacked(gw, gs, gz, H, 2 * I, G)
+    _check_repacked(dw, ds, dz, I, H, G)
+    if x.dim() != 2 or x.shape[1] != H:
+        raise ValueError(f"x must be [M, {H}], got {tuple(x.shape)}")
+    if x.dtype != gs.dtype or x.dtype != ds.dtype:
+        raise ValueError(f"activation dtype {x.dtype} does not match the scale dtypes")
+    if activation not in _GATED_ACT:
+        raise ValueError(f"unsupported activation {activation!r}")
+    if gw.device != x.device or dw.device != x.device:
+        raise ValueError("x and the repacked weights must be on one device")
+    _check_mlp_counters(counters, x.device)
+    _check_out(out, (x.shape[0], H), x.dtype, x.device)
+
+
 @torch.library.custom_op(f"{NAMESPACE}::awq_gated_mlp_out", mutates_args=("counters", "out"), device_types="cuda")
 def _mlp_out_op(x: torch.Tensor, gw: torch.Tensor, gs: torch.Tensor, gz: torch.Tensor, dw: torch.Tensor,
                 ds: torch.Tensor, dz: torch.Tensor, counters: torch.Tensor, out: torch.Tensor, H: int, I: int, G: int,
                 activation: str, polls: int) -> None:
-    _mlp_launch(x, gw, gs, gz, dw, ds, dz, counters, out, H, I, G, activation, polls)
+    _check_mlp_op(x, gw, gs, gz, dw, ds, dz, counters, out, H, I, G, activation)
+    _mlp_launch(_aligned(x), gw, gs, gz, dw, ds, dz, counters, out, H, I, G, activation, polls)
 
 
 @_mlp_out_op.register_fake
@@ -775,9 +800,7 @@ def gated_mlp(x: torch.Tensor, gate_up: Repacked, down: Repacked, H: int, I: int
     for t in (gate_up.w, gate_up.s, gate_up.z, down.w, down.s, down.z):
         if t.device != dev:
             raise ValueError("x and the repacked weights must be on one device")
-    if counters.dtype != torch.int32 or counters.device != dev or not counters.is_contiguous() \
-            or counters.numel() * 4 < _lib.AWQ_MLP_COUNTER_BYTES or counters.data_ptr() % 128:
-        raise ValueError("counters must be make_mlp_counters(device)")
+    _check_mlp_counters(counters, dev)
     G = resolve_group_size(group_size, H)
     M = x.shape[0]
     x = _aligned(x)
@@ -785,8 +808,12 @@ def gated_mlp(x: torch.Tensor, gate_up: Repacked, down: Repacked, H: int, I: int
         out = torch.empty((M, H), dtype=x.dtype, device=dev)
     else:
         _check_out(out, (M, H), x.dtype, dev)
-    torch.ops.sglite_awq.awq_gated_mlp_out(x, gate_up.w, gate_up.s, gate_up.z, down.w, down.s, down.z, counters,
-                                           out, H, I, G, activation, -1 if polls is None else int(polls))
+    args = (x, gate_up.w, gate_up.s, gate_up.z, down.w, down.s, down.z, counters, out, H, I, G, activation,
+            -1 if polls is None else int(polls))
+    if _undispatched(*args[:9]):
+        _mlp_launch(*args)
+    else:
+        torch.ops.sglite_awq.awq_gated_mlp_out(*args)
     return out
 
 
@@ -1821,6 +1848,13 @@ def make_lora_stack(num_adapters: int, max_rank: int, K: int, parts: Sequence[in
                      torch.zeros(num_adapters, dtype=torch.int32, device=device), tuple(int(n) for n in parts))
 
 
+def _check_lora_ids(adapter_ids: torch.Tensor, num_adapters: int) -> None:
+    if adapter_ids.dim() != 1 or adapter_ids.dtype != torch.int32:
+        raise ValueError(f"adapter_ids must be int32 [M], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
+    if not 1 <= num_adapters <= _lib.AWQ_LORA_MAX_ADAPTERS:
+        raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
+
+
 def _lora_route_launch(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = adapter_ids.device
     if dev.index is not None and torch._C._cuda_getDevice() != dev.index:
@@ -1841,7 +1875,8 @@ def _lora_route_launch(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[to
 
 @torch.library.custom_op(f"{NAMESPACE}::awq_lora_route", mutates_args=(), device_types="cuda")
 def _lora_route_op(adapter_ids: torch.Tensor, num_adapters: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    return _lora_route_launch(adapter_ids, num_adapters)
+    _check_lora_ids(adapter_ids, num_adapters)
+    return _lora_route_launch(_aligned(adapter_ids, 4), num_adapters)
 
 
 @_lora_route_op.register_fake
@@ -1856,10 +1891,7 @@ def lora_route(adapter_ids: torch.Tensor, num_adapters: int) -> LoraBatch:
     ``adapter_ids`` [M] int32 names each row's slot; an id outside ``[0, num_adapters)``, as -1, names none.  The
     batch refers to them: they stay as they are until its last use.  For few rows nothing is launched, beyond that
     one kernel sorts them."""
-    if adapter_ids.dim() != 1 or adapter_ids.dtype != torch.int32:
-        raise ValueError(f"adapter_ids must be int32 [M], got {adapter_ids.dtype} {tuple(adapter_ids.shape)}")
-    if not 1 <= num_adapters <= _lib.AWQ_LORA_MAX_ADAPTERS:
-        raise ValueError(f"num_adapters must be in [1, {_lib.AWQ_LORA_MAX_ADAPTERS}], got {num_adapters}")
+    _check_lora_ids(adapter_ids, num_adapters)
     _require_cuda(adapter_ids)
     ids = _aligned(adapter_ids, 4)
     if _lora_unsorted(ids.numel()):
@@ -1897,9 +1929,10 @@ def _lora_launch(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
 def _lora_add_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
                  ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
                  block_adapters: Optional[torch.Tensor], parts: List[int], activation: str) -> torch.Tensor:
-    act = _ACT_CODE[_ACT_NAME[activation]]
+    act = _check_lora_op(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, parts, activation)
     out = torch.empty((y.shape[0], y.shape[1] // 2 if act else y.shape[1]), dtype=y.dtype, device=y.device)
-    _lora_launch(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, out, parts, act)
+    _lora_launch(_aligned(y), _aligned(x), a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, out, parts,
+                 act)
     return out
 
 
@@ -1912,7 +1945,11 @@ def _(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, parts
 def _lora_add_inplace_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
                          ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
                          block_adapters: Optional[torch.Tensor], parts: List[int]) -> None:
-    _lora_launch(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, y, parts, 0)
+    _check_lora_op(y, x, a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, parts, "none")
+    _check_out(y, tuple(y.shape), y.dtype, y.device, "y")
+    if _overlap(y, x):
+        raise ValueError("y must not share memory with x")
+    _lora_launch(y, _aligned(x), a, b, scaling, ranks, adapter_ids, sorted_ids, block_adapters, y, parts, 0)
 
 
 @_lora_add_inplace_op.register_fake
@@ -1965,6 +2002,17 @@ def _check_lora(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraB
         if P != 2 or stack.parts[0] != stack.parts[1]:
             raise ValueError(f"an activation needs two equal parts, gate and up, got {stack.parts}")
     _require_cuda(y, x, a, b, stack.scaling, stack.ranks, batch.adapter_ids)
+
+
+def _check_lora_op(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scaling: torch.Tensor,
+                   ranks: torch.Tensor, adapter_ids: torch.Tensor, sorted_ids: Optional[torch.Tensor],
+                   block_adapters: Optional[torch.Tensor], parts: Sequence[int], activation: str) -> int:
+    """What the registered ops read and write; the activation's code."""
+    if activation not in _ACT_NAME:
+        raise ValueError(f"unsupported activation {activation!r}")
+    batch = LoraBatch(adapter_ids, sorted_ids, block_adapters, b.shape[0] if b.dim() else 0)
+    _check_lora(y, x, LoraStack(a, b, scaling, ranks, tuple(parts)), batch, _ACT_NAME[activation])
+    return _ACT_CODE[_ACT_NAME[activation]]
 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatch, activation: Optional[str] = None,

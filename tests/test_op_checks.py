@@ -147,6 +147,63 @@ def test_sum_and_stack_checks():
             ops._check_expert_stacks(*bad)
 
 
+def mlp(dev, I=384):
+    """The one-launch block's arguments, K being its hidden size."""
+    empty, other = zeros(dev), OTHER[dev]
+
+    def layout(k, n):
+        return (empty((n + 15) // 16 * ((k + 127) // 128) * 256, dtype=I32), empty((n + 15) // 16, k // G, 16),
+                empty((n + 15) // 16, k // G, dtype=I64))
+    gate, down = layout(K, 2 * I), layout(I, K)
+    ok = dict(x=empty(M, K), **dict(zip(("gw", "gs", "gz"), gate)), **dict(zip(("dw", "ds", "dz"), down)),
+              counters=ops.make_mlp_counters(torch.device(dev)), out=empty(M, K), H=K, I=I, G=G, activation="silu")
+    return ok, [{name: ok[name].reshape(-1)[:-1]} for name in ("gw", "gs", "gz", "dw", "ds", "dz")] + [
+        dict(x=empty(M, K - 8)), dict(x=empty(M, K).bfloat16()), dict(gw=ok["gw"].long()), dict(dz=ok["dz"].int()),
+        dict(dw=ok["dw"].to(other)), dict(counters=ok["counters"][:-32]), dict(counters=ok["counters"].long()),
+        dict(counters=ok["counters"].to(other)), dict(out=empty(M - 1, K)), dict(out=empty(M, 2 * K)[:, ::2]),
+        dict(out=empty(M, K).bfloat16()), dict(out=ok["out"].to(other)), dict(H=2 * K), dict(I=2 * I), dict(G=64),
+        dict(activation="relu")]
+
+
+def lora(dev, inplace, L=3, R=8):
+    empty, other = zeros(dev), OTHER[dev]
+    ok = dict(y=empty(M, N), x=empty(M, K), a=empty(L, 2 * R, K), b=empty(L, N, R), scaling=empty(L, dtype=torch.float32),
+              ranks=empty(L, dtype=I32), adapter_ids=empty(M, dtype=I32), sorted_ids=None, block_adapters=None,
+              parts=[N // 2, N // 2])
+    tables = dict(sorted_ids=torch.full((M + 15 * (L + 1),), M, dtype=I32, device=dev),
+                  block_adapters=torch.full((M // 16 + L + 2,), L, dtype=I32, device=dev))
+    bad = [dict(y=empty(M, N - 8)), dict(y=empty(M - 1, N)), dict(x=empty(M, K - 8)), dict(x=empty(M, K).bfloat16()),
+           dict(a=empty(L, 2 * R, K - 8)), dict(a=empty(L - 1, 2 * R, K)), dict(b=empty(L, N, 2 * R)), dict(b=empty()),
+           dict(a=ok["a"].to(other)), dict(scaling=empty(L)), dict(scaling=empty(L - 1, dtype=torch.float32)),
+           dict(ranks=ok["ranks"].long()), dict(ranks=ok["ranks"][:-1]), dict(adapter_ids=ok["adapter_ids"][:-1]),
+           dict(adapter_ids=ok["adapter_ids"].long()), dict(adapter_ids=ok["adapter_ids"].to(other)),
+           dict(sorted_ids=tables["sorted_ids"]), {**tables, "sorted_ids": tables["sorted_ids"][:-1]},
+           {**tables, "block_adapters": tables["block_adapters"][:1]}, dict(parts=[N]), dict(parts=[N // 2, N // 2 - 8])]
+    if inplace:
+        return ok, bad + [dict(y=empty(M, 2 * N)[:, ::2])]
+    return dict(ok, activation="none"), bad + [dict(activation="relu"), dict(parts=[N - 8, 8], activation="silu")]
+
+
+def test_mlp_checks():
+    ok, bad = mlp("cpu")
+    ops._check_mlp_op(**ok)
+    for change in bad:
+        with pytest.raises(ValueError):
+            ops._check_mlp_op(**{**ok, **change})
+
+
+def test_lora_checks(monkeypatch):
+    monkeypatch.setattr(ops, "_require_cuda", lambda *ts: None)
+    ok, bad = lora("cpu", False)
+    ops._check_lora_op(**ok)
+    for change in bad:
+        with pytest.raises(ValueError):
+            ops._check_lora_op(**{**ok, **change})
+    for ids, n in ((torch.zeros(M, dtype=I64), 3), (torch.zeros(M, 1, dtype=I32), 3), (torch.zeros(M, dtype=I32), 0)):
+        with pytest.raises(ValueError):
+            ops._check_lora_ids(ids, n)
+
+
 def refused_by_the_op(name, ok, bad):
     getattr(OPS, name)(**ok)
     for change in bad:
@@ -159,6 +216,33 @@ def refused_by_the_op(name, ok, bad):
 @pytest.mark.parametrize("name", GROUPED)
 def test_grouped_ops(name):
     refused_by_the_op(name, *grouped(name, "cuda"))
+
+
+@pytest.mark.gpu
+def test_mlp_op():
+    ok, bad = mlp("cuda", 128)
+    if ops.gated_mlp_plan(M, K, 128, G) is None:  # then the C ABI refuses the shape, after the checks
+        with pytest.raises(RuntimeError):
+            OPS.awq_gated_mlp_out(**ok, polls=-1)
+    else:
+        OPS.awq_gated_mlp_out(**ok, polls=-1)
+    for change in bad:
+        with pytest.raises(ValueError):
+            OPS.awq_gated_mlp_out(**{**ok, **change}, polls=-1)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_lora_ops():
+    refused_by_the_op("awq_lora_add", *lora("cuda", False))
+    refused_by_the_op("awq_lora_add_", *lora("cuda", True))
+    for ids, n in ((torch.zeros(M, dtype=I64), 3), (torch.zeros(M, 1, dtype=I32), 3), (torch.zeros(M, dtype=I32), 0)):
+        with pytest.raises(ValueError):
+            OPS.awq_lora_route(ids.cuda(), n)
+    ids = torch.arange(40, dtype=I32, device="cuda") % 4 - 1
+    want = ops.lora_route(ids, 3)
+    got = OPS.awq_lora_route(ids.repeat_interleave(2)[::2], 3)  # a strided one is copied
+    assert torch.equal(got[0], want.sorted_ids)
 
 
 @pytest.mark.gpu
