@@ -42,7 +42,7 @@ enum {
   AWQ_STATUS_WORKSPACE = -4         /* workspace missing or too small          */
 };
 
-enum { AWQ_DTYPE_FP16 = 0, AWQ_DTYPE_BF16 = 1, AWQ_DTYPE_FP32 = 2 /* router logits only */ };
+enum { AWQ_DTYPE_FP16 = 0, AWQ_DTYPE_BF16 = 1, AWQ_DTYPE_FP32 = 2 /* router logits, MXFP4 blocks */ };
 
 /* Message of the last failed call on this thread ("" if none). */
 const char* awq_last_error(void);
@@ -64,7 +64,8 @@ const char* awq_version(void);
  * Calls added since without a change to an existing one keep the revision
  * (awq_moe_route with AWQ_DTYPE_FP32, awq_gemm_plan_ring, awq_gemm_launch_info,
  * the AWQ_PLAN_RING knobs, awq_moe_dense_gemm, awq_lora_route,
- * awq_lora_workspace_bytes, awq_lora_add): a caller that binds them by name finds out there.
+ * awq_lora_workspace_bytes, awq_lora_add, all awq_mx4_*): a caller that binds them by name
+ * finds out there.
  * No counterpart in the reference (its kernels are Python and Triton). */
 #define AWQ_ABI_VERSION 4
 int awq_abi_version(void);
@@ -453,9 +454,10 @@ int awq_moe_sum_reduce(const void* in, void* out, int64_t T, int64_t topk, int64
  *   mul_routed_weight each sum times topk_weights[r] first.  Rows that the
  *   sorted table does not hold are not written
  * K % 32 == 0, N % 8 == 0, with an activation I % 32 == 0; x, a, w, bias, out and
- * ws 16-byte aligned.  Limits: K, N and M below 2^24, E <= 512, x below 2^34
- * elements, the routed activation rows below 2 GiB; a call repacks at most 2^24
- * tiles of 16 rows by 512 k. */
+ * ws 16-byte aligned.  Limits: K, N and M below 2^24, E <= 512, top_k below 2^31,
+ * x below 2^34 elements (a product's with K rounded up to 512), the routed
+ * activation rows below 2 GiB, an experts' launch at most 2^22 workgroups of 128
+ * sorted rows by 256 columns; a call repacks below 2^24 tiles of 16 rows by 512 k. */
 int awq_mx4_quantize(const void* x, int dtype, int64_t rows, int64_t K, void* codes, void* scales,
                      awq_stream_t stream);
 int awq_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t K, int dtype, void* out,

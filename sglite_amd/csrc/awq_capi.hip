@@ -888,7 +888,7 @@ int check_mx4_workspace(const Mx4Plan& p, const void* ws, int64_t ws_bytes, cons
 // Rows that a launch of their own quantises: its threads are counted in 32 bits.
 int check_mx4_rows(int64_t rows, int64_t K, const char* who) {
   if (rows >= (int64_t(1) << 24) || rows * mx4_ksteps(K) >= (int64_t(1) << 25))
-    return fail(AWQ_STATUS_UNSUPPORTED, "%s: x must have below 2^24 rows and 2^34 elements", who);
+    return fail(AWQ_STATUS_UNSUPPORTED, "%s: x must have below 2^24 rows and, K rounded up to 512, 2^34 elements", who);
   return AWQ_STATUS_OK;
 }
 

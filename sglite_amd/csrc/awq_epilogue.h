@@ -39,8 +39,9 @@ __device__ __forceinline__ float gated_act(int act, float g) {
 // the relative error stays below 2^-17, and what lies below g 2^-126 may be
 // zero: far below the 16-bit rounding that follows), where a kernel is bound by
 // reading: silu takes 5 vector operations instead of about 25.  It stands in the
-// adapters' kernels and the dense experts' tiles; dense_rows_kernel, which has
-// few outputs, calls the other one.  A row's fp32 value before the rounding thus
+// adapters' kernels and the tiles of dense and MXFP4 experts and of MXFP4 linears;
+// dense_rows_kernel, mx4_rows_kernel and mx4_expert_rows_kernel, which have few
+// outputs, call the other one.  A row's fp32 value before the rounding thus
 // differs in its last bits with the size of its batch, as its sums' order does.
 __device__ __forceinline__ float gated_act_fast(int act, float g) {
   if (act != kActSilu) return gated_act(act, g);

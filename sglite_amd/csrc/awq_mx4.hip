@@ -137,7 +137,9 @@ __global__ __launch_bounds__(kMxThreads) void mx4_dequantize_kernel(const uint32
 __device__ __forceinline__ int tile_column(int t, int i) { return 32 * (t >> 1) + 8 * (i >> 2) + 4 * (t & 1) + (i & 3); }
 
 // Weights between a checkpoint's order and the tiles, one 16-byte block a thread;
-// BACK restores the former.
+// BACK restores the former.  Bound by memory: 28672 x 4096 in 24 us, a stack of 256
+// weights 4096 x 4096 in 860 us, 5.2 to 5.3 TB/s read and written (a copy of its
+// codes alone takes as long); back 22 and 1150 us, 5.6 and 4.0 TB/s.
 template <bool BACK>
 __global__ __launch_bounds__(kMxThreads) void mx4_repack_kernel(u32x4* codes, uint8_t* scales, u32x4* w, uint8_t* s,
                                                                 int64_t total, int N, int KB, int NT, int KT, int KS) {

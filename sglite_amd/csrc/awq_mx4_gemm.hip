@@ -325,12 +325,13 @@ constexpr int kMxStage = kMxCodes + kMxTileM;           // and its scales, 16 by
 // NTW = 4: two stages, weights two k-tiles ahead, two workgroups a CU.  NTW = 2,
 // for grids that leave CUs idle: three stages and weights six k-tiles ahead.
 //
-// 8192 rows of Llama-3-8B's gate/up with silu take 450 to 480 us without the
-// quantising launch, 4.0 to 4.3 PFLOP/s; the MFMA alone, its operands in registers,
-// reaches 6.2 on random data (9.0 on zeros: power).  MFMAs are busy 53 % of the
-// time there, the L2 gives 12 TB/s.  Tiles of 256 x 256 by eight waves, both
-// operands through a ring of LDS stages, take a third less from the L2 and were no
-// faster (526 against 509 us); neither were row operands further ahead, or
+// 8192 rows of Llama-3-8B's gate/up with silu take 470 to 500 us between the
+// layer's other launches, 3.9 to 4.1 PFLOP/s (qkv and o 3.5 to 3.7, down 4.5 to
+// 4.7); the MFMA alone, its operands in registers, reaches 6.2 on random data (9.0
+// on zeros: power).  MFMAs are busy 53 % of the time there, the L2 gives 12 TB/s.
+// Tiles of 256 x 256 by eight waves, both operands through a ring of LDS stages,
+// take a third less from the L2 and were no faster (526 us, when these took 509);
+// neither were row operands further ahead, or
 // workgroups of one CU on one column group.  E = 128, H = 2048, I = 768 top-8 at
 // 4096 tokens: 93 and 86 us, MFMAs busy 20 %: four and two stages a tile, between
 // its start and its scattered rows' stores.
@@ -752,7 +753,8 @@ Mx4Plan plan_mx4_moe(int64_t num_routed, int64_t top_k, int64_t E, int64_t N, in
   // From three rows an expert the tiles are ahead, although they quantise in a
   // launch of their own (us of both products, row by row / by tiles: E = 128, H =
   // 2048, I = 768 top-8 at 24 tokens 64 / 66, 32 70 / 75, 48 78 / 77, 96 87 / 82; E =
-  // 16, H = 4096, I = 1408 top-2 at 8 tokens 31 / 37, at 24 45 / 42).
+  // 16, H = 4096, I = 1408 top-2 at 8 tokens 31 / 37, at 24 45 / 42).  Fewer and
+  // wider experts, of whose tiles there are less than CUs, were not measured.
   p.pre = num_routed > 2 * E;
   p.ws_bytes = p.pre ? expert_codes(rows, K) + expert_scales(rows, K) : 0;
   if (p.pre) {
