@@ -96,6 +96,13 @@ def _undispatched(*tensors: Optional[torch.Tensor]) -> bool:
             and torch.autograd.forward_ad._current_level < 0 and not torch._C._autograd._profiler_enabled())
 
 
+def _written(t: torch.Tensor) -> torch.Tensor:
+    """A caller's tensor that a launch writes without the dispatcher: autograd, which may hold it for a backward pass,
+    has to see the change as it sees a registered op's."""
+    torch._C._increment_version((t,))
+    return t
+
+
 def resolve_group_size(group_size: int, K: int) -> int:
     return K if group_size == -1 else group_size
 
@@ -613,8 +620,7 @@ def gemm(x: torch.Tensor, r: Repacked, K: int, N: int, group_size: int, bias: Op
     if out is not None:
         _check_out(out, (M, ncols), x.dtype, dev)
     if _undispatched(x, r.w, r.s, r.z, bias, counters, out):
-        if out is None:
-            out = torch.empty((M, ncols), dtype=x.dtype, device=dev)
+        out = torch.empty((M, ncols), dtype=x.dtype, device=dev) if out is None else _written(out)
         _gemm_launch(x, r.w, r.s, r.z, bias, counters, out, K, N, G, 0 if activation is None else _GATED_ACT[activation])
         return out
     if activation is None:
@@ -812,6 +818,7 @@ def gated_mlp(x: torch.Tensor, gate_up: Repacked, down: Repacked, H: int, I: int
             -1 if polls is None else int(polls))
     if _undispatched(*args[:9]):
         _mlp_launch(*args)
+        _written(out)
     else:
         torch.ops.sglite_awq.awq_gated_mlp_out(*args)
     return out
@@ -1154,6 +1161,7 @@ def moe_gemm(a: torch.Tensor, experts: RepackedExperts, K: int, N: int, group_si
     if _undispatched(*args[:8]):
         act = _check_moe_gemm_op(*args)
         _moe_gemm_launch(*args[:13], act, args[14])
+        _written(out)
     else:
         torch.ops.sglite_awq.awq_moe_w4a16_gemm(*args)
     return out
@@ -1254,7 +1262,7 @@ def moe_dense_gemm(a: torch.Tensor, w: torch.Tensor, align: MoeAlignment, topk_w
     if _undispatched(a, w, topk_weights, out, align.sorted_ids, align.expert_offsets):
         _moe_dense_launch(a, w, align.sorted_ids, align.expert_offsets, topk_weights, out, num_routed, top_k,
                           _ACT_CODE[activation], mul_routed_weight)
-        return out
+        return _written(out)
     torch.ops.sglite_awq.awq_moe_dense_gemm(a, w, align.sorted_ids, align.expert_offsets, topk_weights, out,
                                             num_routed, top_k, "none" if activation is None else activation,
                                             bool(mul_routed_weight))
@@ -1296,7 +1304,7 @@ def moe_sum_reduce(inp: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
     _check_moe_sum(inp, out)
     if _undispatched(inp, out):
         _moe_sum_launch(inp, out)
-        return out
+        return _written(out)
     torch.ops.sglite_awq.awq_moe_sum_reduce(inp, out)
     return out
 
@@ -1677,6 +1685,8 @@ def mx4_gemm(x: torch.Tensor, weight: Mx4Weight, bias: Optional[torch.Tensor] = 
     if _undispatched(x, w, s, bias, out):
         if out is None:
             out = torch.empty((x.shape[0], N if activation is None else N // 2), dtype=x.dtype, device=x.device)
+        else:
+            _written(out)
         _mx4_gemm_launch(x, w, s, bias, out, N, K, _ACT_CODE[activation])
         return out
     name = "none" if activation is None else activation
@@ -1777,7 +1787,7 @@ def mx4_moe_gemm(a: torch.Tensor, experts: Mx4Weight, align: MoeAlignment, topk_
     if _undispatched(a, w, s, topk_weights, out, align.sorted_ids, align.expert_offsets):
         _mx4_moe_launch(a, w, s, align.sorted_ids, align.expert_offsets, topk_weights, out, N, K, num_routed, top_k,
                         _ACT_CODE[activation], mul_routed_weight)
-        return out
+        return _written(out)
     torch.ops.sglite_awq.awq_mx4_moe_gemm(a, w, s, align.sorted_ids, align.expert_offsets, topk_weights, out, N, K,
                                           num_routed, top_k, "none" if activation is None else activation,
                                           bool(mul_routed_weight))
@@ -2040,6 +2050,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: LoraStack, batch: LoraBatc
             out.copy_(y)
         if _undispatched(out, x, a, b, scaling, ranks, *tables):
             _lora_launch(out, x, a, b, scaling, ranks, *tables, out, stack.parts, 0)
+            _written(out)
         else:
             torch.ops.sglite_awq.awq_lora_add_(out, x, a, b, scaling, ranks, *tables, list(stack.parts))
         return out

@@ -17,6 +17,13 @@ def repacked(empty):
 OTHER = {"cpu": "meta", "cuda": "cpu"}  # another device than the kernels'
 
 
+def on_lines(t):
+    """The same counters at a multiple of 128 bytes, which the host's allocator does not promise."""
+    big = torch.zeros(t.numel() + 32, dtype=t.dtype, device=t.device)
+    at = -big.data_ptr() % 128 // 4
+    return big[at:at + t.numel()]
+
+
 def zeros(dev):
     return lambda *shape, dtype=H, device=dev: torch.zeros(shape, dtype=dtype, device=device)
 
@@ -34,7 +41,7 @@ def linear(name, dev):
     bad = bad_weights(ok, empty, other)
     if name in ("awq_unrepack_cdna4", "awq_dequant_repacked"):
         return ok, bad
-    ok.update(x=empty(M, K), bias=empty(N), counters=ops.make_counters(N, torch.device(dev)))
+    ok.update(x=empty(M, K), bias=empty(N), counters=on_lines(ops.make_counters(N, torch.device(dev))))
     bad += [dict(x=empty(M, K - 8)), dict(x=empty(K)), dict(x=empty(M, K, dtype=torch.bfloat16)), dict(bias=empty(N - 8)),
             dict(bias=empty(N, dtype=torch.float32)), dict(bias=empty(N, device=other)),
             dict(counters=ok["counters"].long()), dict(counters=ok["counters"][::2]),
@@ -156,7 +163,7 @@ def mlp(dev, I=384):
                 empty((n + 15) // 16, k // G, dtype=I64))
     gate, down = layout(K, 2 * I), layout(I, K)
     ok = dict(x=empty(M, K), **dict(zip(("gw", "gs", "gz"), gate)), **dict(zip(("dw", "ds", "dz"), down)),
-              counters=ops.make_mlp_counters(torch.device(dev)), out=empty(M, K), H=K, I=I, G=G, activation="silu")
+              counters=on_lines(ops.make_mlp_counters(torch.device(dev))), out=empty(M, K), H=K, I=I, G=G, activation="silu")
     return ok, [{name: ok[name].reshape(-1)[:-1]} for name in ("gw", "gs", "gz", "dw", "ds", "dz")] + [
         dict(x=empty(M, K - 8)), dict(x=empty(M, K).bfloat16()), dict(gw=ok["gw"].long()), dict(dz=ok["dz"].int()),
         dict(dw=ok["dw"].to(other)), dict(counters=ok["counters"][:-32]), dict(counters=ok["counters"].long()),
